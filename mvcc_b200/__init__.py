@@ -58,6 +58,14 @@ class MoeAttnWeights(ctypes.Structure):
                [("theta", ctypes.c_float), ("eps", ctypes.c_float)]
 
 
+class MoePagedCache(ctypes.Structure):
+    """ctypes mirror of `moe_paged_cache` (include/moe_paged.h)."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "tables", "refs", "lens", "k_scale", "v_scale")] + \
+               [(n, ctypes.c_int32) for n in ("layers", "num_pages", "page", "Hkv", "D", "kv_type", "max_seqs",
+                                              "max_pages")]
+
+
 class MoeTrace(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("logits", "idx", "wts", "routed", "sout", "gate", "sorted",
                                                "offsets")]
@@ -71,7 +79,12 @@ class MoeStats(ctypes.Structure):
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
+_L = ctypes.c_int64
+_Z = ctypes.c_size_t
+_F = ctypes.c_float
 _W = ctypes.POINTER(MoeLayerWeights)
+_A = ctypes.POINTER(MoeAttnWeights)
+_C = ctypes.POINTER(MoePagedCache)
 _SIGS = {
     "moe_check_shape": (_I, [_W]),
     "moe_workspace_bytes": (ctypes.c_size_t, [_W, _I]),
@@ -120,6 +133,23 @@ _SIGS = {
     "moe_rmsnorm": (_I, [_P, _P, _P, _I, _I, ctypes.c_float, _P]),
     "moe_lm_head_workspace_bytes": (ctypes.c_size_t, [_I, _I]),
     "moe_lm_head_argmax": (_I, [_P, _P, _I, _I, _P, _P, _P, ctypes.c_size_t, _P]),
+    # paged key-value cache, its attention and its pages (include/moe_paged.h)
+    "moe_paged_check": (_I, [_C]),
+    "moe_paged_workspace_bytes": (_Z, [_C, _I, _I, _I]),
+    "moe_paged_workspace_error": (_I, [_P, _Z, _P]),
+    "moe_paged_resize": (_I, [_C, _P, _P, _I, _P, _Z, _P]),
+    "moe_paged_fork": (_I, [_C, _P, _P, _I, _P, _Z, _P]),
+    "moe_paged_compact": (_I, [_C, _P, _Z, _P]),
+    "moe_paged_copy": (_I, [_C, _P, _P, _I, _P, _Z, _P]),
+    "moe_paged_append": (_I, [_C, _I, _P, _I, _I, _P, _I, _P, _P, _P, _I, _F, _P, _P, _Z, _P]),
+    "moe_paged_attend": (_I, [_C, _I, _P, _I, _I, _P, _I, _F, _P, _P, _Z, _P]),
+    "moe_attn_paged_workspace_bytes": (_Z, [_A, _C, _I, _I]),
+    "moe_attn_paged_forward_rms": (_I, [_A, _P, _P, _C, _I, _P, _I, _I, _P, _P, _P, _Z, _P]),
+    # logits, probabilities and the verification of drafts (include/moe_spec.h)
+    "moe_lm_head_logits": (_I, [_P, _P, _I, _I, _I, _P, _P]),
+    "moe_softmax_rows": (_I, [_P, _L, _I, _I, _P, _P, _L, _P]),
+    "moe_spec_workspace_bytes": (_Z, [_I, _I]),
+    "moe_spec_verify": (_I, [_P, _L, _P, _L, _P, _P, _P, _I, _I, _I, _P, _P, _P, _Z, _P]),
     # weight pack reader (include/moe_pack.h); the structures are declared in mvcc_b200/pack.py
     "moe_pack_open": (_P, [ctypes.c_char_p, ctypes.c_char_p, ctypes.c_size_t]),
     "moe_pack_close": (None, [_P]),

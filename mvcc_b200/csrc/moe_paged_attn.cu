@@ -1,0 +1,826 @@
+// moe_paged_attn.cu -- attention of a batch's new tokens over a paged key-value cache (moe_paged_attend,
+// include/moe_paged.h).
+//
+// o = sum_j softmax_j(scale q . k_j) v_j for the G = Hq / Hkv query heads and Tq new tokens that share a kv head: each
+// cached value is read once and used by G Tq rows, so up to 64 rows the call is bound by the cache's bytes.
+//
+// Work split: a unit is NG x KT keys of one (sequence, kv head, row block) job. Every CTA of a persistent grid counts
+// the batch's units itself (a scan over the lengths, which only the device knows) and takes an equal, contiguous share
+// of the flattened list, whatever the lengths: a long cache is split over many CTAs, many short ones share a CTA. A CTA
+// has partial results for its first and its last job at most; they go to the workspace as (max, sum, accumulator) and
+// paged_join_kernel merges each split job's parts in CTA order, so the result does not depend on timing. A job that
+// lies in one CTA is finished there. A job of n parts holds n - 1 of the borders between CTAs, so the join runs a CTA
+// a border, and those of one job share its rows.
+//
+// CTA: four consumer warps and a producer warp. The producer walks the CTA's tiles (KT keys of k and v each), reads
+// the page ids 32 at a time and fetches the tiles by TMA (boxes of 64 values x 16 or KT rows inside one page, 128-byte
+// swizzle) into a ring of NS slots, mbarrier-counted. Consumer warp (g, mt) holds 16 query rows as MMA fragments and
+// takes every NG-th tile: S = Q K^T, the running maximum and sum of the softmax, O += P V, all in registers; at a job's
+// end the NG warps of a row tile merge through shared memory.
+//
+// mma.sync and not tcgen05: with 16 to 64 rows a tcgen05.mma (at least 64 rows of the cache as M, and P through TMEM)
+// would leave its tensor core as idle as the register MMA does, and add two TMEM round trips to the softmax of each
+// tile; at 16 rows the register MMA needs under a third of the cycles that the tile's bytes take to arrive.
+#include <algorithm>
+#include <cstring>
+#include <mutex>
+
+#include <cuda.h>
+#include <cuda_fp8.h>
+
+#include "moe_paged.h"
+#include "moe_sync.cuh"
+
+namespace moe {
+namespace {
+
+constexpr int kWarps = 4;                      // consumer warps
+constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kSmemOne = 227 * 1024;           // shared memory of a CTA alone on its SM
+constexpr int kSmemTwo = 113 * 1024;           // of one of two
+
+struct PAttnArgs {
+  const uint16_t* q;
+  uint16_t* out;
+  const float* k_scale;  // of this layer, or null
+  const float* v_scale;
+  const int32_t* seqs;
+  const int32_t* tables;
+  const int32_t* lens;
+  int32_t* joins;  // [ctas][8]: the split job at the border before each CTA (parts = 0: none)
+  float* ml;       // [2 ctas][rows][2]
+  float* acc;      // [2 ctas][rows][D]
+  uint32_t* err;
+  int32_t B, Tq, Hq, Hkv, G, page, num_pages, max_seqs, max_pages, box_rows, row_blocks, rows, ctas;
+  float scale;
+};
+
+template <int D, bool F8>
+struct Cfg {
+  static constexpr int kEs = F8 ? 1 : 2;
+  static constexpr int kRow = D * kEs;                    // bytes of a cached row
+  static constexpr int kSegs = kRow / 128;                // 128-byte column segments of a tile
+  static constexpr int KT = D == 256 ? 16 : 32;           // keys of a tile
+  static constexpr int kSeg = KT * 128;                   // bytes of a segment
+  static constexpr int kTile = KT * kRow;                 // bytes of a k or v tile
+  static constexpr int kSlot = 2 * kTile;
+  static constexpr int kPerSm = D == 256 ? 1 : 2;         // CTAs an SM: registers (accumulator D / 2 a lane)
+  static constexpr int kMerge = 16 * (D + 8) * 4;         // bytes of one warp's partial in the merge buffer
+  static constexpr int kUnits = (kPagedMaxBatch + 1) * 4; // the scan of the units
+  static constexpr int kFixed = 1024 + ((2 * kMerge + kUnits + 127) & ~127) + 1024;
+  static constexpr int kFit = ((kPerSm == 1 ? kSmemOne : kSmemTwo) - kFixed) / kSlot;
+  static constexpr int NS = kFit > 24 ? 24 : kFit;        // ring slots
+  static constexpr int kSmem = kFixed + NS * kSlot;
+  static_assert(NS >= 4, "ring too short");
+};
+
+// D (16x8, fp32) += A (16x16) B (16x8); bf16 or f16 operands.
+template <bool F16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+// Two e4m3 values (the low 16 bits of w) as two f16, exactly.
+__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t w) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float quad_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* mbar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(mbar))
+      : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* mbar) {
+  asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(smem_u32(mbar)) : "memory");
+}
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
+
+// Keys of slot b: its sequence's length, 0 for an unused slot or a bad entry (recorded).
+__device__ __forceinline__ int slot_keys(const PAttnArgs& a, int b, int* seq) {
+  const int s = a.seqs[b];
+  *seq = 0;
+  if (s == -1) return 0;
+  if (s < 0 || s >= a.max_seqs) {
+    atomicOr(a.err, (uint32_t)MOE_ERR_SEQ_ID);
+    return 0;
+  }
+  *seq = s;
+  const int n = a.lens[s];
+  if (n < 0 || n > a.max_pages * a.page) {
+    atomicOr(a.err, (uint32_t)MOE_ERR_SEQ_ID);
+    return 0;
+  }
+  return n;
+}
+
+// The share of one CTA: units [u0, u1) of the flattened list, walked job by job.
+// joins[c]: parts, first CTA, whether its part is that CTA's second, slot, kv head, row block
+enum { JOIN_PARTS = 0, JOIN_FIRST, JOIN_SECOND, JOIN_SLOT, JOIN_HEAD, JOIN_BLOCK, JOIN_INTS = 8 };
+
+struct Walk {
+  int u, end, b, base, U;  // the next unit, the share's end; the slot it falls into, its first unit, its units a job
+  __device__ __forceinline__ void seek(const int* S, int B, int HR) {
+    if (u >= end) return;
+    int lo = 0, hi = B - 1;  // the last slot whose first unit is not behind u; empty slots before it are passed
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (S[mid] * HR <= u) lo = mid;
+      else hi = mid - 1;
+    }
+    b = lo;
+    base = S[b] * HR;
+    U = S[b + 1] - S[b];
+  }
+};
+
+template <int D, bool F8, int MT>
+__global__ void __launch_bounds__(kThreads, Cfg<D, F8>::kPerSm)
+    paged_attn_kernel(const __grid_constant__ PAttnArgs a, const __grid_constant__ CUtensorMap map_k,
+                      const __grid_constant__ CUtensorMap map_v) {
+  using C = Cfg<D, F8>;
+  constexpr int NG = kWarps / MT, KT = C::KT, UK = NG * KT, NS = C::NS;
+  constexpr int NT = D / 8;     // accumulator tiles of 8 columns
+  constexpr int KC = C::kRow / 16;  // 16-byte chunks of a cached row
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full[NS], empty[NS];
+  __shared__ int sm[32];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  float* merge = reinterpret_cast<float*>(ring + (size_t)NS * C::kSlot);
+  int* S = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(merge) + 2 * C::kMerge);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], MT);
+    }
+    mbar_fence_init();
+  }
+  pdl_wait();
+  pdl_launch_dependents();
+  // units of the slots before each slot
+  {
+    const int per = (a.B + kThreads - 1) / kThreads, b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
+    int sum = 0;
+    for (int b = b0; b < b1; ++b) {
+      int s;
+      const int u = (slot_keys(a, b, &s) + UK - 1) / UK;
+      S[b] = sum;
+      sum += u;
+    }
+    int total;
+    const int before = block_excl_scan(sum, sm, &total);
+    for (int b = b0; b < b1; ++b) S[b] += before;
+    if (tid == 0) S[a.B] = total;
+  }
+  __syncthreads();
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {  // no keys: zero rows
+    if (S[b + 1] != S[b]) continue;
+    uint4* o = reinterpret_cast<uint4*>(a.out + (int64_t)b * a.Tq * a.Hq * D);
+    for (int i = tid; i < a.Tq * a.Hq * (D / 8); i += kThreads) o[i] = make_uint4(0, 0, 0, 0);
+  }
+  const int HR = a.Hkv * a.row_blocks, total = S[a.B] * HR;
+  const int per = max(1, (total + a.ctas - 1) / a.ctas);
+  Walk w;
+  w.u = min(total, (int)blockIdx.x * per);
+  w.end = min(total, w.u + per);
+  if (tid == 0) {
+    int32_t* jn = a.joins + (int64_t)blockIdx.x * JOIN_INTS;
+    int parts = 0;
+    if (w.u < w.end) {
+      w.seek(S, a.B, HR);
+      const int job = (w.u - w.base) / w.U, u0 = w.base + job * w.U;
+      if (u0 < w.u) {
+        const int c0 = u0 / per;
+        parts = (u0 + w.U - 1) / per - c0 + 1;
+        jn[JOIN_FIRST] = c0;
+        jn[JOIN_SECOND] = u0 != c0 * per;
+        jn[JOIN_SLOT] = w.b;
+        jn[JOIN_HEAD] = job / a.row_blocks;
+        jn[JOIN_BLOCK] = job % a.row_blocks;
+      }
+    }
+    jn[JOIN_PARTS] = parts;
+  }
+
+  if (warp == kWarps) {
+    // ---------------------------------------------------------------- producer
+    const int none = a.num_pages * a.Hkv;  // a page that is not there: outside the map, reads as zero
+    const int nbox = KT / a.box_rows;
+    int i = 0;      // tiles so far
+    bool ok = true;
+    while (w.u < w.end && ok) {
+      w.seek(S, a.B, HR);
+      const int rel = w.u - w.base, job = rel / w.U, lu = rel - job * w.U, run = min(w.end - w.u, w.U - lu);
+      const int h = job / a.row_blocks;
+      int seq;
+      const int n = slot_keys(a, w.b, &seq);
+      const int32_t* row = a.tables + (int64_t)seq * a.max_pages;
+      const int key_end = (lu + run) * UK;
+      int z = 0, y = 0;
+      int fetched = lu * UK;  // first key whose box no lane holds yet
+      int held = 0;           // first key of lane 0's box
+      for (int key = lu * UK; key < key_end && ok; key += KT, ++i) {
+        const int slot = i % NS, turn = i / NS;
+        if (turn > 0) {
+          ok = bar_wait(&empty[slot], (turn - 1) & 1);
+          if (!ok) {
+            if (lane == 0) atomicOr(a.err, (uint32_t)MOE_ERR_TIMEOUT);
+            break;
+          }
+        }
+        if (key >= n) {  // a unit's tile behind the sequence's end
+          if (lane == 0) mbar_arrive(&full[slot]);
+          continue;
+        }
+        if (key >= fetched) {  // the next 32 boxes' pages
+          held = fetched;
+          const int k = fetched + lane * a.box_rows;
+          z = none;
+          y = 0;
+          if (k < n && k < key_end) {
+            const int pid = row[k / a.page];
+            if (pid >= 0 && pid < a.num_pages) z = pid * a.Hkv + h;
+            else atomicOr(a.err, (uint32_t)MOE_ERR_PAGE_ID);
+            y = k % a.page;
+          }
+          fetched += 32 * a.box_rows;
+        }
+        const int boxes = min(nbox, (n - key + a.box_rows - 1) / a.box_rows);
+        uint8_t* dst = ring + (size_t)slot * C::kSlot;
+        if (lane == 0) expect_tx(&full[slot], (uint32_t)(2 * boxes * a.box_rows * C::kRow));
+        __syncwarp();
+        for (int x = 0; x < boxes; ++x) {
+          const int from = (key - held) / a.box_rows + x;
+          const int bz = __shfl_sync(0xffffffffu, z, from), by = __shfl_sync(0xffffffffu, y, from);
+          if (lane < 2 * C::kSegs) {  // a lane a box: segment lane % kSegs of k or of v
+            const int sg = lane % C::kSegs, is_v = lane / C::kSegs;
+            tma_load_3d(dst + is_v * C::kTile + sg * C::kSeg + x * a.box_rows * 128, is_v ? &map_v : &map_k,
+                        sg * (128 / C::kEs), by, bz, &full[slot]);
+          }
+        }
+        __syncwarp();
+      }
+      w.u += run;
+    }
+    if (!ok)  // no copy may still be landing when the CTA exits
+      for (int j = max(0, i - NS); j < i; ++j) bar_wait(&full[j % NS], (j / NS) & 1);
+    return;
+  }
+
+  // ------------------------------------------------------------------ consumers
+  const int g = warp / MT, mt = warp % MT, qr = lane >> 2, ql = lane & 3;
+  const uint32_t ring32 = smem_u32(ring);
+  // this lane's row of an ldmatrix: k takes the four 8x8 blocks (keys 0-7, chunk c), (0-7, c+1), (8-15, c), (8-15, c+1);
+  // v, transposed, (0-7, c), (8-15, c), (0-7, c+1), (8-15, c+1)
+  const int kk_row = (lane >> 4) * 8 + (lane & 7), kk_ch = (lane >> 3) & 1;
+  const int vv_row = ((lane >> 3) & 1) * 8 + (lane & 7), vv_ch = lane >> 4;
+  auto chunk_addr = [&](uint32_t tile, int r, int ch) {
+    return tile + (ch >> 3) * C::kSeg + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+  };
+  int i0 = 0;   // tiles before this job
+  int njob = 0;
+  bool ok = true;
+  while (w.u < w.end) {
+    w.seek(S, a.B, HR);
+    const int rel = w.u - w.base, job = rel / w.U, lu = rel - job * w.U, run = min(w.end - w.u, w.U - lu);
+    const int h = job / a.row_blocks, rb = job - h * a.row_blocks;
+    int seq;
+    const int n = slot_keys(a, w.b, &seq);
+    const bool whole = lu == 0 && run == w.U;
+    // this lane's two rows: query row r of the kv head is token r / G, head h G + r % G
+    const int rA = rb * a.rows + mt * 16 + qr, rB = rA + 8, M = a.G * a.Tq;
+    const int tA = rA / a.G, tB = rB / a.G;
+    const int limA = rA < M ? n - a.Tq + tA + 1 : 0, limB = rB < M ? n - a.Tq + tB + 1 : 0;  // keys the row sees
+    auto q_row = [&](int r, int t) {
+      return a.q + (((int64_t)w.b * a.Tq + t) * a.Hq + h * a.G + (r - t * a.G)) * D;
+    };
+    uint32_t qf[D / 16][4];
+    float fA = a.scale * 1.4426950408889634f, fB;  // S in units of log 2
+    if (a.k_scale) fA *= a.k_scale[h];
+    fB = fA;
+    {
+      const uint16_t* pA = q_row(rA < M ? rA : 0, rA < M ? tA : 0);
+      const uint16_t* pB = q_row(rB < M ? rB : 0, rB < M ? tB : 0);
+      if constexpr (!F8) {
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          qf[c][0] = *reinterpret_cast<const uint32_t*>(pA + c * 16 + 2 * ql);
+          qf[c][1] = *reinterpret_cast<const uint32_t*>(pB + c * 16 + 2 * ql);
+          qf[c][2] = *reinterpret_cast<const uint32_t*>(pA + c * 16 + 8 + 2 * ql);
+          qf[c][3] = *reinterpret_cast<const uint32_t*>(pB + c * 16 + 8 + 2 * ql);
+        }
+      } else {
+        // e4m3 keys become f16, so the queries do too: scaled by the power of two that brings the row's largest into
+        // [1, 2) (exact), what then falls below f16's range is under 2^-24 of it. A 16-byte chunk of a key is one
+        // k-step here: lane ql holds its values 4 ql .. + 3, and the queries are laid out to match.
+        float mA = 0.f, mB = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          const uint2 xa = *reinterpret_cast<const uint2*>(pA + c * 16 + 4 * ql);
+          const uint2 xb = *reinterpret_cast<const uint2*>(pB + c * 16 + 4 * ql);
+          qf[c][0] = xa.x; qf[c][2] = xa.y; qf[c][1] = xb.x; qf[c][3] = xb.y;
+          mA = fmaxf(fmaxf(mA, fmaxf(fabsf(lo_bf(xa.x)), fabsf(hi_bf(xa.x)))), fmaxf(fabsf(lo_bf(xa.y)), fabsf(hi_bf(xa.y))));
+          mB = fmaxf(fmaxf(mB, fmaxf(fabsf(lo_bf(xb.x)), fabsf(hi_bf(xb.x)))), fmaxf(fabsf(lo_bf(xb.y)), fabsf(hi_bf(xb.y))));
+        }
+        // exponents in [1, 252], so that the factor and its inverse are normal numbers
+        const uint32_t eA = min(max(__float_as_uint(quad_max(mA)) >> 23, 1u), 252u);
+        const uint32_t eB = min(max(__float_as_uint(quad_max(mB)) >> 23, 1u), 252u);
+        const float iA = __uint_as_float((254u - eA) << 23), iB = __uint_as_float((254u - eB) << 23);
+        fA *= __uint_as_float(eA << 23);
+        fB *= __uint_as_float(eB << 23);
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+          qf[c][0] = pack2<true>(lo_bf(qf[c][0]) * iA, hi_bf(qf[c][0]) * iA);
+          qf[c][2] = pack2<true>(lo_bf(qf[c][2]) * iA, hi_bf(qf[c][2]) * iA);
+          qf[c][1] = pack2<true>(lo_bf(qf[c][1]) * iB, hi_bf(qf[c][1]) * iB);
+          qf[c][3] = pack2<true>(lo_bf(qf[c][3]) * iB, hi_bf(qf[c][3]) * iB);
+        }
+      }
+    }
+    float acc[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+    float mA = -INFINITY, mB = -INFINITY, lA = 0.f, lB = 0.f;
+
+    for (int r = 0; r < run; ++r) {
+      const int i = i0 + r * NG + g, slot = i % NS;
+      const int key0 = (lu + r) * UK + g * KT;
+      if (ok && !bar_wait(&full[slot], (i / NS) & 1)) {
+        ok = false;
+        if (lane == 0) atomicOr(a.err, (uint32_t)MOE_ERR_TIMEOUT);
+      }
+      if (ok && key0 < n) {
+        const uint32_t kt = ring32 + slot * C::kSlot, vt = kt + C::kTile;
+        // S = Q K^T, two chains of accumulators per 8 keys
+        float s[KT / 8][4], s2[KT / 8][4];
+#pragma unroll
+        for (int j = 0; j < KT / 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[j][e] = s2[j][e] = 0.f;
+#pragma unroll
+        for (int c = 0; c < KC; c += 2) {
+#pragma unroll
+          for (int j = 0; j < KT / 16; ++j) {
+            uint32_t kf[4];
+            ldsm4(kf, chunk_addr(kt, j * 16 + kk_row, c + kk_ch));
+            if constexpr (!F8) {
+              auto& d0 = (c / 2) & 1 ? s2[2 * j] : s[2 * j];
+              auto& d1 = (c / 2) & 1 ? s2[2 * j + 1] : s[2 * j + 1];
+              mma16816<false>(d0, qf[c / 2], kf[0], kf[1]);
+              mma16816<false>(d1, qf[c / 2], kf[2], kf[3]);
+            } else {
+              mma16816<true>(s[2 * j], qf[c], e4m3x2_f16x2(kf[0]), e4m3x2_f16x2(kf[0] >> 16));
+              mma16816<true>(s2[2 * j], qf[c + 1], e4m3x2_f16x2(kf[1]), e4m3x2_f16x2(kf[1] >> 16));
+              mma16816<true>(s[2 * j + 1], qf[c], e4m3x2_f16x2(kf[2]), e4m3x2_f16x2(kf[2] >> 16));
+              mma16816<true>(s2[2 * j + 1], qf[c + 1], e4m3x2_f16x2(kf[3]), e4m3x2_f16x2(kf[3] >> 16));
+            }
+          }
+        }
+        const bool masked = key0 + KT > n - a.Tq + 1;  // some row does not see all of the tile
+#pragma unroll
+        for (int j = 0; j < KT / 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[j][e] = (s[j][e] + s2[j][e]) * (e < 2 ? fA : fB);
+        if (masked) {
+#pragma unroll
+          for (int j = 0; j < KT / 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (key0 + j * 8 + 2 * ql + (e & 1) >= (e < 2 ? limA : limB)) s[j][e] = -INFINITY;
+        }
+        // running maximum and sum
+        float nA = mA, nB = mB;
+#pragma unroll
+        for (int j = 0; j < KT / 8; ++j) {
+          nA = fmaxf(nA, fmaxf(s[j][0], s[j][1]));
+          nB = fmaxf(nB, fmaxf(s[j][2], s[j][3]));
+        }
+        nA = quad_max(nA);
+        nB = quad_max(nB);
+        const float zA = nA == -INFINITY ? 0.f : nA, zB = nB == -INFINITY ? 0.f : nB;
+        if (__any_sync(0xffffffffu, nA != mA || nB != mB)) {
+          const float cA = ex2(mA - zA), cB = ex2(mB - zB);
+          lA *= cA;
+          lB *= cB;
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            acc[j][0] *= cA;
+            acc[j][1] *= cA;
+            acc[j][2] *= cB;
+            acc[j][3] *= cB;
+          }
+          mA = nA;
+          mB = nB;
+        }
+        // P in the cache's MMA type. The sums take the rounded weights, so that a row's weights still add up to one.
+        // f16 weights carry a common factor 2^15 (it cancels in the division): what a long row's many small weights
+        // lose below f16's normal range then stays under 2^-40 of the largest each.
+        constexpr float kLift = F8 ? 15.f : 0.f;
+        uint32_t pf[KT / 16][4];
+#pragma unroll
+        for (int j = 0; j < KT / 8; ++j) {
+          const float p0 = ex2(s[j][0] - zA + kLift), p1 = ex2(s[j][1] - zA + kLift);
+          const float p2 = ex2(s[j][2] - zB + kLift), p3 = ex2(s[j][3] - zB + kLift);
+          const uint32_t xA = pack2<F8>(p0, p1), xB = pack2<F8>(p2, p3);
+          pf[j >> 1][(j & 1) * 2] = xA;
+          pf[j >> 1][(j & 1) * 2 + 1] = xB;
+          if constexpr (F8) {
+            const float2 ra = __half22float2(*reinterpret_cast<const __half2*>(&xA));
+            const float2 rb2 = __half22float2(*reinterpret_cast<const __half2*>(&xB));
+            lA += ra.x + ra.y;
+            lB += rb2.x + rb2.y;
+          } else {
+            lA += lo_bf(xA) + hi_bf(xA);
+            lB += lo_bf(xB) + hi_bf(xB);
+          }
+        }
+        // O += P V. B fragments of the 16 keys from key0 + 16 ks, the columns of chunk pair c
+        auto pv = [&](auto&& keep, auto&& add) {
+#pragma unroll
+          for (int ks = 0; ks < KT / 16; ++ks) {
+#pragma unroll
+            for (int c = 0; c < KC; c += 2) {
+              uint32_t vf[4];
+              ldsm4t(vf, chunk_addr(vt, ks * 16 + vv_row, c + vv_ch));
+#pragma unroll
+              for (int e = 0; e < 4; ++e) vf[e] &= keep(ks, e & 1);
+              if constexpr (!F8) {
+                add(acc[c], pf[ks], vf[0], vf[1]);
+                add(acc[c + 1], pf[ks], vf[2], vf[3]);
+              } else {
+                // a 16-bit unit holds two columns of one key: even columns to one MMA, odd ones to the next
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const uint32_t b0 = __byte_perm(vf[2 * e], 0, 0x3120), b1 = __byte_perm(vf[2 * e + 1], 0, 0x3120);
+                  add(acc[2 * (c + e)], pf[ks], e4m3x2_f16x2(b0), e4m3x2_f16x2(b1));
+                  add(acc[2 * (c + e) + 1], pf[ks], e4m3x2_f16x2(b0 >> 16), e4m3x2_f16x2(b1 >> 16));
+                }
+              }
+            }
+          }
+        };
+        if (!masked) {
+          pv([](int, int) { return 0xffffffffu; },
+             [](float (&d)[4], const uint32_t (&p)[4], uint32_t b0, uint32_t b1) { mma16816<F8>(d, p, b0, b1); });
+        } else {
+          // Zero weights do not silence a NaN or an infinity, so what a row may not see is taken out of V itself: one
+          // pass per token of these rows, each over the keys that token sees, kept by its rows alone.
+          const int t0 = (rb * a.rows + mt * 16) / a.G, t1 = min(a.Tq - 1, (rb * a.rows + mt * 16 + 15) / a.G);
+          for (int t = t0; t <= t1; ++t) {
+            const int vis = n - a.Tq + t + 1 - key0;  // keys of the tile that token t sees
+            pv([&](int ks, int hi) {
+                 const int k = ks * 16 + hi * 8 + 2 * ql;
+                 return (k < vis ? 0xffffu : 0u) | (k + 1 < vis ? 0xffff0000u : 0u);
+               },
+               [&](float (&d)[4], const uint32_t (&p)[4], uint32_t b0, uint32_t b1) {
+                 float x[4] = {d[0], d[1], d[2], d[3]};
+                 mma16816<F8>(x, p, b0, b1);
+                 if (tA == t) {
+                   d[0] = x[0];
+                   d[1] = x[1];
+                 }
+                 if (tB == t) {
+                   d[2] = x[2];
+                   d[3] = x[3];
+                 }
+               });
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[slot]);
+    }
+    i0 += run * NG;
+    lA = quad_sum(lA);
+    lB = quad_sum(lB);
+
+    // merge the NG warps of a row tile: halves of them hand over until warp mt holds the sum
+#pragma unroll
+    for (int half = NG / 2; half >= 1; half >>= 1) {
+      float* buf = merge + (size_t)((g & (half - 1)) * MT + mt) * (C::kMerge / 4);
+      if (g >= half && g < 2 * half) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          *reinterpret_cast<float4*>(buf + (j * 32 + lane) * 4) = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
+        *reinterpret_cast<float4*>(buf + (NT * 32 + lane) * 4) = make_float4(mA, mB, lA, lB);
+      }
+      consumers_sync();
+      if (g < half) {
+        const float4 o = *reinterpret_cast<const float4*>(buf + (NT * 32 + lane) * 4);
+        const float nA = fmaxf(mA, o.x), nB = fmaxf(mB, o.y);
+        const float zA = nA == -INFINITY ? 0.f : nA, zB = nB == -INFINITY ? 0.f : nB;
+        const float cA = ex2(mA - zA), cB = ex2(mB - zB), dA = ex2(o.x - zA), dB = ex2(o.y - zB);
+        lA = lA * cA + o.z * dA;
+        lB = lB * cB + o.w * dB;
+        mA = nA;
+        mB = nB;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const float4 x = *reinterpret_cast<const float4*>(buf + (j * 32 + lane) * 4);
+          acc[j][0] = acc[j][0] * cA + x.x * dA;
+          acc[j][1] = acc[j][1] * cA + x.y * dA;
+          acc[j][2] = acc[j][2] * cB + x.z * dB;
+          acc[j][3] = acc[j][3] * cB + x.w * dB;
+        }
+      }
+      consumers_sync();
+    }
+    if (g == 0) {
+      // columns of accumulator tile j: bf16 8 j + 2 ql, + 1; e4m3 (tiles 2c, 2c + 1) 16 c + 4 ql + {0, 2}, + {1, 3}
+      if (whole) {
+        const float vs = a.v_scale ? a.v_scale[h] : 1.f;
+        // an empty row is zero; a NaN sum stays
+        const float dA = lA == 0.f ? 0.f : vs / lA, dB = lB == 0.f ? 0.f : vs / lB;
+        uint16_t* oA = a.out + (((int64_t)w.b * a.Tq + tA) * a.Hq + h * a.G + (rA - tA * a.G)) * D;
+        uint16_t* oB = a.out + (((int64_t)w.b * a.Tq + tB) * a.Hq + h * a.G + (rB - tB * a.G)) * D;
+        if constexpr (!F8) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            if (rA < M) *reinterpret_cast<uint32_t*>(oA + 8 * j + 2 * ql) = pack2<false>(acc[j][0] * dA, acc[j][1] * dA);
+            if (rB < M) *reinterpret_cast<uint32_t*>(oB + 8 * j + 2 * ql) = pack2<false>(acc[j][2] * dB, acc[j][3] * dB);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < NT; j += 2) {
+            if (rA < M)
+              *reinterpret_cast<uint2*>(oA + 8 * j + 4 * ql) =
+                  make_uint2(pack2<false>(acc[j][0] * dA, acc[j + 1][0] * dA), pack2<false>(acc[j][1] * dA, acc[j + 1][1] * dA));
+            if (rB < M)
+              *reinterpret_cast<uint2*>(oB + 8 * j + 4 * ql) =
+                  make_uint2(pack2<false>(acc[j][2] * dB, acc[j + 1][2] * dB), pack2<false>(acc[j][3] * dB, acc[j + 1][3] * dB));
+          }
+        }
+      } else {
+        const int64_t part = (int64_t)blockIdx.x * 2 + (njob > 0);
+        const int lrA = mt * 16 + qr, lrB = lrA + 8;
+        float* pA = a.acc + (part * a.rows + lrA) * D;
+        float* pB = a.acc + (part * a.rows + lrB) * D;
+        if (ql == 0) {
+          *reinterpret_cast<float2*>(a.ml + (part * a.rows + lrA) * 2) = make_float2(mA, lA);
+          *reinterpret_cast<float2*>(a.ml + (part * a.rows + lrB) * 2) = make_float2(mB, lB);
+        }
+        if constexpr (!F8) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            if (rA < M) *reinterpret_cast<float2*>(pA + 8 * j + 2 * ql) = make_float2(acc[j][0], acc[j][1]);
+            if (rB < M) *reinterpret_cast<float2*>(pB + 8 * j + 2 * ql) = make_float2(acc[j][2], acc[j][3]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < NT; j += 2) {
+            if (rA < M)
+              *reinterpret_cast<float4*>(pA + 8 * j + 4 * ql) = make_float4(acc[j][0], acc[j + 1][0], acc[j][1], acc[j + 1][1]);
+            if (rB < M)
+              *reinterpret_cast<float4*>(pB + 8 * j + 4 * ql) = make_float4(acc[j][2], acc[j + 1][2], acc[j][3], acc[j + 1][3]);
+          }
+        }
+      }
+    }
+    ++njob;
+    w.u += run;
+  }
+  if (!ok)  // no copy may still be landing when the CTA exits: this warp's last tiles once more
+    for (int i = i0 - NG + g; i >= 0 && i > i0 - NS; i -= NG) bar_wait(&full[i % NS], (i / NS) & 1);
+}
+
+// The join. Border c (before CTA c) inside a job of CTAs c0 .. c1 takes the (c - c0 - 1)-th of c1 - c0 equal shares of
+// the job's (row, four columns) items: their parts, one per CTA of the job in order, are weighted by 2^(m_i - m) and
+// added. A share of few items has its parts spread over the threads.
+constexpr int kJoinThreads = 256;
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PAttnArgs a) {
+  constexpr int kCols = D / 4, kMaxRows = 64;
+  // weights of the share's rows: rows * parts <= (64 / (parts - 1) + 2) * parts
+  __shared__ float wt[2 * kMaxRows + 2 * kPagedMaxCtas];
+  __shared__ float inv[kMaxRows];
+  __shared__ float4 red[kJoinThreads];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x + 1;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int32_t* jn = a.joins + (int64_t)c * JOIN_INTS;
+  const int parts = jn[JOIN_PARTS];
+  if (parts == 0) return;
+  const int c0 = jn[JOIN_FIRST], second = jn[JOIN_SECOND], b = jn[JOIN_SLOT], h = jn[JOIN_HEAD], rb = jn[JOIN_BLOCK];
+  const int rows = min(a.rows, a.G * a.Tq - rb * a.rows), all = rows * kCols, share = c - c0 - 1;
+  const int i0 = (int)((int64_t)all * share / (parts - 1)), i1 = (int)((int64_t)all * (share + 1) / (parts - 1));
+  if (i0 >= i1) return;
+  const int r0 = i0 / kCols, r1 = (i1 - 1) / kCols + 1;
+  auto part = [&](int i) { return (int64_t)(c0 + i) * 2 + (i == 0 ? second : 0); };
+  for (int r = r0 + warp; r < r1; r += kJoinThreads / 32) {
+    float m = -INFINITY;
+    for (int i = lane; i < parts; i += 32) m = fmaxf(m, a.ml[(part(i) * a.rows + r) * 2]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float z = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    for (int i = lane; i < parts; i += 32) {
+      const float2 x = *reinterpret_cast<const float2*>(a.ml + (part(i) * a.rows + r) * 2);
+      const float f = ex2(x.x - z);
+      wt[(r - r0) * parts + i] = f;
+      l = fmaf(x.y, f, l);
+    }
+    l = warp_sum(l);
+    if (lane == 0) inv[r - r0] = l == 0.f ? 0.f : (a.v_scale ? a.v_scale[h] : 1.f) / l;
+  }
+  __syncthreads();
+  // slices: the parts of an item over as many threads as the share leaves, a power of two up to 32
+  int slices = 1;
+  while (slices < 32 && (i1 - i0) * slices * 2 <= kJoinThreads) slices *= 2;
+  const int lanes = kJoinThreads / slices, sl = tid / lanes;
+  for (int base = i0; base < i1; base += lanes) {
+    const int it = base + tid % lanes;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (it < i1) {
+      const int r = it / kCols, col = it % kCols;
+      const float* w = wt + (r - r0) * parts;
+#pragma unroll 4
+      for (int i = sl; i < parts; i += slices) {
+        const float4 x = *reinterpret_cast<const float4*>(a.acc + (part(i) * a.rows + r) * D + col * 4);
+        const float f = w[i];
+        s.x = fmaf(x.x, f, s.x);
+        s.y = fmaf(x.y, f, s.y);
+        s.z = fmaf(x.z, f, s.z);
+        s.w = fmaf(x.w, f, s.w);
+      }
+    }
+    if (slices > 1) {  // one round only: the share fits the threads
+      red[tid] = s;
+      __syncthreads();
+      if (sl != 0) return;
+      for (int k = 1; k < slices; ++k) {
+        const float4 x = red[k * lanes + tid];
+        s.x += x.x;
+        s.y += x.y;
+        s.z += x.z;
+        s.w += x.w;
+      }
+    }
+    if (it < i1) {
+      const int r = it / kCols, col = it % kCols, q = rb * a.rows + r, t = q / a.G;
+      const float d = inv[r - r0];
+      *reinterpret_cast<uint2*>(a.out + (((int64_t)b * a.Tq + t) * a.Hq + h * a.G + (q - t * a.G)) * D + col * 4) =
+          make_uint2(pack2<false>(s.x * d, s.y * d), pack2<false>(s.z * d, s.w * d));
+    }
+  }
+}
+
+// ------------------------------------------------------------------ host side
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+  static EncodeTiled fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiled>(f);
+  });
+  return fn;
+}
+
+// One layer's k or v as [page, head][row][value], fetched in boxes of 128 bytes x box_rows rows.
+bool pool_map(CUtensorMap* m, const moe_paged_cache* c, const void* base, int box_rows) {
+  memset(m, 0, sizeof *m);
+  const EncodeTiled enc = encode_tiled();
+  if (!enc) return false;
+  const int es = kv_size(c->kv_type);
+  const cuuint64_t dims[3] = {(cuuint64_t)c->D, (cuuint64_t)c->page, (cuuint64_t)c->num_pages * c->Hkv};
+  const cuuint64_t strides[2] = {(cuuint64_t)c->D * es, (cuuint64_t)c->page * c->D * es};
+  const cuuint32_t box[3] = {(cuuint32_t)(128 / es), (cuuint32_t)box_rows, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return enc(m, es == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base),
+             dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool F8, int MT>
+cudaError_t launch_attn(const PAttnArgs& args, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t s) {
+  using C = Cfg<D, F8>;
+  const void* fn = reinterpret_cast<const void*>(paged_attn_kernel<D, F8, MT>);
+  static SmemGrant granted;
+  cudaError_t e = grant_smem(fn, C::kSmem, 0, granted);
+  if (e != cudaSuccess) return e;
+  PAttnArgs a = args;
+  a.ctas = std::min(kPagedMaxCtas, paged_sms() * C::kPerSm);
+  CUtensorMap k = mk, v = mv;
+  void* p[] = {&a, &k, &v};
+  e = paged_launch(fn, dim3(a.ctas), dim3(kThreads), C::kSmem, s, p);
+  if (e != cudaSuccess) return e;
+  void* j[] = {&a};
+  return paged_launch(reinterpret_cast<const void*>(paged_join_kernel<D>), dim3(a.ctas - 1),
+                      dim3(kJoinThreads), 0, s, j);
+}
+
+template <int D, bool F8>
+cudaError_t launch_rows(const PAttnArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t s) {
+  if (a.rows == 16) return launch_attn<D, F8, 1>(a, mk, mv, s);
+  if (a.rows == 32) return launch_attn<D, F8, 2>(a, mk, mv, s);
+  return launch_attn<D, F8, 4>(a, mk, mv, s);
+}
+
+int tile_keys(int D) { return D == 256 ? 16 : 32; }
+
+}  // namespace
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" {
+
+int moe_paged_attend(const moe_paged_cache* c, int layer, const int32_t* seqs, int B, int Tq, const uint16_t* q, int Hq,
+                     float scale, uint16_t* out, void* workspace, size_t workspace_bytes, moe_stream_t stream) {
+  if (!paged_ok(c) || layer < 0 || layer >= c->layers || B < 0 || B > kPagedMaxBatch || Tq < 1 || Tq > kPagedMaxNew ||
+      Hq < 1 || Hq > 128 || Hq % c->Hkv != 0 || !workspace || !paged_al16(workspace))
+    return (int)cudaErrorInvalidValue;
+  if (B == 0) return (int)cudaSuccess;
+  if (!seqs || !q || !out || !paged_al16(q) || !paged_al16(out)) return (int)cudaErrorInvalidValue;
+  const PagedWs L = paged_ws(c, Hq, B, Tq);
+  if (workspace_bytes < L.total) return (int)cudaErrorInvalidValue;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  PAttnArgs a;
+  a.q = q;
+  a.out = out;
+  a.k_scale = c->kv_type == MOE_KV_E4M3 && c->k_scale ? c->k_scale + (int64_t)layer * c->Hkv : nullptr;
+  a.v_scale = c->kv_type == MOE_KV_E4M3 && c->v_scale ? c->v_scale + (int64_t)layer * c->Hkv : nullptr;
+  a.seqs = seqs;
+  a.tables = c->tables;
+  a.lens = c->lens;
+  a.joins = reinterpret_cast<int32_t*>(ws + L.joins);
+  a.ml = reinterpret_cast<float*>(ws + L.ml);
+  a.acc = reinterpret_cast<float*>(ws + L.acc);
+  a.err = reinterpret_cast<uint32_t*>(ws + L.err);
+  a.B = B;
+  a.Tq = Tq;
+  a.Hq = Hq;
+  a.Hkv = c->Hkv;
+  a.G = Hq / c->Hkv;
+  a.page = c->page;
+  a.num_pages = c->num_pages;
+  a.max_seqs = c->max_seqs;
+  a.max_pages = c->max_pages;
+  a.rows = paged_block_rows(a.G, Tq);
+  a.row_blocks = (a.G * Tq + a.rows - 1) / a.rows;
+  a.scale = scale;
+  a.ctas = 0;
+  // the flattened unit list is counted in 32 bits; a unit is at least 16 keys
+  const int64_t units = ((int64_t)c->max_pages * c->page + 15) / 16;
+  if (B * units * c->Hkv * a.row_blocks >= ((int64_t)1 << 31) - kPagedMaxCtas) return (int)cudaErrorInvalidValue;
+  const int kt = tile_keys(c->D);
+  a.box_rows = c->page % kt == 0 ? kt : 16;
+  CUtensorMap mk, mv;
+  const int64_t off = layer * paged_layer_bytes(c);
+  if (!pool_map(&mk, c, static_cast<const uint8_t*>(c->k) + off, a.box_rows) ||
+      !pool_map(&mv, c, static_cast<const uint8_t*>(c->v) + off, a.box_rows))
+    return (int)cudaErrorNotSupported;
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (c->kv_type == MOE_KV_E4M3)
+    return (int)(c->D == 256 ? launch_rows<256, true>(a, mk, mv, s) : launch_rows<128, true>(a, mk, mv, s));
+  if (c->D == 256) return (int)launch_rows<256, false>(a, mk, mv, s);
+  return (int)(c->D == 128 ? launch_rows<128, false>(a, mk, mv, s) : launch_rows<64, false>(a, mk, mv, s));
+}
+
+}  // extern "C"

@@ -22,9 +22,11 @@
 #include <algorithm>
 #include <cstring>
 
+#include "../../include/moe_spec.h"
 #include "../../include/moe_stack.h"
 #include "moe_common.cuh"
 #include "moe_device.cuh"
+#include "moe_paged.h"
 #include "moe_sync.cuh"
 
 namespace moe {
@@ -39,7 +41,7 @@ constexpr int kArgmaxMaxCtas = 1024;
 // boundary (its acc is stored as float4).
 __host__ __device__ constexpr int part_stride(int D) { return D + 4; }
 
-enum { EPI_BF16 = 0, EPI_ARGMAX = 1 };
+enum { EPI_BF16 = 0, EPI_ARGMAX = 1, EPI_F32 = 2 };
 
 struct GemvArgs {
   const uint16_t* x;   // bf16 [T][K], or (x == null):
@@ -51,8 +53,8 @@ struct GemvArgs {
   int n0, N, K, T;
   uint16_t* y0;        // bf16 [T][n0]
   uint16_t* y1;        // bf16 [T][N - n0]
-  // argmax (T == 1)
-  float* logits;       // fp32 [N] or null
+  // argmax (T == 1), or the fp32 rows themselves
+  float* logits;       // fp32 [T][N], or null (argmax)
   float* pv;           // per-CTA best value
   int32_t* pi;         // per-CTA best index
   uint32_t* ticket;
@@ -174,13 +176,14 @@ __global__ void __launch_bounds__(kGemvWarps * 32, 2) dense_gemv_kernel(const __
     const int r = wg + q * nw;
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[t] = warp_sum(acc[t]);
-    if (EPI == EPI_BF16) {
+    if (EPI != EPI_ARGMAX) {
       if (lane < T) {
         float v = acc[0];
 #pragma unroll
         for (int t = 1; t < MT; ++t)
           if (lane == t) v = acc[t];
-        if (r < g.n0) g.y0[(int64_t)lane * g.n0 + r] = f2bf(v);
+        if (EPI == EPI_F32) g.logits[(int64_t)lane * N + r] = v;
+        else if (r < g.n0) g.y0[(int64_t)lane * g.n0 + r] = f2bf(v);
         else g.y1[(int64_t)lane * (N - g.n0) + (r - g.n0)] = f2bf(v);
       }
     } else {
@@ -507,6 +510,20 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const float* __restri
   o[(int64_t)job * D + d] = ov;
 }
 
+// o = bf16(o * sigmoid(gate)) over n bf16 values, eight a thread (kernels.cuh:765-769).
+__global__ void __launch_bounds__(256) sigmoid_gate_kernel(uint16_t* __restrict__ o, const uint16_t* __restrict__ z,
+                                                           int64_t n) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 8;
+  if (i >= n) return;
+  const uint4 a = *reinterpret_cast<const uint4*>(o + i), g = *reinterpret_cast<const uint4*>(z + i);
+  auto two = [](uint32_t x, uint32_t y) {
+    return (uint32_t)f2bf(lo_bf(x) * sigmoid(lo_bf(y))) | ((uint32_t)f2bf(hi_bf(x) * sigmoid(hi_bf(y))) << 16);
+  };
+  *reinterpret_cast<uint4*>(o + i) = make_uint4(two(a.x, g.x), two(a.y, g.y), two(a.z, g.z), two(a.w, g.w));
+}
+
 // One CTA per row: y = bf16(x * rsqrt(mean(x^2) + eps) * w).
 __global__ void __launch_bounds__(256) rmsnorm_rows_kernel(const float* __restrict__ x, const uint16_t* __restrict__ w,
                                                            uint16_t* __restrict__ y, int H, float eps) {
@@ -595,6 +612,26 @@ bool attn_ok(const moe_attn_weights* w) {
   if (w->rope_dim <= 0 || w->rope_dim > w->D || w->rope_dim % 64 != 0) return false;
   if (w->Hq * w->D > 8192) return false;  // the o GEMV stages Hq D inputs per token in shared memory
   return true;
+}
+
+// Workspace of the paged attention branch: the paged calls' own (its error word leads both), then the activations.
+struct AttnPagedWs {
+  size_t qkv, z, q, o, total;
+};
+AttnPagedWs attn_paged_ws(const moe_attn_weights* w, const moe_paged_cache* c, int B, int Tq) {
+  AttnPagedWs L;
+  const size_t T = (size_t)B * Tq, nq = (size_t)w->Hq * w->D, nqkv = (size_t)(w->Hq + 2 * w->Hkv) * w->D;
+  size_t off = ws_align(moe_paged_workspace_bytes(c, w->Hq, B, Tq));
+  L.qkv = off;  off = ws_align(off + T * nqkv * 2);
+  L.z = off;    off = ws_align(off + (w->gate ? T * nq * 2 : 0));
+  L.q = off;    off = ws_align(off + T * nq * 2);
+  L.o = off;    off = ws_align(off + T * nq * 2);
+  L.total = off;
+  return L;
+}
+bool attn_paged_ok(const moe_attn_weights* w, const moe_paged_cache* c, int B, int Tq) {
+  return attn_ok(w) && paged_shape_ok(c) && w->D == c->D && w->Hkv == c->Hkv && B >= 1 && B <= kPagedMaxBatch &&
+         Tq >= 1 && Tq <= kPagedMaxNew;
 }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -764,6 +801,91 @@ int moe_lm_head_argmax(const uint16_t* normed, const uint16_t* lm_head, int V, i
   g.pi = reinterpret_cast<int32_t*>(ws + 256 + (size_t)kArgmaxMaxCtas * 4);
   g.next = next;
   return (int)launch_gemv<EPI_ARGMAX>(g, std::min(kArgmaxMaxCtas, stack_sms() * 2), (cudaStream_t)stream);
+}
+
+int moe_lm_head_logits(const uint16_t* normed, const uint16_t* lm_head, int V, int H, int T, float* logits,
+                       moe_stream_t stream) {
+  if (!normed || !lm_head || !logits || V < 1 || H < 8 || H % 8 != 0 || H > 8192 || T < 1 || T > kStackMaxT ||
+      !al16(normed) || !al16(lm_head))
+    return (int)cudaErrorInvalidValue;
+  GemvArgs g;
+  memset(&g, 0, sizeof g);
+  g.x = normed;
+  g.w0 = lm_head;
+  g.n0 = V;
+  g.N = V;
+  g.K = H;
+  g.T = T;
+  g.logits = logits;
+  return (int)launch_gemv<EPI_F32>(g, stack_sms() * 2, (cudaStream_t)stream);
+}
+
+size_t moe_attn_paged_workspace_bytes(const moe_attn_weights* w, const moe_paged_cache* c, int max_batch, int max_new) {
+  if (!attn_paged_ok(w, c, max_batch, max_new)) return 0;
+  return attn_paged_ws(w, c, max_batch, max_new).total;
+}
+
+int moe_attn_paged_forward_rms(const moe_attn_weights* w, const uint16_t* rms1, const float* hidden,
+                               const moe_paged_cache* c, int layer, const int32_t* seqs, int B, int Tq,
+                               const double* inv_freq, uint16_t* attn_out, void* workspace, size_t workspace_bytes,
+                               moe_stream_t stream) {
+  if (!attn_paged_ok(w, c, B, Tq) || !rms1 || !hidden || !seqs || !inv_freq || !attn_out || !workspace ||
+      !al16(rms1) || !al16(hidden) || !al16(workspace) || !al16(w->qkv) || !al16(w->o) || (w->gate && !al16(w->gate)))
+    return (int)cudaErrorInvalidValue;
+  const AttnPagedWs L = attn_paged_ws(w, c, B, Tq);
+  if (workspace_bytes < L.total) return (int)cudaErrorInvalidValue;
+  const cudaStream_t s = (cudaStream_t)stream;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  uint16_t* qkv = reinterpret_cast<uint16_t*>(ws + L.qkv);
+  uint16_t* z = w->gate ? reinterpret_cast<uint16_t*>(ws + L.z) : nullptr;
+  uint16_t* q = reinterpret_cast<uint16_t*>(ws + L.q);
+  uint16_t* o = reinterpret_cast<uint16_t*>(ws + L.o);
+  const int T = B * Tq, nq = w->Hq * w->D, nqkv = (w->Hq + 2 * w->Hkv) * w->D, ctas = stack_sms() * 2;
+  cudaError_t e;
+  GemvArgs g;
+  for (int t = 0; t < T; t += kStackMaxT) {
+    memset(&g, 0, sizeof g);
+    g.xf = hidden + (int64_t)t * w->H;
+    g.xw = rms1;
+    g.eps = w->eps;
+    g.w0 = w->qkv;
+    g.w1 = w->gate;
+    g.n0 = nqkv;
+    g.N = nqkv + (w->gate ? nq : 0);
+    g.K = w->H;
+    g.T = std::min(kStackMaxT, T - t);
+    g.y0 = qkv + (int64_t)t * nqkv;
+    g.y1 = z ? z + (int64_t)t * nq : nullptr;
+    e = launch_gemv<EPI_BF16>(g, ctas, s);
+    if (e != cudaSuccess) return (int)e;
+  }
+  int rc = moe_paged_append(c, layer, seqs, B, Tq, qkv, w->Hq, w->q_norm, w->k_norm, inv_freq, w->rope_dim, w->eps, q,
+                            workspace, workspace_bytes, stream);
+  if (rc != 0) return rc;
+  rc = moe_paged_attend(c, layer, seqs, B, Tq, q, w->Hq, 1.f / sqrtf((float)w->D), o, workspace, workspace_bytes,
+                        stream);
+  if (rc != 0) return rc;
+  if (z) {
+    int64_t n = (int64_t)T * nq;
+    const uint16_t* zz = z;
+    void* args[] = {&o, &zz, &n};
+    e = launch_pdl(reinterpret_cast<const void*>(sigmoid_gate_kernel), dim3((unsigned)((n / 8 + 255) / 256)), dim3(256),
+                   0, s, args);
+    if (e != cudaSuccess) return (int)e;
+  }
+  for (int t = 0; t < T; t += kStackMaxT) {
+    memset(&g, 0, sizeof g);
+    g.x = o + (int64_t)t * nq;
+    g.w0 = w->o;
+    g.n0 = w->H;
+    g.N = w->H;
+    g.K = nq;
+    g.T = std::min(kStackMaxT, T - t);
+    g.y0 = attn_out + (int64_t)t * w->H;
+    e = launch_gemv<EPI_BF16>(g, ctas, s);
+    if (e != cudaSuccess) return (int)e;
+  }
+  return (int)cudaSuccess;
 }
 
 }  // extern "C"

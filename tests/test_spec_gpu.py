@@ -1,0 +1,279 @@
+"""GPU tests of the step from logits to tokens (include/moe_spec.h): several tokens' logits, softmax rows, and the
+verification of drafts, against 64-bit restatements."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F32 = 2.0 ** -24
+
+
+def S():
+    from mvcc_b200 import spec
+    return spec
+
+
+# ------------------------------------------------------------------ logits
+
+@pytest.mark.parametrize("V,H,T", [(1000, 256, 1), (999, 2048, 4), (70, 8, 3), (5000, 8192, 7), (20000, 1024, 2)])
+def test_lm_head_logits(V, H, T):
+    g = torch.Generator(device="cuda").manual_seed(V)
+    w = (0.05 * torch.randn(V, H, generator=g, device="cuda")).to(torch.bfloat16)
+    x = torch.randn(T, H, generator=g, device="cuda").to(torch.bfloat16)
+    out = torch.full((T, V), 7.0, device="cuda")
+    S().lm_head_logits(w.view(torch.int16), x.view(torch.int16), out)
+    want = x.double() @ w.double().T
+    mag = x.double().abs() @ w.double().abs().T
+    assert bool(((out.double() - want).abs() <= (H // 32 + 8) * F32 * mag + 1e-30).all())  # a lane's chain, then the tree
+    if T == 1:  # the same numbers as the argmax head's
+        from mvcc_b200 import stack as st
+        l1, nxt = torch.zeros(V, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+        st.LmHead(w.view(torch.int16)).argmax(x.view(torch.int16)[0], nxt, logits=l1)
+        assert torch.equal(l1, out[0])
+
+
+# ------------------------------------------------------------------ softmax
+
+def softmax64(x, t):
+    """[R, V] doubles, by the header's words; t doubles [R]."""
+    out = torch.zeros_like(x)
+    for i in range(x.shape[0]):
+        v = torch.where(torch.isnan(x[i]), -math.inf, x[i])
+        m = v.max()
+        if m == -math.inf:
+            continue
+        if not t[i] > 0:
+            out[i, int(torch.nonzero(v == m)[0, 0])] = 1.0
+            continue
+        e = torch.where(v == m, 1.0, torch.exp((v - m) / t[i]))
+        out[i] = e / e.sum()
+    return out
+
+
+def near(got, x, t):
+    """2^-20 (the exponential) plus a few roundings of its argument, relative; below fp32's normal range zero will do."""
+    want = softmax64(x.double(), t.double())
+    v = torch.where(torch.isfinite(x), x, 0.0).double()
+    top = torch.where(torch.isfinite(x), x, -math.inf).amax(1, keepdim=True).double()
+    arg = torch.where(torch.isfinite(x.double() - top), (v - top) / torch.where(t > 0, t, 1.0).double()[:, None], 0.0)
+    arg = arg.abs().clamp(max=110)
+    tol = want * (2.0 ** -20 + 8 * F32 * (1 + arg)) + 2.0 ** -120
+    err = (got.double() - want).abs()
+    assert bool((err <= tol).all()), float((err - tol).max())
+
+
+@pytest.mark.parametrize("R,V", [(1, 1), (3, 2), (5, 7), (4, 151936), (9, 1001), (2, 20480), (2, 20484), (3, 40961),
+                                 (2, 163840), (2, 163844), (1, 200001), (2, 262144), (1, 262145), (1, 600000), (70, 640)])
+def test_softmax_rows(R, V):
+    g = torch.Generator(device="cuda").manual_seed(R * V)
+    x = 4 * torch.randn(R, V, generator=g, device="cuda")
+    t = 0.3 + torch.rand(R, generator=g, device="cuda")
+    t[1::3] = 0.0
+    out = torch.full_like(x, 9.0)
+    S().softmax_rows(x, out, temperature=t)
+    near(out, x, t)
+    S().softmax_rows(x, out)
+    near(out, x, torch.ones_like(t))
+    again = x.clone()
+    S().softmax_rows(again, again)  # in place
+    assert torch.equal(again, out)
+
+
+@pytest.mark.parametrize("V", [37, 4096, 50001, 270000])
+def test_softmax_of_masked_and_infinite_rows(V):
+    x = torch.randn(9, V, device="cuda", generator=torch.Generator(device="cuda").manual_seed(V))
+    low = torch.finfo(torch.float32).min
+    x[0] = -math.inf                        # nothing
+    x[1], x[1, V // 2] = -math.inf, -3.0    # one left
+    x[2, ::2] = low                         # masks of the type's lowest value
+    x[3] = low                              # all of them: equal
+    x[4, 5], x[4, V - 1] = math.inf, math.inf
+    x[5] = math.nan
+    x[6, 3], x[6, V // 3] = math.nan, -math.inf
+    x[7] = 1.5                              # ties
+    x[8, 7:] = -math.inf
+    for t in (1.0, 0.0, -1.0, math.nan, 1e-3, 1e-40, 1e30):
+        tt = torch.full((9,), t, device="cuda")
+        out = torch.full_like(x, 9.0)
+        S().softmax_rows(x, out, temperature=tt)
+        if t == 1e-40:  # anything below the maximum is gone
+            want = softmax64(x.double(), torch.full((9,), 1e-12, device="cuda").double())
+            assert bool(((out.double() - want).abs() <= 2.0 ** -20 * want + 2.0 ** -120).all())
+        else:
+            near(out, x, tt)
+
+
+def test_softmax_keeps_what_lies_between_rows():
+    x = torch.randn(6, 1000, device="cuda")
+    y = torch.full((6, 1003), 5.0, device="cuda")
+    S().softmax_rows(x[:, 1:777], y[:, 2:778])  # rows at odd places
+    assert bool((y[:, :2] == 5).all()) and bool((y[:, 778:] == 5).all())
+    near(y[:, 2:778].contiguous(), x[:, 1:777].contiguous(), torch.ones(6, device="cuda"))
+    with pytest.raises(ValueError):
+        S().softmax_rows(x.T, y[:, :6].T)
+    with pytest.raises(ValueError):
+        S().softmax_rows(x, y)
+    with pytest.raises(ValueError):
+        S().softmax_rows(x, torch.empty_like(x), temperature=torch.ones(5, device="cuda"))
+
+
+# ------------------------------------------------------------------ verification
+
+def verify64(p, q, x, u, n):
+    """(tokens, accepted, gap) by the header's words, in numpy doubles. gap: how near, relative to the total, the drawn
+    token's border is to the target: draws nearer than the sums' order can decide are left out of a comparison."""
+    B, K1, V = p.shape
+    K = K1 - 1
+    clean = lambda a: np.where((a > 0) & np.isfinite(a), a, 0.0)  # noqa: E731
+    p = clean(p)
+    q = None if q is None else clean(q)
+    tokens, acc, gap = np.full((B, K1), -1), np.zeros(B, int), np.ones(B)
+    for b in range(B):
+        m = K if n is None else min(max(int(n[b]), 0), K)
+        a = 0
+        while a < m:
+            t = int(x[b, a])
+            if not 0 <= t < V:
+                break
+            if not u[b, a] * (1.0 if q is None else q[b, a, t]) < p[b, a, t]:
+                break
+            tokens[b, a] = t
+            a += 1
+        w = p[b, a].copy()
+        if a < m:
+            if q is not None:
+                w = np.maximum(w - q[b, a], 0)
+            elif 0 <= x[b, a] < V:
+                w[x[b, a]] = max(w[x[b, a]] - 1.0, 0)
+        if not w.sum() > 0:
+            w = p[b, a]
+        acc[b] = a
+        if not w.sum() > 0:
+            continue
+        run = np.cumsum(w)
+        hit = np.flatnonzero((run > u[b, K] * run[-1]) & (w > 0))
+        tokens[b, a] = hit[0] if len(hit) else np.flatnonzero(w > 0)[-1]
+        gap[b] = np.abs(run - u[b, K] * run[-1]).min() / run[-1]
+    return tokens, acc, gap
+
+
+def run_verify(p, q, x, u, n=None, ver=None):
+    B, K1, V = p.shape
+    ver = ver or S().SpecVerifier(B, K1 - 1, V)
+    tok = torch.full((B, K1), 55, dtype=torch.int32, device="cuda")
+    acc = torch.full((B,), 55, dtype=torch.int32, device="cuda")
+    ver.verify(p, q, x, u, tok, acc, n_drafted=n)
+    return tok.cpu().numpy(), acc.cpu().numpy()
+
+
+def compare(p, q, x, u, n=None, ver=None, least=0.9):
+    tok, acc = run_verify(p, q, x, u, n, ver)
+    d = lambda t: None if t is None else t.cpu().numpy().astype(np.float64)  # noqa: E731
+    want, wacc, gap = verify64(d(p), d(q), x.cpu().numpy(), d(u), None if n is None else n.cpu().numpy())
+    assert np.array_equal(acc, wacc)
+    safe = gap > 1e-13  # V x 2^-53 and a margin
+    assert safe.mean() >= least
+    assert np.array_equal(tok[safe], want[safe])
+    return tok, acc
+
+
+def drafts(B, K, V, seed, noise=0.7):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    z = 2 * torch.randn(B, K + 1, V, generator=g, device="cuda")
+    p = torch.softmax(z, -1)
+    y = z[:, :K] + noise * torch.randn(B, K, V, generator=g, device="cuda")
+    q = torch.softmax(y, -1)
+    x = (y - torch.log(-torch.log(torch.rand(B, K, V, generator=g, device="cuda").clamp(1e-30, 1 - 1e-7)))).argmax(-1)
+    return p, q, x.int(), torch.rand(B, K + 1, generator=g, device="cuda")
+
+
+@pytest.mark.parametrize("B,K,V", [(1, 1, 1), (2, 1, 2), (40, 3, 5), (33, 2, 4096), (9, 4, 4097), (64, 4, 8191),
+                                   (5, 3, 151936), (3, 64, 300), (3, 33, 1000), (1, 2, 600001), (300, 1, 50)])
+def test_verify_against_64_bits(B, K, V):
+    p, q, x, u = drafts(B, K, V, seed=B + K + V)
+    ver = S().SpecVerifier(B, K, V)
+    _, a1 = compare(p, q, x, u, ver=ver)
+    compare(p, None, x, u, ver=ver)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    n = torch.randint(-1, K + 2, (B,), generator=g, device="cuda").int()
+    compare(p, q, x, u, n=n, ver=ver)
+    compare(p, None, x, u, n=n, ver=ver)
+    assert np.array_equal(run_verify(p, q, x, u, ver=ver)[1], a1)  # the tickets came back to zero
+    if B >= 30 and V > 100 and K > 1:
+        assert len(set(a1.tolist())) > 1  # some rejected, some not
+
+
+def test_verify_draws_by_the_residual_distribution():
+    """Over many sequences the emitted first token follows the target's probabilities, whatever the draft's are."""
+    V, B = 6, 60000
+    p = torch.tensor([0.05, 0.3, 0.0, 0.4, 0.15, 0.1], device="cuda")
+    q = torch.tensor([0.3, 0.1, 0.2, 0.2, 0.1, 0.1], device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.multinomial(q.expand(B, V), 1, generator=g).int()
+    u = torch.rand(B, 2, generator=g, device="cuda")
+    tok, _ = run_verify(p.expand(B, 2, V).contiguous(), q.expand(B, 1, V).contiguous(), x, u)
+    got = np.bincount(tok[:, 0], minlength=V) / B
+    sigma = np.sqrt(np.maximum(p.cpu().numpy() * (1 - p.cpu().numpy()), 0) / B)
+    assert (np.abs(got - p.cpu().numpy()) <= 5 * sigma + 1e-12).all(), got
+
+
+def test_verify_at_borders_and_with_bad_values():
+    K, V = 2, 10000
+    p = torch.zeros(10, K + 1, V, device="cuda")
+    q = torch.zeros(10, K, V, device="cuda")
+    x = torch.zeros(10, K, dtype=torch.int32, device="cuda")
+    u = torch.full((10, K + 1), 0.5, device="cuda")
+    p[:, :, 4000:4004] = 0.25
+    q[:, :, 4000:4004] = 0.25
+    x[:] = 4001
+    u[0] = 0.0                          # accepted; the draw: the first token with weight
+    u[1] = 1.0                          # out of range: u q < p fails, p = q leaves no residual: drawn from p, its last
+    x[2, 0] = -1                        # no such token
+    x[3, 1] = V
+    x[4, 0] = 7                         # p and q zero there
+    p[5, 0, 4001] = math.nan
+    q[6, 0, 4001] = math.inf            # counts as zero: accepted
+    p[7] = 0.0                          # nothing to draw from
+    p[8, 0], p[8, 0, 9999] = 0.0, 1.0   # residual at the very end
+    x[8, 0], q[8, 0], q[8, 0, 9998] = 9998, 0.0, 1.0
+    p[9, :, 0], p[9, :, 4002], p[9, :, 4003] = -3.0, math.inf, math.nan
+    tok, acc = compare(p, q, x, u, least=0.0)
+    assert acc.tolist() == [2, 0, 0, 1, 0, 0, 2, 0, 0, 2]
+    assert tok[0].tolist() == [4001, 4001, 4000] and tok[1].tolist() == [4003, -1, -1]
+    assert tok[7].tolist() == [-1, -1, -1] and tok[8].tolist() == [9999, -1, -1]
+    assert tok[2, 0] == 4002 and tok[3].tolist() == [4001, 4002, -1] and tok[4, 0] == 4002
+    assert tok[5, 0] in (4000, 4002, 4003) and tok[9, 2] == 4001
+
+
+def test_verify_of_rows_apart_on_another_stream_and_in_a_graph():
+    B, K, V = 6, 3, 5003
+    p, q, x, u = drafts(B, K, V, seed=2)
+    wide_p, wide_q = torch.full((B, K + 1, V + 5), 9.0, device="cuda"), torch.full((B, K, V + 9), 9.0, device="cuda")
+    wide_p[..., :V], wide_q[..., :V] = p, q
+    ver = S().SpecVerifier(8, K, V)  # a workspace for more
+    tok, acc = run_verify(p, q, x, u, ver=ver)
+    t2, a2 = run_verify(wide_p[..., :V], wide_q[..., :V], x, u, ver=ver)
+    assert np.array_equal(tok, t2) and np.array_equal(acc, a2)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    tt, aa = torch.zeros(B, K + 1, dtype=torch.int32, device="cuda"), torch.zeros(B, dtype=torch.int32, device="cuda")
+    with torch.cuda.stream(s):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            ver.verify(p, q, x, u, tt, aa)
+        for _ in range(3):
+            u.copy_(torch.rand(B, K + 1, device="cuda"))
+            graph.replay()
+            s.synchronize()
+            want, wacc, gap = verify64(p.double().cpu().numpy(), q.double().cpu().numpy(), x.cpu().numpy(),
+                                       u.double().cpu().numpy(), None)
+            assert np.array_equal(aa.cpu().numpy(), wacc) and np.array_equal(tt.cpu().numpy()[gap > 1e-13],
+                                                                             want[gap > 1e-13])
+    for bad in (lambda: ver.verify(p[:, :, ::2], q, x, u, tt, aa), lambda: ver.verify(p, q[:, :2], x, u, tt, aa),
+                lambda: ver.verify(p, q, x.long(), u, tt, aa), lambda: ver.verify(p.cpu(), q, x, u, tt, aa),
+                lambda: ver.verify(p.repeat(2, 1, 1), q, x, u, tt, aa), lambda: ver.verify(p, q, x, u, tt[:, :2], aa)):
+        with pytest.raises(ValueError):
+            bad()
