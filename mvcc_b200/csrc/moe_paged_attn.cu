@@ -12,8 +12,9 @@
 // lies in one CTA is finished there. A job of n parts holds n - 1 of the borders between CTAs, so the join runs a CTA
 // a border, and those of one job share its rows.
 //
-// CTA: four consumer warps and a producer warp. The producer walks the CTA's tiles (KT keys of k and v each), reads
-// the page ids 32 at a time and fetches the tiles by TMA (boxes of 64 values x 16 or KT rows inside one page, 128-byte
+// CTA: four consumer warps and NP producer warps, four producers an SM (a thread issues a TMA copy every 95 cycles or
+// so: one alone fetches 3.2 TB/s over the GPU in 2 KB boxes, four 6.4 TB/s). Producer w takes every NP-th of the
+// CTA's tiles (KT keys of k and v each), reads the page ids 32 at a time and fetches the tiles by TMA (boxes of 64 values x 16 or KT rows inside one page, 128-byte
 // swizzle) into a ring of NS slots, mbarrier-counted. Consumer warp (g, mt) holds 16 query rows as MMA fragments and
 // takes every NG-th tile: S = Q K^T, the running maximum and sum of the softmax, O += P V, all in registers; at a job's
 // end the NG warps of a row tile merge through shared memory.
@@ -35,7 +36,6 @@ namespace moe {
 namespace {
 
 constexpr int kWarps = 4;                      // consumer warps
-constexpr int kThreads = (kWarps + 1) * 32;
 constexpr int kSmemOne = 227 * 1024;           // shared memory of a CTA alone on its SM
 constexpr int kSmemTwo = 113 * 1024;           // of one of two
 
@@ -65,13 +65,18 @@ struct Cfg {
   static constexpr int kTile = KT * kRow;                 // bytes of a k or v tile
   static constexpr int kSlot = 2 * kTile;
   static constexpr int kPerSm = D == 256 ? 1 : 2;         // CTAs an SM: registers (accumulator D / 2 a lane)
+  static constexpr int NP = 4 / kPerSm;                   // producer warps
+  static constexpr int kThreads = (kWarps + NP) * 32;
   static constexpr int kMerge = 16 * (D + 8) * 4;         // bytes of one warp's partial in the merge buffer
   static constexpr int kUnits = (kPagedMaxBatch + 1) * 4; // the scan of the units
   static constexpr int kFixed = 1024 + ((2 * kMerge + kUnits + 127) & ~127) + 1024;
   static constexpr int kFit = ((kPerSm == 1 ? kSmemOne : kSmemTwo) - kFixed) / kSlot;
-  static constexpr int NS = kFit > 24 ? 24 : kFit;        // ring slots
+  // Ring slots: a multiple of the producers and of the key groups, so that a slot is always filled by one producer and
+  // read by one group. Barrier waits tell phases apart by parity alone: two producers on one slot could be two turns
+  // apart, and the one ahead would take a slot for free that is still to be filled.
+  static constexpr int NS = (kFit > 24 ? 24 : kFit) / kWarps * kWarps;
   static constexpr int kSmem = kFixed + NS * kSlot;
-  static_assert(NS >= 4, "ring too short");
+  static_assert(NS >= kWarps && NS % NP == 0, "ring");
 };
 
 // D (16x8, fp32) += A (16x16) B (16x8); bf16 or f16 operands.
@@ -173,11 +178,11 @@ struct Walk {
 };
 
 template <int D, bool F8, int MT>
-__global__ void __launch_bounds__(kThreads, Cfg<D, F8>::kPerSm)
+__global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
     paged_attn_kernel(const __grid_constant__ PAttnArgs a, const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v) {
   using C = Cfg<D, F8>;
-  constexpr int NG = kWarps / MT, KT = C::KT, UK = NG * KT, NS = C::NS;
+  constexpr int NG = kWarps / MT, KT = C::KT, UK = NG * KT, NS = C::NS, NP = C::NP, kThreads = C::kThreads;
   constexpr int NT = D / 8;     // accumulator tiles of 8 columns
   constexpr int KC = C::kRow / 16;  // 16-byte chunks of a cached row
   extern __shared__ uint8_t smem_raw[];
@@ -241,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F8>::kPerSm)
     jn[JOIN_PARTS] = parts;
   }
 
-  if (warp == kWarps) {
+  if (warp >= kWarps) {
     // ---------------------------------------------------------------- producer
     const int none = a.num_pages * a.Hkv;  // a page that is not there: outside the map, reads as zero
     const int nbox = KT / a.box_rows;
@@ -259,6 +264,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F8>::kPerSm)
       int fetched = lu * UK;  // first key whose box no lane holds yet
       int held = 0;           // first key of lane 0's box
       for (int key = lu * UK; key < key_end && ok; key += KT, ++i) {
+        if (i % NP != warp - kWarps) continue;
         const int slot = i % NS, turn = i / NS;
         if (turn > 0) {
           ok = bar_wait(&empty[slot], (turn - 1) & 1);
@@ -271,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F8>::kPerSm)
           if (lane == 0) mbar_arrive(&full[slot]);
           continue;
         }
-        if (key >= fetched) {  // the next 32 boxes' pages
+        while (key >= fetched) {  // the next 32 boxes' pages
           held = fetched;
           const int k = fetched + lane * a.box_rows;
           z = none;
@@ -291,10 +297,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F8>::kPerSm)
         for (int x = 0; x < boxes; ++x) {
           const int from = (key - held) / a.box_rows + x;
           const int bz = __shfl_sync(0xffffffffu, z, from), by = __shfl_sync(0xffffffffu, y, from);
-          if (lane < 2 * C::kSegs) {  // a lane a box: segment lane % kSegs of k or of v
-            const int sg = lane % C::kSegs, is_v = lane / C::kSegs;
-            tma_load_3d(dst + is_v * C::kTile + sg * C::kSeg + x * a.box_rows * 128, is_v ? &map_v : &map_k,
-                        sg * (128 / C::kEs), by, bz, &full[slot]);
+          // one lane issues every copy: the operands of a TMA instruction are uniform, lanes would take turns
+          if (lane == 0) {
+#pragma unroll
+            for (int sg = 0; sg < C::kSegs; ++sg) {
+              uint8_t* at = dst + sg * C::kSeg + x * a.box_rows * 128;
+              tma_load_3d(at, &map_k, sg * (128 / C::kEs), by, bz, &full[slot]);
+              tma_load_3d(at + C::kTile, &map_v, sg * (128 / C::kEs), by, bz, &full[slot]);
+            }
           }
         }
         __syncwarp();
@@ -302,7 +312,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, F8>::kPerSm)
       w.u += run;
     }
     if (!ok)  // no copy may still be landing when the CTA exits
-      for (int j = max(0, i - NS); j < i; ++j) bar_wait(&full[j % NS], (j / NS) & 1);
+      for (int j = max(0, i - NS); j < i; ++j)
+        if (j % NP == warp - kWarps) bar_wait(&full[j % NS], (j / NS) & 1);
     return;
   }
 
@@ -748,7 +759,7 @@ cudaError_t launch_attn(const PAttnArgs& args, const CUtensorMap& mk, const CUte
   a.ctas = std::min(kPagedMaxCtas, paged_sms() * C::kPerSm);
   CUtensorMap k = mk, v = mv;
   void* p[] = {&a, &k, &v};
-  e = paged_launch(fn, dim3(a.ctas), dim3(kThreads), C::kSmem, s, p);
+  e = paged_launch(fn, dim3(a.ctas), dim3(C::kThreads), C::kSmem, s, p);
   if (e != cudaSuccess) return e;
   void* j[] = {&a};
   return paged_launch(reinterpret_cast<const void*>(paged_join_kernel<D>), dim3(a.ctas - 1),
