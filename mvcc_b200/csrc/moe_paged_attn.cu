@@ -67,9 +67,10 @@ struct Cfg {
   static constexpr int kPerSm = D == 256 ? 1 : 2;         // CTAs an SM: registers (accumulator D / 2 a lane)
   static constexpr int NP = 4 / kPerSm;                   // producer warps
   static constexpr int kThreads = (kWarps + NP) * 32;
-  static constexpr int kMerge = 16 * (D + 8) * 4;         // bytes of one warp's partial in the merge buffer
-  static constexpr int kUnits = (kPagedMaxBatch + 1) * 4; // the scan of the units
-  static constexpr int kFixed = 1024 + ((2 * kMerge + kUnits + 127) & ~127) + 1024;
+  static constexpr int kMergeRow = 64 + 4;                // floats of a row in the merge buffer: 64 columns, padded
+  static constexpr int kMerge = kWarps * 16 * (kMergeRow + 2) * 4;  // every warp's 64 columns, maxima and sums
+  static constexpr int kSlots = (kPagedMaxBatch + 1) * 4 * 3;       // first unit, keys and sequence of every slot
+  static constexpr int kFixed = 1024 + ((kMerge + kSlots + 127) & ~127) + 1024;
   static constexpr int kFit = ((kPerSm == 1 ? kSmemOne : kSmemTwo) - kFixed) / kSlot;
   // Ring slots: a multiple of the producers and of the key groups, so that a slot is always filled by one producer and
   // read by one group. Barrier waits tell phases apart by parity alone: two producers on one slot could be two turns
@@ -139,6 +140,13 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* mbar) {
 }
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
 
+// Whether one of the values in w (two bf16, or four e4m3) is NaN or infinite.
+template <bool F8>
+__device__ __forceinline__ bool not_finite(uint32_t w) {
+  if constexpr (F8) return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0;  // e4m3 has no infinity
+  else return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+}
+
 // Keys of slot b: its sequence's length, 0 for an unused slot or a bad entry (recorded).
 __device__ __forceinline__ int slot_keys(const PAttnArgs& a, int b, int* seq) {
   const int s = a.seqs[b];
@@ -190,7 +198,10 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
   __shared__ int sm[32];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   float* merge = reinterpret_cast<float*>(ring + (size_t)NS * C::kSlot);
-  int* S = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(merge) + 2 * C::kMerge);
+  float2* merge_ml = reinterpret_cast<float2*>(merge + kWarps * 16 * C::kMergeRow);
+  int* S = reinterpret_cast<int*>(merge_ml + kWarps * 16);
+  int* keys = S + a.B + 1;
+  int* seqs = keys + a.B;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
@@ -206,10 +217,10 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
     const int per = (a.B + kThreads - 1) / kThreads, b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
     int sum = 0;
     for (int b = b0; b < b1; ++b) {
-      int s;
-      const int u = (slot_keys(a, b, &s) + UK - 1) / UK;
+      const int n = slot_keys(a, b, &seqs[b]);
+      keys[b] = n;
       S[b] = sum;
-      sum += u;
+      sum += (n + UK - 1) / UK;
     }
     int total;
     const int before = block_excl_scan(sum, sm, &total);
@@ -256,9 +267,8 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
       w.seek(S, a.B, HR);
       const int rel = w.u - w.base, job = rel / w.U, lu = rel - job * w.U, run = min(w.end - w.u, w.U - lu);
       const int h = job / a.row_blocks;
-      int seq;
-      const int n = slot_keys(a, w.b, &seq);
-      const int32_t* row = a.tables + (int64_t)seq * a.max_pages;
+      const int n = keys[w.b];
+      const int32_t* row = a.tables + (int64_t)seqs[w.b] * a.max_pages;
       const int key_end = (lu + run) * UK;
       int z = 0, y = 0;
       int fetched = lu * UK;  // first key whose box no lane holds yet
@@ -334,8 +344,7 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
     w.seek(S, a.B, HR);
     const int rel = w.u - w.base, job = rel / w.U, lu = rel - job * w.U, run = min(w.end - w.u, w.U - lu);
     const int h = job / a.row_blocks, rb = job - h * a.row_blocks;
-    int seq;
-    const int n = slot_keys(a, w.b, &seq);
+    const int n = keys[w.b];
     const bool whole = lu == 0 && run == w.U;
     // this lane's two rows: query row r of the kv head is token r / G, head h G + r % G
     const int rA = rb * a.rows + mt * 16 + qr, rB = rA + 8, M = a.G * a.Tq;
@@ -509,13 +518,31 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
             }
           }
         };
-        if (!masked) {
+        // A weight of zero does not silence a NaN or an infinity, so what lies behind the sequence is made zero where
+        // it lies, and a row that some tokens see and others do not is looked through for such values first.
+        bool careful = false;
+        if (masked) {
+          uint8_t* v8 = ring + (size_t)slot * C::kSlot + C::kTile;
+          for (int r = max(0, n - key0); r < KT; ++r)
+            if (lane < C::kRow / 16)
+              *reinterpret_cast<uint4*>(v8 + (lane >> 3) * C::kSeg + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+          bool odd = false;
+          for (int r = max(0, n - a.Tq + 1 - key0); r < min(KT, n - key0); ++r)
+            if (lane < C::kRow / 16) {
+              const uint4 x = *reinterpret_cast<const uint4*>(v8 + (lane >> 3) * C::kSeg + r * 128 + (lane & 7) * 16);
+              odd |= not_finite<F8>(x.x) || not_finite<F8>(x.y) || not_finite<F8>(x.z) || not_finite<F8>(x.w);
+            }
+          careful = __any_sync(0xffffffffu, odd);
+          fence_proxy_async_smem();  // the next copy into the slot comes after these writes
+          __syncwarp();
+        }
+        if (!careful) {
           pv([](int, int) { return 0xffffffffu; },
              [](float (&d)[4], const uint32_t (&p)[4], uint32_t b0, uint32_t b1) { mma16816<F8>(d, p, b0, b1); });
         } else {
-          // Zero weights do not silence a NaN or an infinity, so what a row may not see is taken out of V itself: one
-          // pass per token of these rows, each over the keys that token sees, kept by its rows alone.
+          // one pass per token of these rows, over the keys that token sees, kept by its rows alone
           const int t0 = (rb * a.rows + mt * 16) / a.G, t1 = min(a.Tq - 1, (rb * a.rows + mt * 16 + 15) / a.G);
+#pragma unroll 1
           for (int t = t0; t <= t1; ++t) {
             const int vis = n - a.Tq + t + 1 - key0;  // keys of the tile that token t sees
             pv([&](int ks, int hi) {
@@ -544,87 +571,73 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
     lA = quad_sum(lA);
     lB = quad_sum(lB);
 
-    // merge the NG warps of a row tile: halves of them hand over until warp mt holds the sum
-#pragma unroll
-    for (int half = NG / 2; half >= 1; half >>= 1) {
-      float* buf = merge + (size_t)((g & (half - 1)) * MT + mt) * (C::kMerge / 4);
-      if (g >= half && g < 2 * half) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-          *reinterpret_cast<float4*>(buf + (j * 32 + lane) * 4) = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
-        *reinterpret_cast<float4*>(buf + (NT * 32 + lane) * 4) = make_float4(mA, mB, lA, lB);
-      }
-      consumers_sync();
-      if (g < half) {
-        const float4 o = *reinterpret_cast<const float4*>(buf + (NT * 32 + lane) * 4);
-        const float nA = fmaxf(mA, o.x), nB = fmaxf(mB, o.y);
-        const float zA = nA == -INFINITY ? 0.f : nA, zB = nB == -INFINITY ? 0.f : nB;
-        const float cA = ex2(mA - zA), cB = ex2(mB - zB), dA = ex2(o.x - zA), dB = ex2(o.y - zB);
-        lA = lA * cA + o.z * dA;
-        lB = lB * cB + o.w * dB;
-        mA = nA;
-        mB = nB;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const float4 x = *reinterpret_cast<const float4*>(buf + (j * 32 + lane) * 4);
-          acc[j][0] = acc[j][0] * cA + x.x * dA;
-          acc[j][1] = acc[j][1] * cA + x.y * dA;
-          acc[j][2] = acc[j][2] * cB + x.z * dB;
-          acc[j][3] = acc[j][3] * cB + x.w * dB;
-        }
-      }
-      consumers_sync();
+    // The job's end: the NG warps of a row tile meet in shared memory, 64 columns at a time; a thread then holds eight
+    // columns of one row, scales the warps' sums to their common maximum and stores them.
+    if (ql == 0) {
+      merge_ml[warp * 16 + qr] = make_float2(mA, lA);
+      merge_ml[warp * 16 + qr + 8] = make_float2(mB, lB);
     }
-    if (g == 0) {
-      // columns of accumulator tile j: bf16 8 j + 2 ql, + 1; e4m3 (tiles 2c, 2c + 1) 16 c + 4 ql + {0, 2}, + {1, 3}
-      if (whole) {
-        const float vs = a.v_scale ? a.v_scale[h] : 1.f;
-        // an empty row is zero; a NaN sum stays
-        const float dA = lA == 0.f ? 0.f : vs / lA, dB = lB == 0.f ? 0.f : vs / lB;
-        uint16_t* oA = a.out + (((int64_t)w.b * a.Tq + tA) * a.Hq + h * a.G + (rA - tA * a.G)) * D;
-        uint16_t* oB = a.out + (((int64_t)w.b * a.Tq + tB) * a.Hq + h * a.G + (rB - tB * a.G)) * D;
+    const int orow = (tid >> 3) & 15, ocol = (tid & 7) * 8;  // MT row tiles of 16 rows x 64 columns, 128 threads a turn
+    const float vs = a.v_scale ? a.v_scale[h] : 1.f;
+#pragma unroll
+    for (int c0 = 0; c0 < D; c0 += 64) {
+      float* mine = merge + warp * 16 * C::kMergeRow;
+#pragma unroll
+      for (int j = c0 / 8; j < c0 / 8 + 8; j += F8 ? 2 : 1) {
+        // columns of accumulator tile j: bf16 8 j + 2 ql, + 1; e4m3 (tiles j, j + 1) 8 j + 4 ql + {0, 2}, + {1, 3}
         if constexpr (!F8) {
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            if (rA < M) *reinterpret_cast<uint32_t*>(oA + 8 * j + 2 * ql) = pack2<false>(acc[j][0] * dA, acc[j][1] * dA);
-            if (rB < M) *reinterpret_cast<uint32_t*>(oB + 8 * j + 2 * ql) = pack2<false>(acc[j][2] * dB, acc[j][3] * dB);
-          }
+          *reinterpret_cast<float2*>(mine + qr * C::kMergeRow + 8 * j - c0 + 2 * ql) = make_float2(acc[j][0], acc[j][1]);
+          *reinterpret_cast<float2*>(mine + (qr + 8) * C::kMergeRow + 8 * j - c0 + 2 * ql) =
+              make_float2(acc[j][2], acc[j][3]);
         } else {
-#pragma unroll
-          for (int j = 0; j < NT; j += 2) {
-            if (rA < M)
-              *reinterpret_cast<uint2*>(oA + 8 * j + 4 * ql) =
-                  make_uint2(pack2<false>(acc[j][0] * dA, acc[j + 1][0] * dA), pack2<false>(acc[j][1] * dA, acc[j + 1][1] * dA));
-            if (rB < M)
-              *reinterpret_cast<uint2*>(oB + 8 * j + 4 * ql) =
-                  make_uint2(pack2<false>(acc[j][2] * dB, acc[j + 1][2] * dB), pack2<false>(acc[j][3] * dB, acc[j + 1][3] * dB));
-          }
+          *reinterpret_cast<float4*>(mine + qr * C::kMergeRow + 8 * j - c0 + 4 * ql) =
+              make_float4(acc[j][0], acc[j + 1][0], acc[j][1], acc[j + 1][1]);
+          *reinterpret_cast<float4*>(mine + (qr + 8) * C::kMergeRow + 8 * j - c0 + 4 * ql) =
+              make_float4(acc[j][2], acc[j + 1][2], acc[j][3], acc[j + 1][3]);
         }
-      } else {
-        const int64_t part = (int64_t)blockIdx.x * 2 + (njob > 0);
-        const int lrA = mt * 16 + qr, lrB = lrA + 8;
-        float* pA = a.acc + (part * a.rows + lrA) * D;
-        float* pB = a.acc + (part * a.rows + lrB) * D;
-        if (ql == 0) {
-          *reinterpret_cast<float2*>(a.ml + (part * a.rows + lrA) * 2) = make_float2(mA, lA);
-          *reinterpret_cast<float2*>(a.ml + (part * a.rows + lrB) * 2) = make_float2(mB, lB);
-        }
-        if constexpr (!F8) {
+      }
+      consumers_sync();
+#pragma unroll 1
+      for (int x = 0; x < MT; ++x) {
+        const int lr = x * 16 + orow, row = rb * a.rows + lr;  // row in the block, in the job's kv head
+        if (row < M) {
+          float m = -INFINITY;
 #pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            if (rA < M) *reinterpret_cast<float2*>(pA + 8 * j + 2 * ql) = make_float2(acc[j][0], acc[j][1]);
-            if (rB < M) *reinterpret_cast<float2*>(pB + 8 * j + 2 * ql) = make_float2(acc[j][2], acc[j][3]);
+          for (int k = 0; k < NG; ++k) m = fmaxf(m, merge_ml[(k * MT + x) * 16 + orow].x);
+          const float z = m == -INFINITY ? 0.f : m;
+          float l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < NG; ++k) {
+            const float2 ml = merge_ml[(k * MT + x) * 16 + orow];
+            const float f = ex2(ml.x - z);
+            l = fmaf(ml.y, f, l);
+            const float* from = merge + ((k * MT + x) * 16 + orow) * C::kMergeRow + ocol;
+            const float4 p0 = *reinterpret_cast<const float4*>(from), p1 = *reinterpret_cast<const float4*>(from + 4);
+            o[0] = fmaf(p0.x, f, o[0]);
+            o[1] = fmaf(p0.y, f, o[1]);
+            o[2] = fmaf(p0.z, f, o[2]);
+            o[3] = fmaf(p0.w, f, o[3]);
+            o[4] = fmaf(p1.x, f, o[4]);
+            o[5] = fmaf(p1.y, f, o[5]);
+            o[6] = fmaf(p1.z, f, o[6]);
+            o[7] = fmaf(p1.w, f, o[7]);
           }
-        } else {
-#pragma unroll
-          for (int j = 0; j < NT; j += 2) {
-            if (rA < M)
-              *reinterpret_cast<float4*>(pA + 8 * j + 4 * ql) = make_float4(acc[j][0], acc[j + 1][0], acc[j][1], acc[j + 1][1]);
-            if (rB < M)
-              *reinterpret_cast<float4*>(pB + 8 * j + 4 * ql) = make_float4(acc[j][2], acc[j + 1][2], acc[j][3], acc[j + 1][3]);
+          if (whole) {
+            const float d = l == 0.f ? 0.f : vs / l;  // an empty row is zero; a NaN sum stays
+            const int t = row / a.G;
+            uint16_t* dst = a.out + (((int64_t)w.b * a.Tq + t) * a.Hq + h * a.G + (row - t * a.G)) * D + c0 + ocol;
+            *reinterpret_cast<uint4*>(dst) = make_uint4(pack2<false>(o[0] * d, o[1] * d), pack2<false>(o[2] * d, o[3] * d),
+                                                        pack2<false>(o[4] * d, o[5] * d), pack2<false>(o[6] * d, o[7] * d));
+          } else {
+            const int64_t at = ((int64_t)blockIdx.x * 2 + (njob > 0)) * a.rows + lr;
+            if (c0 == 0 && ocol == 0) *reinterpret_cast<float2*>(a.ml + at * 2) = make_float2(m, l);
+            float4* dst = reinterpret_cast<float4*>(a.acc + at * D + c0 + ocol);
+            dst[0] = make_float4(o[0], o[1], o[2], o[3]);
+            dst[1] = make_float4(o[4], o[5], o[6], o[7]);
           }
         }
       }
+      consumers_sync();
     }
     ++njob;
     w.u += run;
@@ -656,35 +669,68 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   if (i0 >= i1) return;
   const int r0 = i0 / kCols, r1 = (i1 - 1) / kCols + 1;
   auto part = [&](int i) { return (int64_t)(c0 + i) * 2 + (i == 0 ? second : 0); };
+  // slices: the parts of an item over as many threads as the share leaves, a power of two up to 32
+  int slices = 1;
+  while (slices < 32 && (i1 - i0) * slices * 2 <= kJoinThreads) slices *= 2;
+  const int lanes = kJoinThreads / slices, sl = tid / lanes;
+  // the first four parts of the thread's first item are on their way while the weights are found
+  constexpr int kAhead = 4;
+  float4 ahead[kAhead];
+  {
+    const int it = min(i0 + tid % lanes, i1 - 1), r = it / kCols, col = it % kCols;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = sl + k * slices;
+      ahead[k] = i < parts ? *reinterpret_cast<const float4*>(a.acc + (part(i) * a.rows + r) * D + col * 4)
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  }
   for (int r = r0 + warp; r < r1; r += kJoinThreads / 32) {
+    float2 x[kAhead];
     float m = -INFINITY;
-    for (int i = lane; i < parts; i += 32) m = fmaxf(m, a.ml[(part(i) * a.rows + r) * 2]);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = lane + 32 * k;
+      x[k] = i < parts ? *reinterpret_cast<const float2*>(a.ml + (part(i) * a.rows + r) * 2) : make_float2(-INFINITY, 0.f);
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) m = fmaxf(m, x[k].x);
+    for (int i = lane + 32 * kAhead; i < parts; i += 32) m = fmaxf(m, a.ml[(part(i) * a.rows + r) * 2]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float z = m == -INFINITY ? 0.f : m;
     float l = 0.f;
-    for (int i = lane; i < parts; i += 32) {
-      const float2 x = *reinterpret_cast<const float2*>(a.ml + (part(i) * a.rows + r) * 2);
-      const float f = ex2(x.x - z);
+    for (int i = lane, k = 0; i < parts; i += 32, ++k) {
+      float2 v;
+      if (k < kAhead) v = k == 0 ? x[0] : (k == 1 ? x[1] : (k == 2 ? x[2] : x[3]));
+      else v = *reinterpret_cast<const float2*>(a.ml + (part(i) * a.rows + r) * 2);
+      const float f = ex2(v.x - z);
       wt[(r - r0) * parts + i] = f;
-      l = fmaf(x.y, f, l);
+      l = fmaf(v.y, f, l);
     }
     l = warp_sum(l);
     if (lane == 0) inv[r - r0] = l == 0.f ? 0.f : (a.v_scale ? a.v_scale[h] : 1.f) / l;
   }
   __syncthreads();
-  // slices: the parts of an item over as many threads as the share leaves, a power of two up to 32
-  int slices = 1;
-  while (slices < 32 && (i1 - i0) * slices * 2 <= kJoinThreads) slices *= 2;
-  const int lanes = kJoinThreads / slices, sl = tid / lanes;
   for (int base = i0; base < i1; base += lanes) {
     const int it = base + tid % lanes;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     if (it < i1) {
       const int r = it / kCols, col = it % kCols;
       const float* w = wt + (r - r0) * parts;
+      int i = sl;
+      if (base == i0) {
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k, i += slices) {
+          const float f = i < parts ? w[i] : 0.f;
+          s.x = fmaf(ahead[k].x, f, s.x);
+          s.y = fmaf(ahead[k].y, f, s.y);
+          s.z = fmaf(ahead[k].z, f, s.z);
+          s.w = fmaf(ahead[k].w, f, s.w);
+        }
+      }
 #pragma unroll 4
-      for (int i = sl; i < parts; i += slices) {
+      for (; i < parts; i += slices) {
         const float4 x = *reinterpret_cast<const float4*>(a.acc + (part(i) * a.rows + r) * D + col * 4);
         const float f = w[i];
         s.x = fmaf(x.x, f, s.x);
