@@ -5,6 +5,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/moe_paged.h"
 #include "moe_common.cuh"
 
@@ -95,12 +97,16 @@ inline cudaError_t paged_launch(const void* fn, dim3 grid, dim3 block, size_t sm
   return launched(cudaLaunchKernelExC(&cfg, fn, args));
 }
 
-// SMs of the current device (148 where there is none: the host-side checks run without a GPU).
+// SMs of the current device, asked once per device (148 where there is none: the host-side checks run without a GPU).
 inline int paged_sms() {
+  constexpr int kDevices = 64;
+  static std::atomic<int> known[kDevices];
   int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    n = 0;
-  return n > 0 ? n : 148;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev >= 0 && dev < kDevices && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+  if (dev >= 0 && dev < kDevices) known[dev].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 }  // namespace moe

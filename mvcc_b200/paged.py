@@ -18,17 +18,20 @@ KV_BF16, KV_E4M3 = 0, 1
 ERR_TIMEOUT, ERR_PAGE_ID, ERR_SEQ_ID, ERR_NO_PAGES, ERR_SHARED = 1 << 3, 1 << 8, 1 << 9, 1 << 10, 1 << 11
 
 
+_I16, _I32, _F32, _F64 = torch.int16, torch.int32, torch.float32, torch.float64
+
+
 def _need(ok, what):
     if not ok:
         raise ValueError(what)
 
 
-def raw_stream(device, stream=None):
-    """The handle of `stream`, or of the device's current stream. The library launches on the current device, so that
-    must be the one that holds the tensors."""
-    if device.index != torch.cuda.current_device():
-        raise ValueError(f"tensors on {device}, but the current device is cuda:{torch.cuda.current_device()}")
-    return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(device.index)
+def raw_stream(index, stream=None):
+    """The handle of `stream`, or of the current stream of device `index`, which holds the tensors. The library launches
+    on the current device, so that must be the same."""
+    if index != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors on cuda:{index}, but the current device is cuda:{torch.cuda.current_device()}")
+    return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(index)
 
 
 class PagedCache:
@@ -58,6 +61,7 @@ class PagedCache:
         self.k, self.v, self.tables, self.refs, self.lens = k, v, tables, refs, lens
         self.k_scale, self.v_scale = k_scale, v_scale
         self.device, self.Hq, self.max_batch, self.max_new = k.device, Hq, max_batch, max_new
+        self._dev = k.get_device()
         self.c = MoePagedCache(*[None if t is None else t.data_ptr() for t in (k, v, tables, refs, lens, k_scale,
                                                                                v_scale)],
                                self.layers, self.num_pages, self.page, self.Hkv, self.D, self.kv_type, self.max_seqs,
@@ -81,19 +85,26 @@ class PagedCache:
                    torch.zeros(num_pages, dtype=torch.int32, device=dev),
                    torch.zeros(max_seqs, dtype=torch.int32, device=dev), Hq, max_batch, max_new, k_scale, v_scale)
 
-    def _list(self, t, what, n=None):
-        _need(t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and t.device == self.device
-              and (n is None or t.numel() == n), f"{what}: expected a contiguous int32 list on {self.device}")
+    # The calls below are a few microseconds of host time each, so their checks are written out rather than shared.
+    def _list(self, t, what, n):
+        if t.dtype is not _I32 or t.numel() != n or t.dim() != 1 or not t.is_contiguous() or t.get_device() != self._dev:
+            raise ValueError(f"{what}: expected a contiguous int32 list of {n} on {self.device}")
         return t.data_ptr()
 
     def _rows(self, t, what, n):
-        _need(t.dtype == torch.int16 and t.is_contiguous() and t.device == self.device and t.numel() == n,
-              f"{what}: expected {n} contiguous bf16 values (int16 bits) on {self.device}")
+        if t.dtype is not _I16 or t.numel() != n or not t.is_contiguous() or t.get_device() != self._dev:
+            raise ValueError(f"{what}: expected {n} contiguous bf16 values (int16 bits) on {self.device}")
         return t.data_ptr()
+
+    def _batch(self, seqs):
+        B = seqs.numel()
+        if B > self.max_batch:
+            raise ValueError(f"a list of {B} sequences: max_batch is {self.max_batch}")
+        return B
 
     def error_word(self, stream=None):
         """Reads and clears the workspace's error word (the ERR_ bits of this module)."""
-        rc = _lib.moe_paged_workspace_error(*self._ws, raw_stream(self.device, stream))
+        rc = _lib.moe_paged_workspace_error(*self._ws, raw_stream(self._dev, stream))
         if rc < 0:
             raise MoeError(f"moe_paged_workspace_error failed: cudaError {-rc}")
         return rc
@@ -101,53 +112,56 @@ class PagedCache:
     def resize(self, seqs, new_lens, stream=None):
         """Sets the listed sequences' lengths: pages are released, taken, or copied where a partly filled last page is
         shared."""
-        n = seqs.numel()
-        _need(n <= self.max_batch, f"a list of {n} sequences: max_batch is {self.max_batch}")
-        _check(_lib.moe_paged_resize(self._c, self._list(seqs, "seqs"), self._list(new_lens, "new_lens", n), n,
-                                     *self._ws, raw_stream(self.device, stream)), "moe_paged_resize")
+        n = self._batch(seqs)
+        _check(_lib.moe_paged_resize(self._c, self._list(seqs, "seqs", n), self._list(new_lens, "new_lens", n), n,
+                                     *self._ws, raw_stream(self._dev, stream)), "moe_paged_resize")
 
     def fork(self, src, dst, stream=None):
         """Makes each empty dst sequence share all pages of its src."""
-        n = src.numel()
-        _need(n <= self.max_batch, f"a list of {n} sequences: max_batch is {self.max_batch}")
-        _check(_lib.moe_paged_fork(self._c, self._list(src, "src"), self._list(dst, "dst", n), n, *self._ws,
-                                   raw_stream(self.device, stream)), "moe_paged_fork")
+        n = self._batch(src)
+        _check(_lib.moe_paged_fork(self._c, self._list(src, "src", n), self._list(dst, "dst", n), n, *self._ws,
+                                   raw_stream(self._dev, stream)), "moe_paged_fork")
 
     def compact(self, stream=None):
         """Moves the live pages to the lowest ids."""
-        _check(_lib.moe_paged_compact(self._c, *self._ws, raw_stream(self.device, stream)), "moe_paged_compact")
+        _check(_lib.moe_paged_compact(self._c, *self._ws, raw_stream(self._dev, stream)), "moe_paged_compact")
 
     def copy_pages(self, src, dst, stream=None):
         """Copies whole pages src[i] to dst[i] in every layer."""
         n = src.numel()
-        _check(_lib.moe_paged_copy(self._c, self._list(src, "src"), self._list(dst, "dst", n), n, *self._ws,
-                                   raw_stream(self.device, stream)), "moe_paged_copy")
+        _check(_lib.moe_paged_copy(self._c, self._list(src, "src", n), self._list(dst, "dst", n), n, *self._ws,
+                                   raw_stream(self._dev, stream)), "moe_paged_copy")
 
     def append(self, layer, seqs, qkv, q_out, Tq=1, q_norm=None, k_norm=None, inv_freq=None, eps=1e-6, stream=None):
         """Norm, rotation and write of the new tokens' keys and values; q_out receives their queries."""
-        B, D = seqs.numel(), self.D
-        _need(B <= self.max_batch, f"a batch of {B}: max_batch is {self.max_batch}")
+        B, D = self._batch(seqs), self.D
+        T = B * Tq
+        freq = pairs = 0
         if inv_freq is not None:
-            _need(inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous()
-                  and inv_freq.device == self.device, "inv_freq: expected a contiguous float64 list")
-        _check(_lib.moe_paged_append(
-            self._c, layer, self._list(seqs, "seqs"), B, Tq,
-            self._rows(qkv, "qkv", B * Tq * (self.Hq + 2 * self.Hkv) * D), self.Hq,
+            pairs = inv_freq.numel()
+            if inv_freq.dtype is not _F64 or not inv_freq.is_contiguous() or inv_freq.get_device() != self._dev:
+                raise ValueError("inv_freq: expected a contiguous float64 list")
+            freq = inv_freq.data_ptr()
+        rc = _lib.moe_paged_append(
+            self._c, layer, self._list(seqs, "seqs", B), B, Tq,
+            self._rows(qkv, "qkv", T * (self.Hq + 2 * self.Hkv) * D), self.Hq,
             None if q_norm is None else self._rows(q_norm, "q_norm", D),
-            None if k_norm is None else self._rows(k_norm, "k_norm", D),
-            None if inv_freq is None else inv_freq.data_ptr(), 0 if inv_freq is None else 2 * inv_freq.numel(), eps,
-            self._rows(q_out, "q_out", B * Tq * self.Hq * D), *self._ws, raw_stream(self.device, stream)),
-            "moe_paged_append")
+            None if k_norm is None else self._rows(k_norm, "k_norm", D), freq or None, 2 * pairs, eps,
+            self._rows(q_out, "q_out", T * self.Hq * D), *self._ws, raw_stream(self._dev, stream))
+        if rc:
+            _check(rc, "moe_paged_append")
 
     def attend(self, layer, seqs, q, out, Tq=1, scale=None, stream=None):
         """Causal attention of the new tokens over their sequences' keys and values (scale: D^-1/2)."""
-        B = seqs.numel()
-        _need(B <= self.max_batch and Tq <= self.max_new,
-              f"a batch of {B} x {Tq}: max_batch is {self.max_batch}, max_new {self.max_new}")
+        B = self._batch(seqs)
+        if Tq > self.max_new:
+            raise ValueError(f"{Tq} new tokens a sequence: max_new is {self.max_new}")
         n = B * Tq * self.Hq * self.D
-        _check(_lib.moe_paged_attend(self._c, layer, self._list(seqs, "seqs"), B, Tq, self._rows(q, "q", n), self.Hq,
-                                     self._default_scale if scale is None else scale, self._rows(out, "out", n),
-                                     *self._ws, raw_stream(self.device, stream)), "moe_paged_attend")
+        rc = _lib.moe_paged_attend(self._c, layer, self._list(seqs, "seqs", B), B, Tq, self._rows(q, "q", n), self.Hq,
+                                   self._default_scale if scale is None else scale, self._rows(out, "out", n),
+                                   *self._ws, raw_stream(self._dev, stream))
+        if rc:
+            _check(rc, "moe_paged_attend")
 
 
 def inv_frequencies(shape, device="cuda"):
@@ -174,7 +188,7 @@ class PagedAttnBlock:
         torch.cuda.current_stream(cache.device).synchronize()
 
     def error_word(self, stream=None):
-        rc = _lib.moe_paged_workspace_error(_ptr(self.ws), self.ws.numel(), raw_stream(self.cache.device, stream))
+        rc = _lib.moe_paged_workspace_error(_ptr(self.ws), self.ws.numel(), raw_stream(self.cache._dev, stream))
         if rc < 0:
             raise MoeError(f"moe_paged_workspace_error failed: cudaError {-rc}")
         return rc
@@ -182,15 +196,16 @@ class PagedAttnBlock:
     def forward_rms(self, hidden, rms1, attn_out, seqs, Tq=1, stream=None):
         """AttnBlock.forward_rms for the batch: hidden fp32 [B Tq, H], attn_out bf16 bits [B Tq, H]; the sequences' lens
         already count the new tokens."""
-        c, H, B = self.cache, self.layer.shape.H, seqs.numel()
-        _need(B <= c.max_batch and Tq <= c.max_new, f"a batch of {B} x {Tq}: max_batch is {c.max_batch}, max_new "
-                                                    f"{c.max_new}")
-        _need(hidden.dtype == torch.float32 and hidden.is_contiguous() and hidden.device == c.device
-              and hidden.numel() == B * Tq * H, f"hidden: expected contiguous float32 [{B * Tq}, {H}]")
+        c, H = self.cache, self.layer.shape.H
+        B = c._batch(seqs)
+        _need(Tq <= c.max_new, f"{Tq} new tokens a sequence: max_new is {c.max_new}")
+        if hidden.dtype is not _F32 or hidden.numel() != B * Tq * H or not hidden.is_contiguous() \
+                or hidden.get_device() != c._dev:
+            raise ValueError(f"hidden: expected contiguous float32 [{B * Tq}, {H}] on {c.device}")
         _check(_lib.moe_attn_paged_forward_rms(
             ctypes.byref(self.layer.c), c._rows(rms1, "rms1", H), hidden.data_ptr(), c._c, self.index,
-            c._list(seqs, "seqs"), B, Tq, self.inv_freq.data_ptr(), c._rows(attn_out, "attn_out", B * Tq * H),
-            _ptr(self.ws), self.ws.numel(), raw_stream(c.device, stream)), "moe_attn_paged_forward_rms")
+            c._list(seqs, "seqs", B), B, Tq, self.inv_freq.data_ptr(), c._rows(attn_out, "attn_out", B * Tq * H),
+            _ptr(self.ws), self.ws.numel(), raw_stream(c._dev, stream)), "moe_attn_paged_forward_rms")
 
 
 class PagedDecodeStack:

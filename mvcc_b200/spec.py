@@ -4,7 +4,7 @@ streams only."""
 import torch
 
 from . import _check, _lib
-from .paged import _need, raw_stream
+from .paged import _F32, _I32, _need, raw_stream
 
 
 def lm_head_logits(weight, normed, logits, stream=None):
@@ -17,7 +17,7 @@ def lm_head_logits(weight, normed, logits, stream=None):
           and normed.numel() == T * H and normed.device == dev, "weight [V, H], normed [T, H]: contiguous bf16 bits")
     _need(logits.dtype == torch.float32 and logits.is_contiguous() and logits.numel() == T * V and logits.device == dev,
           f"logits: expected contiguous float32 [{T}, {V}]")
-    s = raw_stream(dev, stream)
+    s = raw_stream(weight.get_device(), stream)
     for t in range(0, T, 4):
         _check(_lib.moe_lm_head_logits(normed.data_ptr() + t * H * 2, weight.data_ptr(), V, H, min(4, T - t),
                                        logits.data_ptr() + t * V * 4, s), "moe_lm_head_logits")
@@ -27,17 +27,27 @@ def softmax_rows(logits, probs, temperature=None, stream=None):
     """probs = softmax(logits / temperature) over the last dimension, row by row: fp32 [R, V], rows any distance apart;
     temperature fp32 [R], 0 for a one-hot row at the largest logit. probs may be logits."""
     R, V = logits.shape
-    dev = logits.device
-    _need(logits.dtype == probs.dtype == torch.float32 and probs.shape == logits.shape and probs.device == dev
-          and (V == 1 or logits.stride(1) == probs.stride(1) == 1), "logits, probs: float32 [R, V] on one GPU, each row "
-                                                                    "contiguous")
-    _need(temperature is None or (temperature.dtype == torch.float32 and temperature.shape == (R,)
-                                  and temperature.is_contiguous() and temperature.device == dev),
-          f"temperature: expected contiguous float32 ({R},)")
-    # the distance between rows means nothing for one row (torch allows any value there)
-    ldx, ldy = (logits.stride(0), probs.stride(0)) if R > 1 else (V, V)
-    _check(_lib.moe_softmax_rows(logits.data_ptr(), ldx, R, V, None if temperature is None else temperature.data_ptr(),
-                                 probs.data_ptr(), ldy, raw_stream(dev, stream)), "moe_softmax_rows")
+    dev = logits.get_device()
+    ldx, unit_x = logits.stride()
+    ldy, unit_y = probs.stride()
+    if logits.dtype is not _F32 or probs.dtype is not _F32 or probs.shape != logits.shape or probs.get_device() != dev \
+            or (V > 1 and (unit_x != 1 or unit_y != 1)) or dev < 0:
+        raise ValueError("logits, probs: expected float32 [R, V] on one GPU, each row contiguous")
+    t = None
+    if temperature is not None:
+        if temperature.dtype is not _F32 or temperature.numel() != R or not temperature.is_contiguous() \
+                or temperature.get_device() != dev:
+            raise ValueError(f"temperature: expected contiguous float32 ({R},)")
+        t = temperature.data_ptr()
+    if R < 2:
+        ldx = ldy = V  # torch allows any distance between the rows of one
+    rc = _lib.moe_softmax_rows(logits.data_ptr(), ldx, R, V, t, probs.data_ptr(), ldy, raw_stream(dev, stream))
+    if rc:
+        _check(rc, "moe_softmax_rows")
+
+
+def _dense(t, dtype, n, dev):
+    return t.dtype is dtype and t.numel() == n and t.is_contiguous() and t.get_device() == dev
 
 
 class SpecVerifier:
@@ -49,7 +59,8 @@ class SpecVerifier:
         if n == 0 or not 1 <= K <= 64:
             raise ValueError("unsupported sizes for the verification of drafts")
         self.ws = torch.zeros(n, dtype=torch.uint8, device=device)
-        self.device = self.ws.device
+        self.device, self._dev = self.ws.device, self.ws.get_device()
+        self._ws = (self.ws.data_ptr(), n)
         torch.cuda.current_stream(self.device).synchronize()
 
     def verify(self, target, draft, drafted, u, tokens, accepted, n_drafted=None, stream=None):
@@ -57,23 +68,30 @@ class SpecVerifier:
         fp32 [B, K + 1] in [0, 1), n_drafted int32 [B] or None -> tokens int32 [B, K + 1] (-1 behind the drawn one),
         accepted int32 [B]."""
         B, K1, V = target.shape
-        K = K1 - 1
-        _need(1 <= B <= self.max_B and K == self.K and V == self.V,
-              f"target [{B}, {K1}, {V}]: the verifier takes up to {self.max_B} x {self.K + 1} x {self.V}")
-        for n, t, rows in (("target", target, K1), ("draft", draft, K)):
-            _need(t is None or (t.dtype == torch.float32 and t.shape == (B, rows, V) and t.device == self.device
-                                and (V == 1 or t.stride(2) == 1) and t.stride(1) >= V
-                                and (B == 1 or t.stride(0) == rows * t.stride(1))),
-                  f"{n}: expected float32 [{B}, {rows}, {V}] on {self.device}, rows one distance apart")
-        for n, t, shape, dt in (("drafted", drafted, (B, K), torch.int32), ("u", u, (B, K1), torch.float32),
-                                ("tokens", tokens, (B, K1), torch.int32), ("accepted", accepted, (B,), torch.int32),
-                                ("n_drafted", n_drafted, (B,), torch.int32)):
-            _need((t is None and n == "n_drafted") or (t.dtype == dt and t.shape == shape and t.is_contiguous()
-                                                       and t.device == self.device),
-                  f"{n}: expected contiguous {dt} {shape} on {self.device}")
-        _check(_lib.moe_spec_verify(
-            target.data_ptr(), target.stride(1), None if draft is None else draft.data_ptr(),
-            0 if draft is None else draft.stride(1), drafted.data_ptr(),
-            None if n_drafted is None else n_drafted.data_ptr(), u.data_ptr(), B, K, V, tokens.data_ptr(),
-            accepted.data_ptr(), self.ws.data_ptr(), self.ws.numel(), raw_stream(self.device, stream)),
-            "moe_spec_verify")
+        K, dev = self.K, self._dev
+        if B > self.max_B or K1 != K + 1 or V != self.V:
+            raise ValueError(f"target {tuple(target.shape)}: the verifier takes up to {self.max_B} x {K + 1} x {self.V}")
+        ldp = self._rows(target, "target", B, K1)
+        ldq, q = 0, None
+        if draft is not None:
+            ldq, q = self._rows(draft, "draft", B, K), draft.data_ptr()
+        if not (_dense(drafted, _I32, B * K, dev) and _dense(u, _F32, B * K1, dev) and _dense(tokens, _I32, B * K1, dev)
+                and _dense(accepted, _I32, B, dev)):
+            raise ValueError(f"expected contiguous drafted int32 ({B}, {K}), u float32 ({B}, {K1}), tokens int32 "
+                             f"({B}, {K1}) and accepted int32 ({B},) on {self.device}")
+        n = None
+        if n_drafted is not None:
+            _need(_dense(n_drafted, _I32, B, dev), f"n_drafted: expected contiguous int32 ({B},) on {self.device}")
+            n = n_drafted.data_ptr()
+        rc = _lib.moe_spec_verify(target.data_ptr(), ldp, q, ldq, drafted.data_ptr(), n, u.data_ptr(), B, K, V,
+                                  tokens.data_ptr(), accepted.data_ptr(), *self._ws, raw_stream(dev, stream))
+        if rc:
+            _check(rc, "moe_spec_verify")
+
+    def _rows(self, t, what, B, rows):
+        """The distance between the rows of t [B, rows, V], one for all of them."""
+        s0, s1, s2 = t.stride()
+        if t.dtype is not _F32 or t.shape != (B, rows, self.V) or t.get_device() != self._dev \
+                or (s2 != 1 and self.V > 1) or s1 < self.V or (B > 1 and s0 != rows * s1):
+            raise ValueError(f"{what}: expected float32 [{B}, {rows}, {self.V}] on {self.device}, rows one distance apart")
+        return s1
