@@ -111,7 +111,7 @@ MOE_API int moe_paged_copy(const moe_paged_cache* c, const int32_t* src, const i
  * this model theta^(-2 d / rope_dim); the angle is formed and reduced in fp64, so far positions keep their accuracy;
  * rope_dim 0 with inv_freq NULL = no rotation). q goes to q_out bf16 [B Tq][Hq D]; k and v go into the pages at the
  * tokens' positions, for e4m3 as x / scale rounded to nearest even and saturated. B <= 2048, B * Tq < 2^24, rope_dim
- * even and <= D. Rows of unused slots and of no token are left as they were. */
+ * even and <= D; qkv, q_out and the norms 16-byte aligned. Rows of unused slots and of no token are left as they were. */
 MOE_API int moe_paged_append(const moe_paged_cache* c, int layer, const int32_t* seqs, int B, int Tq,
                              const uint16_t* qkv, int Hq, const uint16_t* q_norm, const uint16_t* k_norm,
                              const double* inv_freq, int rope_dim, float eps, uint16_t* q_out, void* workspace,

@@ -389,121 +389,225 @@ struct AppendArgs {
 };
 
 constexpr int kAppendWarps = 8;
+constexpr int kAppendMany = 4;  // tokens a CTA where there are many
 
-// A CTA takes eight heads of one token, a warp each: the token's angles are formed once per CTA (in fp64: position times
-// frequency, in half turns, reduced to [-1, 1] before the fp32 sine and cosine) and shared. Lane owns D / 32
-// consecutive values; the pairs of the rotation meet in shared memory.
-template <int D, bool F8>
-__global__ void __launch_bounds__(kAppendWarps * 32) append_kernel(const __grid_constant__ AppendArgs a) {
-  constexpr int E = D / 32;
-  __shared__ float cs[D / 2], sn[D / 2];
-  __shared__ __align__(16) float rows[kAppendWarps][D];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int tok = blockIdx.x, b = tok / a.Tq, t = tok - b * a.Tq;
-  const int heads = a.Hq + 2 * a.Hkv, h = blockIdx.y * kAppendWarps + warp, half = a.rope_dim >> 1;
+// Packed pairs of fp32 (sm_100a): two roundings to nearest an instruction.
+__device__ __forceinline__ u64 pair(float lo, float hi) {
+  return ((u64)__float_as_uint(hi) << 32) | __float_as_uint(lo);
+}
+__device__ __forceinline__ u64 mul2(u64 x, u64 y) {
+  u64 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
+__device__ __forceinline__ u64 fma2(u64 x, u64 y, u64 z) {
+  u64 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+  return r;
+}
+
+// A CTA takes TT tokens: their positions are looked up and their angles formed once (in fp64: position times frequency,
+// in half turns, reduced to [-1, 1] before the fp32 sine and cosine), while the first rows are on their way. A head is
+// L = D / 16 lanes of 16 values, the chunks of eight lane and lane + L; a warp takes 32 / L heads of a token at a time
+// and fetches the next ones before it works on these. The pairs of the rotation meet by shuffles, in one lane (rope_dim
+// = D), or in shared memory where they lie at different places of two lanes. TT = 1 and several CTAs a token where the
+// CTAs of TT = 4 would not fill the GPU twice.
+template <int D, bool F8, int TT>
+__global__ void __launch_bounds__(kAppendWarps * 32, 4) append_kernel(const __grid_constant__ AppendArgs a) {
+  constexpr int L = D / 16, kHeads = 32 / L;
+  __shared__ __align__(16) float cs[TT][D / 2], sn[TT][D / 2];
+  __shared__ __align__(16) float rows[kAppendWarps][kHeads][D];
+  __shared__ int seq_s[TT], pos_s[TT];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hl = lane % L, hw = lane / L;
+  const int tok0 = blockIdx.x * TT, T = a.B * a.Tq, here = min(TT, T - tok0);
+  const int heads = a.Hq + 2 * a.Hkv, half = a.rope_dim >> 1;
+  // this CTA's share of the (token, group of heads) items, token by token, a warp every kAppendWarps-th
+  const int groups = (heads + kHeads - 1) / kHeads, items = here * groups;
+  const int begin = (int)((int64_t)items * blockIdx.y / gridDim.y), end = (int)((int64_t)items * (blockIdx.y + 1) / gridDim.y);
+  struct Item {
+    int k, g, left;  // token, group, items from this one to the end
+    __device__ __forceinline__ void on(int groups) {
+      left -= kAppendWarps;
+      for (g += kAppendWarps; g >= groups; g -= groups) ++k;
+    }
+  };
+  Item cur, ahead;
+  ahead.k = (begin + warp) / groups;
+  ahead.g = begin + warp - ahead.k * groups;
+  ahead.left = end - begin - warp;
+  cur = ahead;
   pdl_wait();
   pdl_launch_dependents();
-  const int s = a.seqs[b];
-  if (s < 0 || s >= a.max_seqs) {
-    if (s != -1 && tid == 0) atomicOr(a.err, (uint32_t)MOE_ERR_SEQ_ID);
-    return;
-  }
-  const int len = a.lens[s], pos = len - a.Tq + t;
-  if (len < 0 || len > a.max_pages * a.page) {
-    if (tid == 0) atomicOr(a.err, (uint32_t)MOE_ERR_SEQ_ID);
-    return;
-  }
-  if (pos < 0) return;
-  for (int d = tid; d < half; d += kAppendWarps * 32) {
-    double x = (double)pos * a.inv_freq[d] * 0.31830988618379067154;  // 1 / pi
-    x -= 2.0 * rint(0.5 * x);
-    sincospif((float)x, &sn[d], &cs[d]);
+  const uint4* const qkv0 = reinterpret_cast<const uint4*>(a.qkv + (int64_t)tok0 * heads * D) + hl;
+  auto fetch = [&](const Item& it, uint4 (&x)[2]) {
+    const int h = it.g * kHeads + hw;
+    if (it.left > 0 && h < heads) {
+      const uint4* src = qkv0 + (it.k * heads + h) * (D / 8);
+      x[0] = src[0];
+      x[1] = src[L];
+    }
+  };
+  uint4 next[2];
+  fetch(ahead, next);
+  // the tokens: sequence and position (-1: none, or a fault)
+  if (tid < TT) {
+    const int tok = tok0 + tid, b = tok / a.Tq, t = tok - b * a.Tq;
+    int pos = -1;
+    const int s = tok < T ? a.seqs[b] : -1;
+    if (s >= 0 && s < a.max_seqs) {
+      const int len = a.lens[s];
+      if (len >= 0 && len <= a.max_pages * a.page) pos = max(-1, len - a.Tq + t);
+      else atomicOr(a.err, (uint32_t)MOE_ERR_SEQ_ID);
+    } else if (s != -1) {
+      atomicOr(a.err, (uint32_t)MOE_ERR_SEQ_ID);
+    }
+    seq_s[tid] = s;
+    pos_s[tid] = pos;
   }
   __syncthreads();
-  if (h >= heads) return;
-  float v[E];
-  {
-    const uint16_t* src = a.qkv + ((int64_t)tok * heads + h) * D + lane * E;
-    uint32_t w[E / 2];
-    if constexpr (E == 8) {
-      const uint4 x = *reinterpret_cast<const uint4*>(src);
-      w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
-    } else if constexpr (E == 4) {
-      const uint2 x = *reinterpret_cast<const uint2*>(src);
-      w[0] = x.x; w[1] = x.y;
-    } else {
-      w[0] = *reinterpret_cast<const uint32_t*>(src);
-    }
-#pragma unroll
-    for (int i = 0; i < E / 2; ++i) {
-      v[2 * i] = lo_bf(w[i]);
-      v[2 * i + 1] = hi_bf(w[i]);
-    }
+  for (int i = tid; i < TT * half; i += kAppendWarps * 32) {
+    const int k = i / half, d = i - k * half;
+    double x = (double)pos_s[k] * a.inv_freq[d] * 0.31830988618379067154;  // 1 / pi
+    x -= 2.0 * rint(0.5 * x);
+    sincospif((float)x, &sn[k][d], &cs[k][d]);
   }
-  const bool is_v = h >= a.Hq + a.Hkv, is_q = h < a.Hq;
-  if (!is_v) {
-    const uint16_t* norm = is_q ? a.q_norm : a.k_norm;
-    if (norm) {
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < E; ++i) ss = fmaf(v[i], v[i], ss);
-      const float inv = rsqrtf(warp_sum(ss) / (float)D + a.eps);
-#pragma unroll
-      for (int i = 0; i < E; ++i) v[i] = v[i] * inv * bf2f(norm[lane * E + i]);
-    }
-    if (half) {
-      float* r = rows[warp];
-#pragma unroll
-      for (int i = 0; i < E; ++i) r[lane * E + i] = v[i];
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const int d = lane * E + i;
-        if (d < half) v[i] = v[i] * cs[d] - r[d + half] * sn[d];
-        else if (d < 2 * half) v[i] = v[i] * cs[d - half] + r[d - half] * sn[d - half];
+  __syncthreads();
+  const bool by_lane = half == D / 2, by_shuffle = half % 8 == 0 && 4 * half <= D;
+  for (; cur.left > 0; cur = ahead) {
+    uint4 raw[2] = {next[0], next[1]};
+    ahead.on(groups);
+    fetch(ahead, next);
+    const int k = cur.k, h = cur.g * kHeads + hw, pos = pos_s[k];
+    if (pos < 0) continue;  // the same for the whole warp
+    const bool there = h < heads, is_q = h < a.Hq, is_v = h >= a.Hq + a.Hkv;
+    // a key's or value's page (-1: not to be written)
+    int page = -1;
+    if (there && !is_q) {
+      page = a.tables[(int64_t)seq_s[k] * a.max_pages + pos / a.page];
+      if (page < 0 || page >= a.num_pages) {
+        atomicOr(a.err, (uint32_t)MOE_ERR_PAGE_ID);
+        page = -1;
+      } else if (a.refs[page] != 1) {
+        atomicOr(a.err, (uint32_t)MOE_ERR_SHARED);
+        page = -1;
       }
     }
-  }
-  uint32_t o[E / 2];
+    float v[2][8];
 #pragma unroll
-  for (int i = 0; i < E / 2; ++i) o[i] = (uint32_t)f2bf(v[2 * i]) | ((uint32_t)f2bf(v[2 * i + 1]) << 16);
-  auto store = [&](uint16_t* dst) {
-    if constexpr (E == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
-    else if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(o[0], o[1]);
-    else *reinterpret_cast<uint32_t*>(dst) = o[0];
-  };
-  if (is_q) {
-    store(a.q_out + ((int64_t)tok * a.Hq + h) * D + lane * E);
-    return;
-  }
-  const int kvh = h - a.Hq - (is_v ? a.Hkv : 0);
-  const int pid = a.tables[(int64_t)s * a.max_pages + pos / a.page];
-  if (pid < 0 || pid >= a.num_pages) {
-    if (lane == 0) atomicOr(a.err, (uint32_t)MOE_ERR_PAGE_ID);
-    return;
-  }
-  if (a.refs[pid] != 1) {
-    if (lane == 0) atomicOr(a.err, (uint32_t)MOE_ERR_SHARED);
-    return;
-  }
-  const int64_t at = (((int64_t)pid * a.Hkv + kvh) * a.page + pos % a.page) * D + lane * E;
-  uint8_t* pool = is_v ? a.v : a.k;
-  if constexpr (!F8) {
-    store(reinterpret_cast<uint16_t*>(pool) + at);
-  } else {
-    const float* sp = is_v ? a.v_scale : a.k_scale;
-    const float sc = sp ? sp[kvh] : 1.f;
-    uint32_t q[E / 4];
-#pragma unroll
-    for (int i = 0; i < E / 4; ++i) {
-      uint32_t w = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        w |= (uint32_t)__nv_cvt_float_to_fp8(__fdiv_rn(v[4 * i + j], sc), __NV_SATFINITE, __NV_E4M3) << (8 * j);
-      q[i] = w;
+    for (int c = 0; c < 2; ++c) {
+      v[c][0] = lo_bf(raw[c].x); v[c][1] = hi_bf(raw[c].x); v[c][2] = lo_bf(raw[c].y); v[c][3] = hi_bf(raw[c].y);
+      v[c][4] = lo_bf(raw[c].z); v[c][5] = hi_bf(raw[c].z); v[c][6] = lo_bf(raw[c].w); v[c][7] = hi_bf(raw[c].w);
     }
-    if constexpr (E == 8) *reinterpret_cast<uint2*>(pool + at) = make_uint2(q[0], q[1]);
-    else *reinterpret_cast<uint32_t*>(pool + at) = q[0];
+    if (a.q_norm) {
+      u64 s2 = 0ull;
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const u64 x = pair(v[i >> 3][i & 7], v[i >> 3][(i & 7) + 1]);
+        s2 = fma2(x, x, s2);
+      }
+      float ss = lo_f(s2) + hi_f(s2);
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (!is_v) {
+        const float inv = rsqrtf(ss * (1.f / (float)D) + a.eps);
+        const u64 inv2 = pair(inv, inv);
+        const uint4* norm = reinterpret_cast<const uint4*>(is_q ? a.q_norm : a.k_norm);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint4 w4 = norm[hl + c * L];
+          const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const u64 x = mul2(mul2(pair(v[c][2 * i], v[c][2 * i + 1]), inv2), pair(lo_bf(w[i]), hi_bf(w[i])));
+            v[c][2 * i] = lo_f(x);
+            v[c][2 * i + 1] = hi_f(x);
+          }
+        }
+      }
+    }
+    if (by_lane) {
+      if (!is_v) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+          const float4 c4 = *reinterpret_cast<const float4*>(&cs[k][hl * 8 + i]);
+          const float4 s4 = *reinterpret_cast<const float4*>(&sn[k][hl * 8 + i]);
+          const float cc[4] = {c4.x, c4.y, c4.z, c4.w}, ss[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float x = v[0][i + j], y = v[1][i + j];
+            v[0][i + j] = x * cc[j] - y * ss[j];
+            v[1][i + j] = y * cc[j] + x * ss[j];
+          }
+        }
+      }
+    } else if (by_shuffle && half) {
+      const int hc = half / 8;  // the pair's second chunk is hc lanes on
+      const bool low = hl < hc, rot = hl < 2 * hc;
+      const int from = low ? lane + hc : (rot ? lane - hc : lane), d0 = (low ? hl : hl - hc) * 8;
+      float other[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(0xffffffffu, v[0][i], from);
+      if (rot && !is_v) {
+        const float sign = low ? -1.f : 1.f;
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+          const float4 c4 = *reinterpret_cast<const float4*>(&cs[k][d0 + i]);
+          const float4 s4 = *reinterpret_cast<const float4*>(&sn[k][d0 + i]);
+          v[0][i] = fmaf(v[0][i], c4.x, sign * other[i] * s4.x);
+          v[0][i + 1] = fmaf(v[0][i + 1], c4.y, sign * other[i + 1] * s4.y);
+          v[0][i + 2] = fmaf(v[0][i + 2], c4.z, sign * other[i + 2] * s4.z);
+          v[0][i + 3] = fmaf(v[0][i + 3], c4.w, sign * other[i + 3] * s4.w);
+        }
+      }
+    } else if (half) {
+      float* r = rows[warp][hw];
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) r[(i >> 3) * (D / 2) + hl * 8 + (i & 7)] = v[i >> 3][i & 7];
+      __syncwarp();
+      if (!is_v) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int d = (i >> 3) * (D / 2) + hl * 8 + (i & 7);
+          float& x = v[i >> 3][i & 7];
+          if (d < half) x = x * cs[k][d] - r[d + half] * sn[k][d];
+          else if (d < 2 * half) x = x * cs[k][d - half] + r[d - half] * sn[k][d - half];
+        }
+      }
+    }
+    if (!there) continue;
+    auto two = [](float x, float y) {
+      const __nv_bfloat162 p = __floats2bfloat162_rn(x, y);
+      return *reinterpret_cast<const uint32_t*>(&p);
+    };
+    if (is_q || !F8) {
+      if (!is_q && page < 0) continue;
+      const int kvh = h - a.Hq - (is_v ? a.Hkv : 0);
+      uint16_t* dst = is_q ? a.q_out + ((int64_t)(tok0 + k) * a.Hq + h) * D
+                           : reinterpret_cast<uint16_t*>(is_v ? a.v : a.k) +
+                                 (((int64_t)page * a.Hkv + kvh) * a.page + pos % a.page) * D;
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        reinterpret_cast<uint4*>(dst)[hl + c * L] = make_uint4(two(v[c][0], v[c][1]), two(v[c][2], v[c][3]),
+                                                               two(v[c][4], v[c][5]), two(v[c][6], v[c][7]));
+    } else if (page >= 0) {
+      const int kvh = h - a.Hq - (is_v ? a.Hkv : 0);
+      const float* sp = is_v ? a.v_scale : a.k_scale;
+      const float sc = sp ? sp[kvh] : 1.f;
+      uint8_t* dst = (is_v ? a.v : a.k) + (((int64_t)page * a.Hkv + kvh) * a.page + pos % a.page) * D;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t q[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          q[i] = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            q[i] |= (uint32_t)__nv_cvt_float_to_fp8(__fdiv_rn(v[c][4 * i + j], sc), __NV_SATFINITE, __NV_E4M3) << (8 * j);
+        }
+        reinterpret_cast<uint2*>(dst)[hl + c * L] = make_uint2(q[0], q[1]);
+      }
+    }
   }
 }
 
@@ -511,8 +615,13 @@ template <int D, bool F8>
 cudaError_t launch_append(const AppendArgs& a, cudaStream_t s) {
   AppendArgs arg = a;
   void* args[] = {&arg};
-  const dim3 grid(a.B * a.Tq, (a.Hq + 2 * a.Hkv + kAppendWarps - 1) / kAppendWarps);
-  return paged_launch(reinterpret_cast<const void*>(append_kernel<D, F8>), grid, dim3(kAppendWarps * 32), 0, s, args);
+  const int T = a.B * a.Tq, per_token = (a.Hq + 2 * a.Hkv + 512 / D - 1) / (512 / D);
+  const bool many = T > paged_sms() * 2 * kAppendMany;
+  const void* fn = many ? reinterpret_cast<const void*>(append_kernel<D, F8, kAppendMany>)
+                        : reinterpret_cast<const void*>(append_kernel<D, F8, 1>);
+  const dim3 grid(many ? (T + kAppendMany - 1) / kAppendMany : T,
+                  many ? 1 : (per_token + kAppendWarps - 1) / kAppendWarps);
+  return paged_launch(fn, grid, dim3(kAppendWarps * 32), 0, s, args);
 }
 
 PageArgs page_args(const moe_paged_cache* c, const int32_t* x, const int32_t* y, int n, void* workspace,
@@ -654,7 +763,7 @@ int moe_paged_append(const moe_paged_cache* c, int layer, const int32_t* seqs, i
       Hq % c->Hkv != 0 || rope_dim < 0 || rope_dim > c->D || rope_dim % 2 != 0)
     return (int)cudaErrorInvalidValue;
   if (B == 0) return (int)cudaSuccess;
-  if (!seqs || !qkv || !q_out || !paged_al16(qkv) || !paged_al16(q_out) || (q_norm == nullptr) != (k_norm == nullptr) ||
+  if (!seqs || !qkv || !q_out || !paged_al16(qkv) || !paged_al16(q_out) || !paged_al16(q_norm) || !paged_al16(k_norm) || (q_norm == nullptr) != (k_norm == nullptr) ||
       (rope_dim > 0) != (inv_freq != nullptr))
     return (int)cudaErrorInvalidValue;
   const int64_t off = layer * paged_layer_bytes(c);
