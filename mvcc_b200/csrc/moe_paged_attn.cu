@@ -4,7 +4,7 @@
 // o = sum_j softmax_j(scale q . k_j) v_j for the G = Hq / Hkv query heads and Tq new tokens that share a kv head: each
 // cached value is read once and used by G Tq rows, so up to 64 rows the call is bound by the cache's bytes.
 //
-// Work split: a unit is NG x KT keys of one (sequence, kv head, row block) job. Every CTA of a persistent grid counts
+// Work split: a unit is NG x KT keys of one (sequence, kv head, row block) job, and a job costs a few units more. Every CTA of a persistent grid counts
 // the batch's units itself (a scan over the lengths, which only the device knows) and takes an equal, contiguous share
 // of the flattened list, whatever the lengths: a long cache is split over many CTAs, many short ones share a CTA. A CTA
 // has partial results for its first and its last job at most; they go to the workspace as (max, sum, accumulator) and
@@ -36,8 +36,8 @@ namespace moe {
 namespace {
 
 constexpr int kWarps = 4;                      // consumer warps
-constexpr int kSmemOne = 227 * 1024;           // shared memory of a CTA alone on its SM
-constexpr int kSmemTwo = 113 * 1024;           // of one of two
+constexpr int kSmemOne = 226 * 1024;           // dynamic shared memory of a CTA alone on its SM
+constexpr int kSmemTwo = 112 * 1024;           // of one of two
 
 struct PAttnArgs {
   const uint16_t* q;
@@ -51,7 +51,7 @@ struct PAttnArgs {
   float* ml;       // [2 ctas][rows][2]
   float* acc;      // [2 ctas][rows][D]
   uint32_t* err;
-  int32_t B, Tq, Hq, Hkv, G, page, num_pages, max_seqs, max_pages, box_rows, row_blocks, rows, ctas;
+  int32_t B, Tq, Hq, Hkv, G, page, num_pages, max_seqs, max_pages, box_rows, row_blocks, rows, ctas, ns;
   float scale;
 };
 
@@ -60,24 +60,27 @@ struct Cfg {
   static constexpr int kEs = F8 ? 1 : 2;
   static constexpr int kRow = D * kEs;                    // bytes of a cached row
   static constexpr int kSegs = kRow / 128;                // 128-byte column segments of a tile
-  static constexpr int KT = D == 256 ? 16 : 32;           // keys of a tile
+  static constexpr int KT = kRow <= 128 ? 32 : 16;        // keys of a tile
   static constexpr int kSeg = KT * 128;                   // bytes of a segment
   static constexpr int kTile = KT * kRow;                 // bytes of a k or v tile
-  static constexpr int kSlot = 2 * kTile;
+  static constexpr int kSlot = 2 * kTile;                 // 8 KB, or 16 KB for rows of 512 bytes
   static constexpr int kPerSm = D == 256 ? 1 : 2;         // CTAs an SM: registers (accumulator D / 2 a lane)
   static constexpr int NP = 4 / kPerSm;                   // producer warps
   static constexpr int kThreads = (kWarps + NP) * 32;
-  static constexpr int kMergeRow = 64 + 4;                // floats of a row in the merge buffer: 64 columns, padded
-  static constexpr int kMerge = kWarps * 16 * (kMergeRow + 2) * 4;  // every warp's 64 columns, maxima and sums
-  static constexpr int kSlots = (kPagedMaxBatch + 1) * 4 * 3;       // first unit, keys and sequence of every slot
-  static constexpr int kFixed = 1024 + ((kMerge + kSlots + 127) & ~127) + 1024;
-  static constexpr int kFit = ((kPerSm == 1 ? kSmemOne : kSmemTwo) - kFixed) / kSlot;
-  // Ring slots: a multiple of the producers and of the key groups, so that a slot is always filled by one producer and
-  // read by one group. Barrier waits tell phases apart by parity alone: two producers on one slot could be two turns
-  // apart, and the one ahead would take a slot for free that is still to be filled.
-  static constexpr int NS = (kFit > 24 ? 24 : kFit) / kWarps * kWarps;
-  static constexpr int kSmem = kFixed + NS * kSlot;
-  static_assert(NS >= kWarps && NS % NP == 0, "ring");
+  static constexpr int kMergeCols = 32;                   // columns that meet at a time at a job's end
+  static constexpr int kMergeRow = kMergeCols + 4;        // floats of a row in the merge buffer, padded
+  static constexpr int kMerge = kWarps * 16 * (kMergeRow + 2) * 4;  // every warp's columns, maxima and sums
+  static constexpr int kMaxNS = 24;
+  // Ring slots for a batch of B: what shared memory leaves beside the merge buffer and three ints a slot of the batch.
+  // At least three a key group keep two tiles on their way while one is worked on (two: 15 % less of the bandwidth).
+  // A multiple of the producers and of the key groups, so that a ring slot is always filled by one producer and read by
+  // one group: barrier waits tell phases apart by parity alone, and two producers on one slot could be two turns apart.
+  static int fixed_bytes(int B) { return 2048 + kMerge + (3 * B + 1) * 4; }
+  static int slots(int B) {
+    const int fit = ((kPerSm == 1 ? kSmemOne : kSmemTwo) - fixed_bytes(B)) / kSlot;
+    return (fit > kMaxNS ? kMaxNS : fit) / kWarps * kWarps;
+  }
+  static_assert(kWarps % NP == 0, "a ring slot has one producer");
 };
 
 // D (16x8, fp32) += A (16x16) B (16x8); bf16 or f16 operands.
@@ -124,10 +127,6 @@ __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
 }
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __shfl_xor_sync(0xffffffffu, v, 1);
-  return v + __shfl_xor_sync(0xffffffffu, v, 2);
-}
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* mbar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
@@ -165,14 +164,31 @@ __device__ __forceinline__ int slot_keys(const PAttnArgs& a, int b, int* seq) {
   return n;
 }
 
-// The share of one CTA: units [u0, u1) of the flattened list, walked job by job.
 // joins[c]: parts, first CTA, whether its part is that CTA's second, slot, kv head, row block
 enum { JOIN_PARTS = 0, JOIN_FIRST, JOIN_SECOND, JOIN_SLOT, JOIN_HEAD, JOIN_BLOCK, JOIN_INTS = 8 };
 
+// The share of one CTA: [u, end) of the flattened list, walked job by job. A job counts kSetup units of its own before
+// its units of keys: its queries, its first tile's latency and its merge cost a CTA about as much, and a batch with
+// many short sequences would otherwise pile them up in a few CTAs.
+constexpr int kSetup = 5;
 struct Walk {
-  int u, end, b, base, U;  // the next unit, the share's end; the slot it falls into, its first unit, its units a job
+  int u, end;           // what is left of the share
+  int b, job, W;        // the slot, its job (kv head and row block), units of each of its jobs
+  int base;             // first unit of the slot
+  int lu, run;          // units of keys of the job that are this CTA's: [lu, lu + run)
+  // The next job of the share that has keys here; false at the end.
+  __device__ __forceinline__ bool next(const int* S, int B, int HR) {
+    while (u < end) {
+      seek(S, B, HR);
+      const int at = u - base - job * W, n = min(end - u, W - at);
+      lu = max(0, at - kSetup);
+      run = max(0, at + n - kSetup) - lu;
+      u += n;
+      if (run > 0) return true;
+    }
+    return false;
+  }
   __device__ __forceinline__ void seek(const int* S, int B, int HR) {
-    if (u >= end) return;
     int lo = 0, hi = B - 1;  // the last slot whose first unit is not behind u; empty slots before it are passed
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -181,7 +197,8 @@ struct Walk {
     }
     b = lo;
     base = S[b] * HR;
-    U = S[b + 1] - S[b];
+    W = S[b + 1] - S[b];
+    job = (u - base) / W;
   }
 };
 
@@ -190,11 +207,12 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
     paged_attn_kernel(const __grid_constant__ PAttnArgs a, const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v) {
   using C = Cfg<D, F8>;
-  constexpr int NG = kWarps / MT, KT = C::KT, UK = NG * KT, NS = C::NS, NP = C::NP, kThreads = C::kThreads;
+  constexpr int NG = kWarps / MT, KT = C::KT, UK = NG * KT, NP = C::NP, kThreads = C::kThreads;
+  const int NS = a.ns;
   constexpr int NT = D / 8;     // accumulator tiles of 8 columns
   constexpr int KC = C::kRow / 16;  // 16-byte chunks of a cached row
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t full[NS], empty[NS];
+  __shared__ __align__(8) uint64_t full[C::kMaxNS], empty[C::kMaxNS];
   __shared__ int sm[32];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   float* merge = reinterpret_cast<float*>(ring + (size_t)NS * C::kSlot);
@@ -220,7 +238,7 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
       const int n = slot_keys(a, b, &seqs[b]);
       keys[b] = n;
       S[b] = sum;
-      sum += (n + UK - 1) / UK;
+      sum += n > 0 ? (n + UK - 1) / UK + kSetup : 0;
     }
     int total;
     const int before = block_excl_scan(sum, sm, &total);
@@ -243,15 +261,15 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
     int parts = 0;
     if (w.u < w.end) {
       w.seek(S, a.B, HR);
-      const int job = (w.u - w.base) / w.U, u0 = w.base + job * w.U;
+      const int u0 = w.base + w.job * w.W + kSetup;  // the job's first unit of keys
       if (u0 < w.u) {
         const int c0 = u0 / per;
-        parts = (u0 + w.U - 1) / per - c0 + 1;
+        parts = (u0 - kSetup + w.W - 1) / per - c0 + 1;
         jn[JOIN_FIRST] = c0;
-        jn[JOIN_SECOND] = u0 != c0 * per;
+        jn[JOIN_SECOND] = u0 - kSetup > c0 * per;  // another job's units lie before it in that CTA
         jn[JOIN_SLOT] = w.b;
-        jn[JOIN_HEAD] = job / a.row_blocks;
-        jn[JOIN_BLOCK] = job % a.row_blocks;
+        jn[JOIN_HEAD] = w.job / a.row_blocks;
+        jn[JOIN_BLOCK] = w.job % a.row_blocks;
       }
     }
     jn[JOIN_PARTS] = parts;
@@ -261,21 +279,26 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
     // ---------------------------------------------------------------- producer
     const int none = a.num_pages * a.Hkv;  // a page that is not there: outside the map, reads as zero
     const int nbox = KT / a.box_rows;
-    int i = 0;      // tiles so far
+    int i = 0;      // tiles so far: slot i % NS, for the turn-th time
+    int slot = 0, turn = 0;
+    auto on = [&] {
+      ++i;
+      if (++slot == NS) {
+        slot = 0;
+        ++turn;
+      }
+    };
     bool ok = true;
-    while (w.u < w.end && ok) {
-      w.seek(S, a.B, HR);
-      const int rel = w.u - w.base, job = rel / w.U, lu = rel - job * w.U, run = min(w.end - w.u, w.U - lu);
-      const int h = job / a.row_blocks;
+    while (ok && w.next(S, a.B, HR)) {
+      const int lu = w.lu, run = w.run, h = w.job / a.row_blocks;
       const int n = keys[w.b];
       const int32_t* row = a.tables + (int64_t)seqs[w.b] * a.max_pages;
       const int key_end = (lu + run) * UK;
       int z = 0, y = 0;
       int fetched = lu * UK;  // first key whose box no lane holds yet
       int held = 0;           // first key of lane 0's box
-      for (int key = lu * UK; key < key_end && ok; key += KT, ++i) {
+      for (int key = lu * UK; key < key_end && ok; key += KT, on()) {
         if (i % NP != warp - kWarps) continue;
-        const int slot = i % NS, turn = i / NS;
         if (turn > 0) {
           ok = bar_wait(&empty[slot], (turn - 1) & 1);
           if (!ok) {
@@ -319,7 +342,6 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
         }
         __syncwarp();
       }
-      w.u += run;
     }
     if (!ok)  // no copy may still be landing when the CTA exits
       for (int j = max(0, i - NS); j < i; ++j)
@@ -334,18 +356,20 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
   // v, transposed, (0-7, c), (8-15, c), (0-7, c+1), (8-15, c+1)
   const int kk_row = (lane >> 4) * 8 + (lane & 7), kk_ch = (lane >> 3) & 1;
   const int vv_row = ((lane >> 3) & 1) * 8 + (lane & 7), vv_ch = lane >> 4;
-  auto chunk_addr = [&](uint32_t tile, int r, int ch) {
-    return tile + (ch >> 3) * C::kSeg + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+  // Offset of chunk pair 0 in a tile, swizzled; pair i of the four in a 128-byte segment is the same with bits 5-6
+  // flipped by i, row group j (16 keys) 2048 bytes further on
+  const uint32_t k_lane = kk_row * 128 + ((kk_ch ^ (kk_row & 7)) << 4);
+  const uint32_t v_lane = vv_row * 128 + ((vv_ch ^ (vv_row & 7)) << 4);
+  auto chunk_addr = [&](const uint32_t (&base)[4], int j, int c) {
+    return base[(c >> 1) & 3] + (c >> 3) * C::kSeg + j * 2048;
   };
-  int i0 = 0;   // tiles before this job
+  int slot = g, turn = 0;  // of this group's next tile
   int njob = 0;
   bool ok = true;
-  while (w.u < w.end) {
-    w.seek(S, a.B, HR);
-    const int rel = w.u - w.base, job = rel / w.U, lu = rel - job * w.U, run = min(w.end - w.u, w.U - lu);
-    const int h = job / a.row_blocks, rb = job - h * a.row_blocks;
+  while (w.next(S, a.B, HR)) {
+    const int lu = w.lu, run = w.run, h = w.job / a.row_blocks, rb = w.job - h * a.row_blocks;
     const int n = keys[w.b];
-    const bool whole = lu == 0 && run == w.U;
+    const bool whole = run == w.W - kSetup;
     // this lane's two rows: query row r of the kv head is token r / G, head h G + r % G
     const int rA = rb * a.rows + mt * 16 + qr, rB = rA + 8, M = a.G * a.Tq;
     const int tA = rA / a.G, tB = rB / a.G;
@@ -354,9 +378,12 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
       return a.q + (((int64_t)w.b * a.Tq + t) * a.Hq + h * a.G + (r - t * a.G)) * D;
     };
     uint32_t qf[D / 16][4];
-    float fA = a.scale * 1.4426950408889634f, fB;  // S in units of log 2
+    // scores in units of log 2 are S times fA or fB, kept above zero: a negative scale turns the queries' signs, and one
+    // of zero is as good as the smallest factor
+    float fA = a.scale * 1.4426950408889634f, fB;
     if (a.k_scale) fA *= a.k_scale[h];
-    fB = fA;
+    const uint32_t flip = fA < 0.f ? 0x80008000u : 0u;
+    fA = fB = fmaxf(fabsf(fA), 1.1754944e-38f);
     {
       const uint16_t* pA = q_row(rA < M ? rA : 0, rA < M ? tA : 0);
       const uint16_t* pB = q_row(rB < M ? rB : 0, rB < M ? tB : 0);
@@ -367,6 +394,8 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
           qf[c][1] = *reinterpret_cast<const uint32_t*>(pB + c * 16 + 2 * ql);
           qf[c][2] = *reinterpret_cast<const uint32_t*>(pA + c * 16 + 8 + 2 * ql);
           qf[c][3] = *reinterpret_cast<const uint32_t*>(pB + c * 16 + 8 + 2 * ql);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) qf[c][e] ^= flip;
         }
       } else {
         // e4m3 keys become f16, so the queries do too: scaled by the power of two that brings the row's largest into
@@ -377,7 +406,7 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
         for (int c = 0; c < D / 16; ++c) {
           const uint2 xa = *reinterpret_cast<const uint2*>(pA + c * 16 + 4 * ql);
           const uint2 xb = *reinterpret_cast<const uint2*>(pB + c * 16 + 4 * ql);
-          qf[c][0] = xa.x; qf[c][2] = xa.y; qf[c][1] = xb.x; qf[c][3] = xb.y;
+          qf[c][0] = xa.x ^ flip; qf[c][2] = xa.y ^ flip; qf[c][1] = xb.x ^ flip; qf[c][3] = xb.y ^ flip;
           mA = fmaxf(fmaxf(mA, fmaxf(fabsf(lo_bf(xa.x)), fabsf(hi_bf(xa.x)))), fmaxf(fabsf(lo_bf(xa.y)), fabsf(hi_bf(xa.y))));
           mB = fmaxf(fmaxf(mB, fmaxf(fabsf(lo_bf(xb.x)), fabsf(hi_bf(xb.x)))), fmaxf(fabsf(lo_bf(xb.y)), fabsf(hi_bf(xb.y))));
         }
@@ -399,47 +428,59 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
     float acc[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-    float mA = -INFINITY, mB = -INFINITY, lA = 0.f, lB = 0.f;
+    float lsum[4] = {0.f, 0.f, 0.f, 0.f};  // the weights' sums, as one more accumulator tile: P times a column of ones
+    constexpr uint32_t kOnes = F8 ? 0x3c003c00u : 0x3f803f80u;
+    float mA = -INFINITY, mB = -INFINITY;  // the maxima of S
 
     for (int r = 0; r < run; ++r) {
-      const int i = i0 + r * NG + g, slot = i % NS;
       const int key0 = (lu + r) * UK + g * KT;
-      if (ok && !bar_wait(&full[slot], (i / NS) & 1)) {
+      if (ok && !bar_wait(&full[slot], turn & 1)) {
         ok = false;
         if (lane == 0) atomicOr(a.err, (uint32_t)MOE_ERR_TIMEOUT);
       }
       if (ok && key0 < n) {
         const uint32_t kt = ring32 + slot * C::kSlot, vt = kt + C::kTile;
-        // S = Q K^T, two chains of accumulators per 8 keys
-        float s[KT / 8][4], s2[KT / 8][4];
+        const uint32_t k0 = kt + k_lane, v0 = vt + v_lane;
+        const uint32_t kb[4] = {k0, k0 ^ 32, k0 ^ 64, k0 ^ 96}, vb[4] = {v0, v0 ^ 32, v0 ^ 64, v0 ^ 96};
+        // S = Q K^T. Two chains of accumulators per 8 keys where a tile's 16 keys alone give too few to hide an MMA's
+        // latency (21 cycles against 8 of issue)
+        constexpr int kChains = KT == 16 ? 2 : 1;
+        float s[KT / 8][4], s2[kChains == 2 ? KT / 8 : 1][4];
 #pragma unroll
         for (int j = 0; j < KT / 8; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[j][e] = s2[j][e] = 0.f;
+          for (int e = 0; e < 4; ++e) {
+            s[j][e] = 0.f;
+            if constexpr (kChains == 2) s2[j][e] = 0.f;
+          }
+        auto other = [&](int j) -> float(&)[4] {
+          if constexpr (kChains == 2) return s2[j];
+          else return s[j];
+        };
 #pragma unroll
         for (int c = 0; c < KC; c += 2) {
 #pragma unroll
           for (int j = 0; j < KT / 16; ++j) {
             uint32_t kf[4];
-            ldsm4(kf, chunk_addr(kt, j * 16 + kk_row, c + kk_ch));
+            ldsm4(kf, chunk_addr(kb, j, c));
             if constexpr (!F8) {
-              auto& d0 = (c / 2) & 1 ? s2[2 * j] : s[2 * j];
-              auto& d1 = (c / 2) & 1 ? s2[2 * j + 1] : s[2 * j + 1];
-              mma16816<false>(d0, qf[c / 2], kf[0], kf[1]);
-              mma16816<false>(d1, qf[c / 2], kf[2], kf[3]);
+              mma16816<false>((c / 2) & 1 ? other(2 * j) : s[2 * j], qf[c / 2], kf[0], kf[1]);
+              mma16816<false>((c / 2) & 1 ? other(2 * j + 1) : s[2 * j + 1], qf[c / 2], kf[2], kf[3]);
             } else {
               mma16816<true>(s[2 * j], qf[c], e4m3x2_f16x2(kf[0]), e4m3x2_f16x2(kf[0] >> 16));
-              mma16816<true>(s2[2 * j], qf[c + 1], e4m3x2_f16x2(kf[1]), e4m3x2_f16x2(kf[1] >> 16));
               mma16816<true>(s[2 * j + 1], qf[c], e4m3x2_f16x2(kf[2]), e4m3x2_f16x2(kf[2] >> 16));
-              mma16816<true>(s2[2 * j + 1], qf[c + 1], e4m3x2_f16x2(kf[3]), e4m3x2_f16x2(kf[3] >> 16));
+              mma16816<true>(other(2 * j), qf[c + 1], e4m3x2_f16x2(kf[1]), e4m3x2_f16x2(kf[1] >> 16));
+              mma16816<true>(other(2 * j + 1), qf[c + 1], e4m3x2_f16x2(kf[3]), e4m3x2_f16x2(kf[3] >> 16));
             }
           }
         }
         const bool masked = key0 + KT > n - a.Tq + 1;  // some row does not see all of the tile
+        if constexpr (kChains == 2) {
 #pragma unroll
-        for (int j = 0; j < KT / 8; ++j)
+          for (int j = 0; j < KT / 8; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[j][e] = (s[j][e] + s2[j][e]) * (e < 2 ? fA : fB);
+            for (int e = 0; e < 4; ++e) s[j][e] += s2[j][e];
+        }
         if (masked) {
 #pragma unroll
           for (int j = 0; j < KT / 8; ++j)
@@ -447,7 +488,7 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
             for (int e = 0; e < 4; ++e)
               if (key0 + j * 8 + 2 * ql + (e & 1) >= (e < 2 ? limA : limB)) s[j][e] = -INFINITY;
         }
-        // running maximum and sum
+        // running maximum
         float nA = mA, nB = mB;
 #pragma unroll
         for (int j = 0; j < KT / 8; ++j) {
@@ -456,11 +497,14 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
         }
         nA = quad_max(nA);
         nB = quad_max(nB);
-        const float zA = nA == -INFINITY ? 0.f : nA, zB = nB == -INFINITY ? 0.f : nB;
+        // f16 weights carry a common factor 2^15 (it cancels in the division): what a long row's many small weights
+        // lose below f16's normal range then stays under 2^-40 of the largest each.
+        constexpr float kLift = F8 ? 15.f : 0.f;
+        const float zA = nA == -INFINITY ? 0.f : nA * fA, zB = nB == -INFINITY ? 0.f : nB * fB;
         if (__any_sync(0xffffffffu, nA != mA || nB != mB)) {
-          const float cA = ex2(mA - zA), cB = ex2(mB - zB);
-          lA *= cA;
-          lB *= cB;
+          const float cA = ex2(fmaf(mA, fA, -zA)), cB = ex2(fmaf(mB, fB, -zB));
+          lsum[0] *= cA;
+          lsum[2] *= cB;
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
             acc[j][0] *= cA;
@@ -471,28 +515,16 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
           mA = nA;
           mB = nB;
         }
-        // P in the cache's MMA type. The sums take the rounded weights, so that a row's weights still add up to one.
-        // f16 weights carry a common factor 2^15 (it cancels in the division): what a long row's many small weights
-        // lose below f16's normal range then stays under 2^-40 of the largest each.
-        constexpr float kLift = F8 ? 15.f : 0.f;
+        // P in the cache's MMA type; the sums take the rounded weights, so that a row's weights still add up to one
         uint32_t pf[KT / 16][4];
+        const float yA = kLift - zA, yB = kLift - zB;
 #pragma unroll
         for (int j = 0; j < KT / 8; ++j) {
-          const float p0 = ex2(s[j][0] - zA + kLift), p1 = ex2(s[j][1] - zA + kLift);
-          const float p2 = ex2(s[j][2] - zB + kLift), p3 = ex2(s[j][3] - zB + kLift);
-          const uint32_t xA = pack2<F8>(p0, p1), xB = pack2<F8>(p2, p3);
-          pf[j >> 1][(j & 1) * 2] = xA;
-          pf[j >> 1][(j & 1) * 2 + 1] = xB;
-          if constexpr (F8) {
-            const float2 ra = __half22float2(*reinterpret_cast<const __half2*>(&xA));
-            const float2 rb2 = __half22float2(*reinterpret_cast<const __half2*>(&xB));
-            lA += ra.x + ra.y;
-            lB += rb2.x + rb2.y;
-          } else {
-            lA += lo_bf(xA) + hi_bf(xA);
-            lB += lo_bf(xB) + hi_bf(xB);
-          }
+          pf[j >> 1][(j & 1) * 2] = pack2<F8>(ex2(fmaf(s[j][0], fA, yA)), ex2(fmaf(s[j][1], fA, yA)));
+          pf[j >> 1][(j & 1) * 2 + 1] = pack2<F8>(ex2(fmaf(s[j][2], fB, yB)), ex2(fmaf(s[j][3], fB, yB)));
         }
+#pragma unroll
+        for (int ks = 0; ks < KT / 16; ++ks) mma16816<F8>(lsum, pf[ks], kOnes, kOnes);
         // O += P V. B fragments of the 16 keys from key0 + 16 ks, the columns of chunk pair c
         auto pv = [&](auto&& keep, auto&& add) {
 #pragma unroll
@@ -500,7 +532,7 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
 #pragma unroll
             for (int c = 0; c < KC; c += 2) {
               uint32_t vf[4];
-              ldsm4t(vf, chunk_addr(vt, ks * 16 + vv_row, c + vv_ch));
+              ldsm4t(vf, chunk_addr(vb, ks, c));
 #pragma unroll
               for (int e = 0; e < 4; ++e) vf[e] &= keep(ks, e & 1);
               if constexpr (!F8) {
@@ -566,24 +598,29 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[slot]);
+      if ((slot += NG) >= NS) {
+        slot = g;
+        ++turn;
+      }
     }
-    i0 += run * NG;
-    lA = quad_sum(lA);
-    lB = quad_sum(lB);
+    const float lA = lsum[0], lB = lsum[2];
+    // maxima in units of log 2 from here on
+    mA = mA == -INFINITY ? mA : mA * fA;
+    mB = mB == -INFINITY ? mB : mB * fB;
 
-    // The job's end: the NG warps of a row tile meet in shared memory, 64 columns at a time; a thread then holds eight
+    // The job's end: the NG warps of a row tile meet in shared memory, 32 columns at a time; a thread then holds four
     // columns of one row, scales the warps' sums to their common maximum and stores them.
     if (ql == 0) {
       merge_ml[warp * 16 + qr] = make_float2(mA, lA);
       merge_ml[warp * 16 + qr + 8] = make_float2(mB, lB);
     }
-    const int orow = (tid >> 3) & 15, ocol = (tid & 7) * 8;  // MT row tiles of 16 rows x 64 columns, 128 threads a turn
+    const int orow = (tid >> 3) & 15, ocol = (tid & 7) * 4;  // 16 rows x 32 columns, 128 threads a turn
     const float vs = a.v_scale ? a.v_scale[h] : 1.f;
 #pragma unroll
-    for (int c0 = 0; c0 < D; c0 += 64) {
+    for (int c0 = 0; c0 < D; c0 += C::kMergeCols) {
       float* mine = merge + warp * 16 * C::kMergeRow;
 #pragma unroll
-      for (int j = c0 / 8; j < c0 / 8 + 8; j += F8 ? 2 : 1) {
+      for (int j = c0 / 8; j < (c0 + C::kMergeCols) / 8; j += F8 ? 2 : 1) {
         // columns of accumulator tile j: bf16 8 j + 2 ql, + 1; e4m3 (tiles j, j + 1) 8 j + 4 ql + {0, 2}, + {1, 3}
         if constexpr (!F8) {
           *reinterpret_cast<float2*>(mine + qr * C::kMergeRow + 8 * j - c0 + 2 * ql) = make_float2(acc[j][0], acc[j][1]);
@@ -605,45 +642,40 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
 #pragma unroll
           for (int k = 0; k < NG; ++k) m = fmaxf(m, merge_ml[(k * MT + x) * 16 + orow].x);
           const float z = m == -INFINITY ? 0.f : m;
-          float l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          float l = 0.f;
+          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int k = 0; k < NG; ++k) {
             const float2 ml = merge_ml[(k * MT + x) * 16 + orow];
             const float f = ex2(ml.x - z);
             l = fmaf(ml.y, f, l);
-            const float* from = merge + ((k * MT + x) * 16 + orow) * C::kMergeRow + ocol;
-            const float4 p0 = *reinterpret_cast<const float4*>(from), p1 = *reinterpret_cast<const float4*>(from + 4);
-            o[0] = fmaf(p0.x, f, o[0]);
-            o[1] = fmaf(p0.y, f, o[1]);
-            o[2] = fmaf(p0.z, f, o[2]);
-            o[3] = fmaf(p0.w, f, o[3]);
-            o[4] = fmaf(p1.x, f, o[4]);
-            o[5] = fmaf(p1.y, f, o[5]);
-            o[6] = fmaf(p1.z, f, o[6]);
-            o[7] = fmaf(p1.w, f, o[7]);
+            const float4 p = *reinterpret_cast<const float4*>(merge + ((k * MT + x) * 16 + orow) * C::kMergeRow + ocol);
+            o.x = fmaf(p.x, f, o.x);
+            o.y = fmaf(p.y, f, o.y);
+            o.z = fmaf(p.z, f, o.z);
+            o.w = fmaf(p.w, f, o.w);
           }
           if (whole) {
             const float d = l == 0.f ? 0.f : vs / l;  // an empty row is zero; a NaN sum stays
             const int t = row / a.G;
             uint16_t* dst = a.out + (((int64_t)w.b * a.Tq + t) * a.Hq + h * a.G + (row - t * a.G)) * D + c0 + ocol;
-            *reinterpret_cast<uint4*>(dst) = make_uint4(pack2<false>(o[0] * d, o[1] * d), pack2<false>(o[2] * d, o[3] * d),
-                                                        pack2<false>(o[4] * d, o[5] * d), pack2<false>(o[6] * d, o[7] * d));
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<false>(o.x * d, o.y * d), pack2<false>(o.z * d, o.w * d));
           } else {
             const int64_t at = ((int64_t)blockIdx.x * 2 + (njob > 0)) * a.rows + lr;
             if (c0 == 0 && ocol == 0) *reinterpret_cast<float2*>(a.ml + at * 2) = make_float2(m, l);
-            float4* dst = reinterpret_cast<float4*>(a.acc + at * D + c0 + ocol);
-            dst[0] = make_float4(o[0], o[1], o[2], o[3]);
-            dst[1] = make_float4(o[4], o[5], o[6], o[7]);
+            *reinterpret_cast<float4*>(a.acc + at * D + c0 + ocol) = o;
           }
         }
       }
       consumers_sync();
     }
     ++njob;
-    w.u += run;
   }
-  if (!ok)  // no copy may still be landing when the CTA exits: this warp's last tiles once more
-    for (int i = i0 - NG + g; i >= 0 && i > i0 - NS; i -= NG) bar_wait(&full[i % NS], (i / NS) & 1);
+  if (!ok)  // no copy may still be landing when the CTA exits: this group's last tiles once more
+    for (int k = g; k < NS; k += NG) {
+      const int t = k < slot ? turn : turn - 1;  // the slot's last turn
+      if (t >= 0) bar_wait(&full[k], t & 1);
+    }
 }
 
 // The join. Border c (before CTA c) inside a job of CTAs c0 .. c1 takes the (c - c0 - 1)-th of c1 - c0 equal shares of
@@ -799,13 +831,15 @@ cudaError_t launch_attn(const PAttnArgs& args, const CUtensorMap& mk, const CUte
   using C = Cfg<D, F8>;
   const void* fn = reinterpret_cast<const void*>(paged_attn_kernel<D, F8, MT>);
   static SmemGrant granted;
-  cudaError_t e = grant_smem(fn, C::kSmem, 0, granted);
-  if (e != cudaSuccess) return e;
   PAttnArgs a = args;
+  a.ns = C::slots(a.B);
+  const int smem = C::fixed_bytes(a.B) + a.ns * C::kSlot;
+  cudaError_t e = grant_smem(fn, smem, C::kPerSm == 1 ? kSmemOne : kSmemTwo, granted);
+  if (e != cudaSuccess) return e;
   a.ctas = std::min(kPagedMaxCtas, paged_sms() * C::kPerSm);
   CUtensorMap k = mk, v = mv;
   void* p[] = {&a, &k, &v};
-  e = paged_launch(fn, dim3(a.ctas), dim3(C::kThreads), C::kSmem, s, p);
+  e = paged_launch(fn, dim3(a.ctas), dim3(C::kThreads), smem, s, p);
   if (e != cudaSuccess) return e;
   void* j[] = {&a};
   return paged_launch(reinterpret_cast<const void*>(paged_join_kernel<D>), dim3(a.ctas - 1),
@@ -819,7 +853,7 @@ cudaError_t launch_rows(const PAttnArgs& a, const CUtensorMap& mk, const CUtenso
   return launch_attn<D, F8, 4>(a, mk, mv, s);
 }
 
-int tile_keys(int D) { return D == 256 ? 16 : 32; }
+int tile_keys(int row_bytes) { return row_bytes <= 128 ? 32 : 16; }
 
 }  // namespace
 }  // namespace moe
@@ -864,9 +898,9 @@ int moe_paged_attend(const moe_paged_cache* c, int layer, const int32_t* seqs, i
   a.scale = scale;
   a.ctas = 0;
   // the flattened unit list is counted in 32 bits; a unit is at least 16 keys
-  const int64_t units = ((int64_t)c->max_pages * c->page + 15) / 16;
+  const int64_t units = ((int64_t)c->max_pages * c->page + 15) / 16 + kSetup;
   if (B * units * c->Hkv * a.row_blocks >= ((int64_t)1 << 31) - kPagedMaxCtas) return (int)cudaErrorInvalidValue;
-  const int kt = tile_keys(c->D);
+  const int kt = tile_keys(c->D * kv_size(c->kv_type));
   a.box_rows = c->page % kt == 0 ? kt : 16;
   CUtensorMap mk, mv;
   const int64_t off = layer * paged_layer_bytes(c);
