@@ -7,10 +7,11 @@
 // Work split: a unit is NG x KT keys of one (sequence, kv head, row block) job, and a job costs a few units more. Every CTA of a persistent grid counts
 // the batch's units itself (a scan over the lengths, which only the device knows) and takes an equal, contiguous share
 // of the flattened list, whatever the lengths: a long cache is split over many CTAs, many short ones share a CTA. A CTA
-// has partial results for its first and its last job at most; they go to the workspace as (max, sum, accumulator) and
-// paged_join_kernel merges each split job's parts in CTA order, so the result does not depend on timing. A job that
-// lies in one CTA is finished there. A job of n parts holds n - 1 of the borders between CTAs, so the join runs a CTA
-// a border, and those of one job share its rows.
+// has partial results for its first and its last job at most; they go to the workspace as (max, sum, accumulator), and
+// behind a barrier over the grid each split job's parts are merged in CTA order, so the result does not depend on timing.
+// A job that lies in one CTA is finished there. A job of n parts holds n - 1 of the borders between CTAs: the CTA behind
+// each border takes an equal share of the job's rows. (The merge as a kernel of its own cost 3 us of host time and as
+// much between the kernels.)
 //
 // CTA: four consumer warps and NP producer warps, four producers an SM (a thread issues a TMA copy every 95 cycles or
 // so: one alone fetches 3.2 TB/s over the GPU in 2 KB boxes, four 6.4 TB/s). Producer w takes every NP-th of the
@@ -47,13 +48,17 @@ struct PAttnArgs {
   const int32_t* seqs;
   const int32_t* tables;
   const int32_t* lens;
-  int32_t* joins;  // [ctas][8]: the split job at the border before each CTA (parts = 0: none)
+  unsigned long long* gbar;  // arrivals at the end of the work, over all launches
   float* ml;       // [2 ctas][rows][2]
   float* acc;      // [2 ctas][rows][D]
   uint32_t* err;
   int32_t B, Tq, Hq, Hkv, G, page, num_pages, max_seqs, max_pages, box_rows, row_blocks, rows, ctas, ns;
-  float scale;
+  float scale, inv_G;
 };
+
+// The token of row r of a kv head, r / G for r < 2^12 and G <= 128: half a row off, the product stays clear of the next
+// whole number by 0.5 / G, far more than its rounding.
+__device__ __forceinline__ int token_of(const PAttnArgs& a, int r) { return __float2int_rd(((float)r + 0.5f) * a.inv_G); }
 
 template <int D, bool F8>
 struct Cfg {
@@ -67,9 +72,9 @@ struct Cfg {
   static constexpr int kPerSm = D == 256 ? 1 : 2;         // CTAs an SM: registers (accumulator D / 2 a lane)
   static constexpr int NP = 4 / kPerSm;                   // producer warps
   static constexpr int kThreads = (kWarps + NP) * 32;
-  static constexpr int kMergeCols = 32;                   // columns that meet at a time at a job's end
+  static constexpr int kMergeCols = D == 256 ? 64 : 32;   // columns that meet at a time at a job's end
   static constexpr int kMergeRow = kMergeCols + 4;        // floats of a row in the merge buffer, padded
-  static constexpr int kMerge = kWarps * 16 * (kMergeRow + 2) * 4;  // every warp's columns, maxima and sums
+  static constexpr int kMerge = kWarps * 16 * (kMergeRow + 2) * 4;  // every warp's columns; maxima and sums
   static constexpr int kMaxNS = 24;
   // Ring slots for a batch of B: what shared memory leaves beside the merge buffer and three ints a slot of the batch.
   // At least three a key group keep two tiles on their way while one is worked on (two: 15 % less of the bandwidth).
@@ -164,8 +169,9 @@ __device__ __forceinline__ int slot_keys(const PAttnArgs& a, int b, int* seq) {
   return n;
 }
 
-// joins[c]: parts, first CTA, whether its part is that CTA's second, slot, kv head, row block
-enum { JOIN_PARTS = 0, JOIN_FIRST, JOIN_SECOND, JOIN_SLOT, JOIN_HEAD, JOIN_BLOCK, JOIN_INTS = 8 };
+// The split job at the border before a CTA: its parts (0: none), its first CTA, whether its part is that CTA's second,
+// slot, kv head and row block.
+enum { JOIN_PARTS = 0, JOIN_FIRST, JOIN_SECOND, JOIN_SLOT, JOIN_HEAD, JOIN_BLOCK, JOIN_INTS };
 
 // The share of one CTA: [u, end) of the flattened list, walked job by job. A job counts kSetup units of its own before
 // its units of keys: its queries, its first tile's latency and its merge cost a CTA about as much, and a batch with
@@ -202,6 +208,122 @@ struct Walk {
   }
 };
 
+// The join, by the consumer threads of CTA c, whose share begins inside a job of CTAs c0 .. c1: they take the
+// (c - c0 - 1)-th of c1 - c0 equal shares of the job's (row, four columns) items. An item's parts, one per CTA of the
+// job in order, are weighted by 2^(m_i - m) and added; a share of few items has its parts spread over the threads.
+struct JoinScratch {
+  static constexpr int kMaxRows = 64;
+  float4 red[kWarps * 32];
+  // weights of the share's rows: rows * parts <= (64 / (parts - 1) + 2) * parts
+  float wt[2 * kMaxRows + 2 * kPagedMaxCtas];
+  float inv[kMaxRows];
+};
+template <int D>
+__device__ void join_share(const PAttnArgs& a, const int (&jn)[JOIN_INTS], JoinScratch& js) {
+  constexpr int kCols = D / 4, kT = kWarps * 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x;
+  const int parts = jn[JOIN_PARTS], c0 = jn[JOIN_FIRST], second = jn[JOIN_SECOND], b = jn[JOIN_SLOT], h = jn[JOIN_HEAD],
+            rb = jn[JOIN_BLOCK];
+  const int rows = min(a.rows, a.G * a.Tq - rb * a.rows), all = rows * kCols, share = c - c0 - 1;
+  const int i0 = all * share / (parts - 1), i1 = all * (share + 1) / (parts - 1);  // all <= 2^12, parts <= 320
+  if (i0 >= i1) return;
+  const int r0 = i0 / kCols, r1 = (i1 - 1) / kCols + 1;
+  auto part = [&](int i) { return (int64_t)(c0 + i) * 2 + (i == 0 ? second : 0); };
+  // Few items (many parts): the parts of an item over `slices` threads, a power of two up to 32. Many items (few parts):
+  // kItems items a thread at a time. Either way each thread's first kAhead values are on their way while the weights are
+  // found: eight parts of one item, or two of each of four.
+  constexpr int kAhead = 8, kItems = 4;
+  int lg = 0;
+  while (lg < 5 && (i1 - i0) << (lg + 1) <= kT) ++lg;
+  const int slices = 1 << lg, lanes = kT >> lg, sl = (tid << lg) / kT, mine = i0 + (tid & (lanes - 1));
+  auto load = [&](int it, int i) {
+    const int r = it / kCols, col = it % kCols;
+    return it < i1 && i < parts ? __ldcg(reinterpret_cast<const float4*>(a.acc + (part(i) * a.rows + r) * D + col * 4))
+                                : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  auto weight = [&](int it, int i) { return it < i1 && i < parts ? js.wt[(it / kCols - r0) * parts + i] : 0.f; };
+  auto add = [](float4& s, const float4& x, float f) {
+    s.x = fmaf(x.x, f, s.x);
+    s.y = fmaf(x.y, f, s.y);
+    s.z = fmaf(x.z, f, s.z);
+    s.w = fmaf(x.w, f, s.w);
+  };
+  auto store = [&](int it, const float4& s) {
+    if (it >= i1) return;
+    const int r = it / kCols, col = it % kCols, q = rb * a.rows + r, t = token_of(a, q);
+    const float d = js.inv[r - r0];
+    *reinterpret_cast<uint2*>(a.out + (((int64_t)b * a.Tq + t) * a.Hq + h * a.G + (q - t * a.G)) * D + col * 4) =
+        make_uint2(pack2<false>(s.x * d, s.y * d), pack2<false>(s.z * d, s.w * d));
+  };
+  float4 ahead[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k)
+    ahead[k] = slices > 1 ? load(mine, sl + k * slices) : load(mine + k % kItems * kT, k / kItems);
+  for (int r = r0 + warp; r < r1; r += kWarps) {
+    constexpr int kHeld = 3;  // a lane's parts that stay in registers
+    float2 x[kHeld];
+    float m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+      const int i = lane + 32 * k;
+      x[k] = i < parts ? __ldcg(reinterpret_cast<const float2*>(a.ml + (part(i) * a.rows + r) * 2))
+                       : make_float2(-INFINITY, 0.f);
+    }
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) m = fmaxf(m, x[k].x);
+    for (int i = lane + 32 * kHeld; i < parts; i += 32) m = fmaxf(m, __ldcg(a.ml + (part(i) * a.rows + r) * 2));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float z = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+      const int i = lane + 32 * k;
+      const float f = ex2(x[k].x - z);
+      if (i < parts) js.wt[(r - r0) * parts + i] = f;
+      l = fmaf(x[k].y, f, l);
+    }
+    for (int i = lane + 32 * kHeld; i < parts; i += 32) {
+      const float2 v = __ldcg(reinterpret_cast<const float2*>(a.ml + (part(i) * a.rows + r) * 2));
+      const float f = ex2(v.x - z);
+      js.wt[(r - r0) * parts + i] = f;
+      l = fmaf(v.y, f, l);
+    }
+    l = warp_sum(l);
+    if (lane == 0) js.inv[r - r0] = l == 0.f ? 0.f : (a.v_scale ? a.v_scale[h] : 1.f) / l;
+  }
+  consumers_sync();
+  if (slices > 1) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) add(s, ahead[k], weight(mine, sl + k * slices));
+#pragma unroll 4
+    for (int i = sl + kAhead * slices; i < parts; i += slices) add(s, load(mine, i), weight(mine, i));
+    js.red[tid] = s;
+    consumers_sync();
+    if (sl != 0) return;
+    for (int k = 1; k < slices; ++k) add(s, js.red[k * lanes + tid], 1.f);
+    store(mine, s);
+  } else {
+    for (int base = mine; base < i1; base += kItems * kT) {
+      float4 s[kItems];
+#pragma unroll
+      for (int k = 0; k < kItems; ++k) s[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int i = 0; i < parts; i += 2) {
+        if (i > 0 || base != mine) {
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k) ahead[k] = load(base + k % kItems * kT, i + k / kItems);
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+          add(s[k % kItems], ahead[k], weight(base + k % kItems * kT, i + k / kItems));
+      }
+#pragma unroll
+      for (int k = 0; k < kItems; ++k) store(base + k * kT, s[k]);
+    }
+  }
+}
+
 template <int D, bool F8, int MT>
 __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
     paged_attn_kernel(const __grid_constant__ PAttnArgs a, const __grid_constant__ CUtensorMap map_k,
@@ -214,6 +336,8 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[C::kMaxNS], empty[C::kMaxNS];
   __shared__ int sm[32];
+  __shared__ int jn[JOIN_INTS], joined;
+  __shared__ unsigned long long gbar_base;
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   float* merge = reinterpret_cast<float*>(ring + (size_t)NS * C::kSlot);
   float2* merge_ml = reinterpret_cast<float2*>(merge + kWarps * 16 * C::kMergeRow);
@@ -228,6 +352,8 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
     }
     mbar_fence_init();
   }
+  if (warp == kWarps && lane < 2)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(lane ? &map_v : &map_k) : "memory");
   pdl_wait();
   pdl_launch_dependents();
   // units of the slots before each slot
@@ -256,25 +382,6 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
   Walk w;
   w.u = min(total, (int)blockIdx.x * per);
   w.end = min(total, w.u + per);
-  if (tid == 0) {
-    int32_t* jn = a.joins + (int64_t)blockIdx.x * JOIN_INTS;
-    int parts = 0;
-    if (w.u < w.end) {
-      w.seek(S, a.B, HR);
-      const int u0 = w.base + w.job * w.W + kSetup;  // the job's first unit of keys
-      if (u0 < w.u) {
-        const int c0 = u0 / per;
-        parts = (u0 - kSetup + w.W - 1) / per - c0 + 1;
-        jn[JOIN_FIRST] = c0;
-        jn[JOIN_SECOND] = u0 - kSetup > c0 * per;  // another job's units lie before it in that CTA
-        jn[JOIN_SLOT] = w.b;
-        jn[JOIN_HEAD] = w.job / a.row_blocks;
-        jn[JOIN_BLOCK] = w.job % a.row_blocks;
-      }
-    }
-    jn[JOIN_PARTS] = parts;
-  }
-
   if (warp >= kWarps) {
     // ---------------------------------------------------------------- producer
     const int none = a.num_pages * a.Hkv;  // a page that is not there: outside the map, reads as zero
@@ -350,6 +457,31 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
   }
 
   // ------------------------------------------------------------------ consumers
+  // Off the others' way while the first tile travels: where the grid barrier stands (every launch adds one arrival a CTA,
+  // so whatever is read before this CTA's own gives the launch's start), and the split job at the border before this CTA.
+  if (tid == 32) {
+    const unsigned long long v = ld_relaxed_u64(a.gbar);
+    gbar_base = v - v % gridDim.x;
+  }
+  if (tid == 64) {
+    int parts = 0;
+    Walk at = w;
+    if (at.u < at.end) {
+      at.seek(S, a.B, HR);
+      const int u0 = at.base + at.job * at.W + kSetup;  // the job's first unit of keys
+      if (u0 < at.u) {
+        const int c0 = u0 / per;
+        parts = (u0 - kSetup + at.W - 1) / per - c0 + 1;
+        jn[JOIN_FIRST] = c0;
+        jn[JOIN_SECOND] = u0 - kSetup > c0 * per;  // another job's units lie before it in that CTA
+        jn[JOIN_SLOT] = at.b;
+        jn[JOIN_HEAD] = at.job / a.row_blocks;
+        jn[JOIN_BLOCK] = at.job % a.row_blocks;
+      }
+    }
+    jn[JOIN_PARTS] = parts;
+  }
+
   const int g = warp / MT, mt = warp % MT, qr = lane >> 2, ql = lane & 3;
   const uint32_t ring32 = smem_u32(ring);
   // this lane's row of an ldmatrix: k takes the four 8x8 blocks (keys 0-7, chunk c), (0-7, c+1), (8-15, c), (8-15, c+1);
@@ -372,7 +504,7 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
     const bool whole = run == w.W - kSetup;
     // this lane's two rows: query row r of the kv head is token r / G, head h G + r % G
     const int rA = rb * a.rows + mt * 16 + qr, rB = rA + 8, M = a.G * a.Tq;
-    const int tA = rA / a.G, tB = rB / a.G;
+    const int tA = token_of(a, rA), tB = token_of(a, rB);
     const int limA = rA < M ? n - a.Tq + tA + 1 : 0, limB = rB < M ? n - a.Tq + tB + 1 : 0;  // keys the row sees
     auto q_row = [&](int r, int t) {
       return a.q + (((int64_t)w.b * a.Tq + t) * a.Hq + h * a.G + (r - t * a.G)) * D;
@@ -573,7 +705,7 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
              [](float (&d)[4], const uint32_t (&p)[4], uint32_t b0, uint32_t b1) { mma16816<F8>(d, p, b0, b1); });
         } else {
           // one pass per token of these rows, over the keys that token sees, kept by its rows alone
-          const int t0 = (rb * a.rows + mt * 16) / a.G, t1 = min(a.Tq - 1, (rb * a.rows + mt * 16 + 15) / a.G);
+          const int r0 = rb * a.rows + mt * 16, t0 = token_of(a, r0), t1 = min(a.Tq - 1, token_of(a, r0 + 15));
 #pragma unroll 1
           for (int t = t0; t <= t1; ++t) {
             const int vis = n - a.Tq + t + 1 - key0;  // keys of the tile that token t sees
@@ -608,63 +740,78 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
     mA = mA == -INFINITY ? mA : mA * fA;
     mB = mB == -INFINITY ? mB : mB * fB;
 
-    // The job's end: the NG warps of a row tile meet in shared memory, 32 columns at a time; a thread then holds four
-    // columns of one row, scales the warps' sums to their common maximum and stores them.
+    // The job's end: the NG warps of a row tile exchange their maxima and sums, scale what they hold to the common
+    // maximum, and add up in shared memory, kMergeCols columns at a time; a thread then holds four columns of a row.
     if (ql == 0) {
       merge_ml[warp * 16 + qr] = make_float2(mA, lA);
       merge_ml[warp * 16 + qr + 8] = make_float2(mB, lB);
     }
-    const int orow = (tid >> 3) & 15, ocol = (tid & 7) * 4;  // 16 rows x 32 columns, 128 threads a turn
+    consumers_sync();
+    float sA, sB;  // this warp's factors
+    {
+      float xA = -INFINITY, xB = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        xA = fmaxf(xA, merge_ml[(k * MT + mt) * 16 + qr].x);
+        xB = fmaxf(xB, merge_ml[(k * MT + mt) * 16 + qr + 8].x);
+      }
+      sA = ex2(mA - (xA == -INFINITY ? 0.f : xA));
+      sB = ex2(mB - (xB == -INFINITY ? 0.f : xB));
+    }
+    constexpr int kLanes = C::kMergeCols / 4, kRows = kWarps * 32 / kLanes;  // threads of a row, rows a turn
+    const int ocol = (tid % kLanes) * 4;
     const float vs = a.v_scale ? a.v_scale[h] : 1.f;
 #pragma unroll
     for (int c0 = 0; c0 < D; c0 += C::kMergeCols) {
-      float* mine = merge + warp * 16 * C::kMergeRow;
+      float* mine = merge + (warp * 16 + qr) * C::kMergeRow;
 #pragma unroll
       for (int j = c0 / 8; j < (c0 + C::kMergeCols) / 8; j += F8 ? 2 : 1) {
         // columns of accumulator tile j: bf16 8 j + 2 ql, + 1; e4m3 (tiles j, j + 1) 8 j + 4 ql + {0, 2}, + {1, 3}
         if constexpr (!F8) {
-          *reinterpret_cast<float2*>(mine + qr * C::kMergeRow + 8 * j - c0 + 2 * ql) = make_float2(acc[j][0], acc[j][1]);
-          *reinterpret_cast<float2*>(mine + (qr + 8) * C::kMergeRow + 8 * j - c0 + 2 * ql) =
-              make_float2(acc[j][2], acc[j][3]);
+          float* at = mine + 8 * j - c0 + 2 * ql;
+          *reinterpret_cast<float2*>(at) = make_float2(acc[j][0] * sA, acc[j][1] * sA);
+          *reinterpret_cast<float2*>(at + 8 * C::kMergeRow) = make_float2(acc[j][2] * sB, acc[j][3] * sB);
         } else {
-          *reinterpret_cast<float4*>(mine + qr * C::kMergeRow + 8 * j - c0 + 4 * ql) =
-              make_float4(acc[j][0], acc[j + 1][0], acc[j][1], acc[j + 1][1]);
-          *reinterpret_cast<float4*>(mine + (qr + 8) * C::kMergeRow + 8 * j - c0 + 4 * ql) =
-              make_float4(acc[j][2], acc[j + 1][2], acc[j][3], acc[j + 1][3]);
+          float* at = mine + 8 * j - c0 + 4 * ql;
+          *reinterpret_cast<float4*>(at) = make_float4(acc[j][0] * sA, acc[j + 1][0] * sA, acc[j][1] * sA, acc[j + 1][1] * sA);
+          *reinterpret_cast<float4*>(at + 8 * C::kMergeRow) =
+              make_float4(acc[j][2] * sB, acc[j + 1][2] * sB, acc[j][3] * sB, acc[j + 1][3] * sB);
         }
       }
       consumers_sync();
 #pragma unroll 1
-      for (int x = 0; x < MT; ++x) {
-        const int lr = x * 16 + orow, row = rb * a.rows + lr;  // row in the block, in the job's kv head
-        if (row < M) {
-          float m = -INFINITY;
+      for (int lr = tid / kLanes; lr < min(MT * 16, M - rb * a.rows); lr += kRows) {
+        const int x = lr >> 4, row = rb * a.rows + lr;  // row tile; row in the job's kv head
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int k = 0; k < NG; ++k) m = fmaxf(m, merge_ml[(k * MT + x) * 16 + orow].x);
-          const float z = m == -INFINITY ? 0.f : m;
-          float l = 0.f;
-          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < NG; ++k) {
+          const float4 p =
+              *reinterpret_cast<const float4*>(merge + ((k * MT + x) * 16 + (lr & 15)) * C::kMergeRow + ocol);
+          o.x += p.x;
+          o.y += p.y;
+          o.z += p.z;
+          o.w += p.w;
+        }
+        float m = -INFINITY, l = 0.f;
+        if (whole || (c0 == 0 && ocol == 0)) {
+          float2 ml[NG];
 #pragma unroll
           for (int k = 0; k < NG; ++k) {
-            const float2 ml = merge_ml[(k * MT + x) * 16 + orow];
-            const float f = ex2(ml.x - z);
-            l = fmaf(ml.y, f, l);
-            const float4 p = *reinterpret_cast<const float4*>(merge + ((k * MT + x) * 16 + orow) * C::kMergeRow + ocol);
-            o.x = fmaf(p.x, f, o.x);
-            o.y = fmaf(p.y, f, o.y);
-            o.z = fmaf(p.z, f, o.z);
-            o.w = fmaf(p.w, f, o.w);
+            ml[k] = merge_ml[(k * MT + x) * 16 + (lr & 15)];
+            m = fmaxf(m, ml[k].x);
           }
-          if (whole) {
-            const float d = l == 0.f ? 0.f : vs / l;  // an empty row is zero; a NaN sum stays
-            const int t = row / a.G;
-            uint16_t* dst = a.out + (((int64_t)w.b * a.Tq + t) * a.Hq + h * a.G + (row - t * a.G)) * D + c0 + ocol;
-            *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<false>(o.x * d, o.y * d), pack2<false>(o.z * d, o.w * d));
-          } else {
-            const int64_t at = ((int64_t)blockIdx.x * 2 + (njob > 0)) * a.rows + lr;
-            if (c0 == 0 && ocol == 0) *reinterpret_cast<float2*>(a.ml + at * 2) = make_float2(m, l);
-            *reinterpret_cast<float4*>(a.acc + at * D + c0 + ocol) = o;
-          }
+#pragma unroll
+          for (int k = 0; k < NG; ++k) l = fmaf(ml[k].y, ex2(ml[k].x - (m == -INFINITY ? 0.f : m)), l);
+        }
+        if (whole) {
+          const float d = l == 0.f ? 0.f : vs / l;  // an empty row is zero; a NaN sum stays
+          const int t = token_of(a, row);
+          uint16_t* dst = a.out + (((int64_t)w.b * a.Tq + t) * a.Hq + h * a.G + (row - t * a.G)) * D + c0 + ocol;
+          *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<false>(o.x * d, o.y * d), pack2<false>(o.z * d, o.w * d));
+        } else {
+          const int64_t at = ((int64_t)blockIdx.x * 2 + (njob > 0)) * a.rows + lr;
+          if (c0 == 0 && ocol == 0) *reinterpret_cast<float2*>(a.ml + at * 2) = make_float2(m, l);
+          *reinterpret_cast<float4*>(a.acc + at * D + c0 + ocol) = o;
         }
       }
       consumers_sync();
@@ -676,120 +823,25 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
       const int t = k < slot ? turn : turn - 1;  // the slot's last turn
       if (t >= 0) bar_wait(&full[k], t & 1);
     }
-}
-
-// The join. Border c (before CTA c) inside a job of CTAs c0 .. c1 takes the (c - c0 - 1)-th of c1 - c0 equal shares of
-// the job's (row, four columns) items: their parts, one per CTA of the job in order, are weighted by 2^(m_i - m) and
-// added. A share of few items has its parts spread over the threads.
-constexpr int kJoinThreads = 256;
-template <int D>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PAttnArgs a) {
-  constexpr int kCols = D / 4, kMaxRows = 64;
-  // weights of the share's rows: rows * parts <= (64 / (parts - 1) + 2) * parts
-  __shared__ float wt[2 * kMaxRows + 2 * kPagedMaxCtas];
-  __shared__ float inv[kMaxRows];
-  __shared__ float4 red[kJoinThreads];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x + 1;
-  pdl_wait();
-  pdl_launch_dependents();
-  const int32_t* jn = a.joins + (int64_t)c * JOIN_INTS;
-  const int parts = jn[JOIN_PARTS];
-  if (parts == 0) return;
-  const int c0 = jn[JOIN_FIRST], second = jn[JOIN_SECOND], b = jn[JOIN_SLOT], h = jn[JOIN_HEAD], rb = jn[JOIN_BLOCK];
-  const int rows = min(a.rows, a.G * a.Tq - rb * a.rows), all = rows * kCols, share = c - c0 - 1;
-  const int i0 = (int)((int64_t)all * share / (parts - 1)), i1 = (int)((int64_t)all * (share + 1) / (parts - 1));
-  if (i0 >= i1) return;
-  const int r0 = i0 / kCols, r1 = (i1 - 1) / kCols + 1;
-  auto part = [&](int i) { return (int64_t)(c0 + i) * 2 + (i == 0 ? second : 0); };
-  // slices: the parts of an item over as many threads as the share leaves, a power of two up to 32
-  int slices = 1;
-  while (slices < 32 && (i1 - i0) * slices * 2 <= kJoinThreads) slices *= 2;
-  const int lanes = kJoinThreads / slices, sl = tid / lanes;
-  // the first four parts of the thread's first item are on their way while the weights are found
-  constexpr int kAhead = 4;
-  float4 ahead[kAhead];
-  {
-    const int it = min(i0 + tid % lanes, i1 - 1), r = it / kCols, col = it % kCols;
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int i = sl + k * slices;
-      ahead[k] = i < parts ? *reinterpret_cast<const float4*>(a.acc + (part(i) * a.rows + r) * D + col * 4)
-                           : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-  }
-  for (int r = r0 + warp; r < r1; r += kJoinThreads / 32) {
-    float2 x[kAhead];
-    float m = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int i = lane + 32 * k;
-      x[k] = i < parts ? *reinterpret_cast<const float2*>(a.ml + (part(i) * a.rows + r) * 2) : make_float2(-INFINITY, 0.f);
-    }
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) m = fmaxf(m, x[k].x);
-    for (int i = lane + 32 * kAhead; i < parts; i += 32) m = fmaxf(m, a.ml[(part(i) * a.rows + r) * 2]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float z = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    for (int i = lane, k = 0; i < parts; i += 32, ++k) {
-      float2 v;
-      if (k < kAhead) v = k == 0 ? x[0] : (k == 1 ? x[1] : (k == 2 ? x[2] : x[3]));
-      else v = *reinterpret_cast<const float2*>(a.ml + (part(i) * a.rows + r) * 2);
-      const float f = ex2(v.x - z);
-      wt[(r - r0) * parts + i] = f;
-      l = fmaf(v.y, f, l);
-    }
-    l = warp_sum(l);
-    if (lane == 0) inv[r - r0] = l == 0.f ? 0.f : (a.v_scale ? a.v_scale[h] : 1.f) / l;
-  }
-  __syncthreads();
-  for (int base = i0; base < i1; base += lanes) {
-    const int it = base + tid % lanes;
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (it < i1) {
-      const int r = it / kCols, col = it % kCols;
-      const float* w = wt + (r - r0) * parts;
-      int i = sl;
-      if (base == i0) {
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k, i += slices) {
-          const float f = i < parts ? w[i] : 0.f;
-          s.x = fmaf(ahead[k].x, f, s.x);
-          s.y = fmaf(ahead[k].y, f, s.y);
-          s.z = fmaf(ahead[k].z, f, s.z);
-          s.w = fmaf(ahead[k].w, f, s.w);
-        }
+  // The split jobs. Every CTA arrives once its parts are written; one whose share began inside a job waits for all (the
+  // launch is cooperative, so all are resident) and takes its share of that job's join. The ring is free by now.
+  consumers_sync();
+  if (tid == 0) asm volatile("red.release.gpu.global.add.u64 [%0], 1;" ::"l"(a.gbar) : "memory");
+  if (jn[JOIN_PARTS] == 0) return;
+  if (tid == 0) {
+    int there = 1;
+    for (long long it = 0; ld_acquire_u64(a.gbar) < gbar_base + gridDim.x;) {
+      if (++it > kSpinLimit) {
+        atomicOr(a.err, (uint32_t)MOE_ERR_BARRIER);
+        there = 0;
+        break;
       }
-#pragma unroll 4
-      for (; i < parts; i += slices) {
-        const float4 x = *reinterpret_cast<const float4*>(a.acc + (part(i) * a.rows + r) * D + col * 4);
-        const float f = w[i];
-        s.x = fmaf(x.x, f, s.x);
-        s.y = fmaf(x.y, f, s.y);
-        s.z = fmaf(x.z, f, s.z);
-        s.w = fmaf(x.w, f, s.w);
-      }
+      if (it > 64) __nanosleep(20);
     }
-    if (slices > 1) {  // one round only: the share fits the threads
-      red[tid] = s;
-      __syncthreads();
-      if (sl != 0) return;
-      for (int k = 1; k < slices; ++k) {
-        const float4 x = red[k * lanes + tid];
-        s.x += x.x;
-        s.y += x.y;
-        s.z += x.z;
-        s.w += x.w;
-      }
-    }
-    if (it < i1) {
-      const int r = it / kCols, col = it % kCols, q = rb * a.rows + r, t = q / a.G;
-      const float d = inv[r - r0];
-      *reinterpret_cast<uint2*>(a.out + (((int64_t)b * a.Tq + t) * a.Hq + h * a.G + (q - t * a.G)) * D + col * 4) =
-          make_uint2(pack2<false>(s.x * d, s.y * d), pack2<false>(s.z * d, s.w * d));
-    }
+    joined = there;
   }
+  consumers_sync();
+  if (joined) join_share<D>(a, jn, *reinterpret_cast<JoinScratch*>(ring));
 }
 
 // ------------------------------------------------------------------ host side
@@ -839,11 +891,7 @@ cudaError_t launch_attn(const PAttnArgs& args, const CUtensorMap& mk, const CUte
   a.ctas = std::min(kPagedMaxCtas, paged_sms() * C::kPerSm);
   CUtensorMap k = mk, v = mv;
   void* p[] = {&a, &k, &v};
-  e = paged_launch(fn, dim3(a.ctas), dim3(C::kThreads), smem, s, p);
-  if (e != cudaSuccess) return e;
-  void* j[] = {&a};
-  return paged_launch(reinterpret_cast<const void*>(paged_join_kernel<D>), dim3(a.ctas - 1),
-                      dim3(kJoinThreads), 0, s, j);
+  return paged_launch(fn, dim3(a.ctas), dim3(C::kThreads), smem, s, p, 1, true);
 }
 
 template <int D, bool F8>
@@ -880,7 +928,7 @@ int moe_paged_attend(const moe_paged_cache* c, int layer, const int32_t* seqs, i
   a.seqs = seqs;
   a.tables = c->tables;
   a.lens = c->lens;
-  a.joins = reinterpret_cast<int32_t*>(ws + L.joins);
+  a.gbar = reinterpret_cast<unsigned long long*>(ws + (c->D == 256 ? L.gbar1 : L.gbar2));
   a.ml = reinterpret_cast<float*>(ws + L.ml);
   a.acc = reinterpret_cast<float*>(ws + L.acc);
   a.err = reinterpret_cast<uint32_t*>(ws + L.err);
@@ -896,6 +944,7 @@ int moe_paged_attend(const moe_paged_cache* c, int layer, const int32_t* seqs, i
   a.rows = paged_block_rows(a.G, Tq);
   a.row_blocks = (a.G * Tq + a.rows - 1) / a.rows;
   a.scale = scale;
+  a.inv_G = 1.f / (float)a.G;
   a.ctas = 0;
   // the flattened unit list is counted in 32 bits; a unit is at least 16 keys
   const int64_t units = ((int64_t)c->max_pages * c->page + 15) / 16 + kSetup;
