@@ -28,8 +28,8 @@ inline int paged_block_rows(int G, int Tq) {
 // Offsets (bytes) of the caller-owned workspace's sections, each 256-byte aligned. The error word leads; what the page
 // calls and the attention keep shares the space behind it, since one workspace serves one call at a time.
 struct PagedWs {
-  // grid-barrier counters, one for each size of grid that counts on it: one CTA an SM, two, and the page calls'
-  size_t err, gbar1, gbar2, gbar_pages;
+  // arrivals at the attention's grid barrier, one counter for each size of grid: one CTA an SM, two
+  size_t err, gbar1, gbar2;
   // page calls: number of page copies, their (source, destination, rows) triples, the free-page list and the page map
   size_t ncopy, copies, list, map;
   // attention: partial maxima and sums, partial accumulators
@@ -41,7 +41,7 @@ inline PagedWs paged_ws(const moe_paged_cache* c, int Hq, int max_batch, int max
   PagedWs L;
   size_t o = 0;
   L.err = o;    o = ws_align(o + 4);
-  L.gbar1 = o;  L.gbar2 = o + 64;  L.gbar_pages = o + 128;  o = ws_align(o + 192);
+  L.gbar1 = o;  L.gbar2 = o + 64;  o = ws_align(o + 128);
   const size_t base = o;
   L.ncopy = o;  o = ws_align(o + 4);
   L.copies = o; o = ws_align(o + 12 * (size_t)(c->num_pages > max_batch ? c->num_pages : max_batch));

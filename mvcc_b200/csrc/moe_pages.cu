@@ -3,8 +3,10 @@
 //
 // A page call is a plan and a move. The plan (which pages change hands) is integer work over lists, tables and the
 // holder counts: one CTA of 1024 threads, so that its steps are separated by block barriers and its result depends on
-// the inputs alone. The move (plane_copy_kernel) is pure traffic: the plan's (source, destination, rows) triples times
-// layers times {k, v}, cut into 16 KB pieces that the whole GPU takes in turn.
+// the inputs alone. The move is pure traffic: the plan's (source, destination, rows) triples times layers times {k, v},
+// cut into 16 KB pieces that the whole GPU takes in turn. The move is a launch of its own, programmatically dependent on
+// the plan's: as one cooperative launch with a barrier between them, forking 32 sequences and growing them took 36 us
+// instead of 22.
 #include <algorithm>
 #include <cstring>
 
@@ -35,26 +37,35 @@ struct PageArgs {
 
 // The lowest `want` free pages in ascending order into list (all of them when want >= their number); returns how many
 // were found, the same in every thread. Each warp looks at 32 k pages a turn, lane by lane, so that a ballot gives
-// the order.
-__device__ int find_free(const int32_t* refs, int num_pages, int want, int32_t* list, int* sm) {
-  constexpr int kU = 4;
+// the order. `ahead`: the first turn's holder counts, read before.
+constexpr int kFreeU = 4;
+struct Ahead {
+  int refs[kFreeU];
+  __device__ __forceinline__ void read(const int32_t* r, int num_pages) {
+    const int w0 = (threadIdx.x >> 5) * 32 * kFreeU + (threadIdx.x & 31);
+#pragma unroll
+    for (int u = 0; u < kFreeU; ++u) refs[u] = w0 + u * 32 < num_pages ? __ldcg(r + w0 + u * 32) : 1;
+  }
+};
+__device__ int find_free(const int32_t* refs, int num_pages, int want, int32_t* list, int* sm, const Ahead* ahead) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int found = 0;
-  for (int base = 0; base < num_pages && found < want; base += kPlanThreads * kU) {
-    const int w0 = base + warp * 32 * kU;
-    uint32_t free_mask[kU];
+  for (int base = 0; base < num_pages && found < want; base += kPlanThreads * kFreeU) {
+    const int w0 = base + warp * 32 * kFreeU;
+    uint32_t free_mask[kFreeU];
     int mine = 0;
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
+    for (int u = 0; u < kFreeU; ++u) {
       const int p = w0 + u * 32 + lane;
-      free_mask[u] = __ballot_sync(0xffffffffu, p < num_pages && __ldcg(refs + p) == 0);
+      const int r = base == 0 && ahead ? ahead->refs[u] : (p < num_pages ? __ldcg(refs + p) : 1);
+      free_mask[u] = __ballot_sync(0xffffffffu, r == 0);
       mine += __popc(free_mask[u]);
     }
     int total;
     const int before = block_excl_scan(lane == 0 ? mine : 0, sm, &total);
     int at = found + __shfl_sync(0xffffffffu, before, 0);
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
+    for (int u = 0; u < kFreeU; ++u) {
       if (free_mask[u] >> lane & 1) {
         const int i = at + __popc(free_mask[u] & ((1u << lane) - 1));
         if (i < want) list[i] = w0 + u * 32 + lane;
@@ -69,11 +80,11 @@ __device__ int find_free(const int32_t* refs, int num_pages, int want, int32_t* 
 
 __device__ __forceinline__ bool page_ok(const PageArgs& a, int p) { return p >= 0 && p < a.num_pages; }
 
-// moe_paged_resize. Shared memory: six ints a list entry and a bit a sequence.
+// moe_paged_resize. Shared memory: five ints a list entry and a bit a sequence.
 __global__ void __launch_bounds__(kPlanThreads) resize_plan_kernel(const __grid_constant__ PageArgs a) {
   extern __shared__ int sh[];
   __shared__ int sm[32];
-  __shared__ int bad, copies;
+  __shared__ int bad, copies, released;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = kPlanThreads / 32, n = a.n, pg = a.page;
   int* seq = sh;
   int* old = seq + n;
@@ -83,9 +94,12 @@ __global__ void __launch_bounds__(kPlanThreads) resize_plan_kernel(const __grid_
   uint32_t* seen = reinterpret_cast<uint32_t*>(start + n);
   pdl_wait();
   pdl_launch_dependents();
+  Ahead ahead;
+  ahead.read(a.refs, a.num_pages);
   if (tid == 0) {
     bad = 0;
     copies = 0;
+    released = 0;
     *a.ncopy = 0;
   }
   for (int i = tid; i < (a.max_seqs + 31) / 32; i += kPlanThreads) seen[i] = 0;
@@ -114,6 +128,7 @@ __global__ void __launch_bounds__(kPlanThreads) resize_plan_kernel(const __grid_
       if (page_ok(a, p)) atomicSub(&a.refs[p], 1);
       else atomicOr(a.err, (uint32_t)MOE_ERR_PAGE_ID);
     }
+    if (lane == 0 && want < held) released = 1;
   }
   // 2. the partly filled page at the end of what stays
   for (int i = tid; i < n; i += kPlanThreads) {
@@ -154,7 +169,7 @@ __global__ void __launch_bounds__(kPlanThreads) resize_plan_kernel(const __grid_
     if (base > a.num_pages) break;  // more than there can be: no sum may pass the list
   }
   const int want_all = base;
-  const int found = want_all > a.num_pages ? -1 : find_free(a.refs, a.num_pages, want_all, a.list, sm);
+  const int found = want_all > a.num_pages ? -1 : find_free(a.refs, a.num_pages, want_all, a.list, sm, released ? nullptr : &ahead);
   __syncthreads();
   if (found < want_all) {  // nothing is changed: the holders come back
     for (int i = warp; i < n; i += nw) {
@@ -211,14 +226,16 @@ __global__ void __launch_bounds__(kPlanThreads) fork_kernel(const __grid_constan
   for (int i = tid; i < (a.max_seqs + 31) / 32; i += kPlanThreads) seen[i] = 0;
   __syncthreads();
   for (int i = tid; i < a.n; i += kPlanThreads) {
-    const int d = a.b[i];
-    if (d < 0 || d >= a.max_seqs || (atomicOr(&seen[d >> 5], 1u << (d & 31)) >> (d & 31) & 1) || a.lens[d] != 0) bad = 1;
+    const int d = a.b[i], s = a.a[i];
+    const bool dst = d >= 0 && d < a.max_seqs, src = s >= 0 && s < a.max_seqs;
+    const int dn = dst ? a.lens[d] : 1, sn = src ? a.lens[s] : -1;
+    if (dn != 0 || sn < 0 || sn > a.max_pages * a.page) bad = 1;
+    if (dst && (atomicOr(&seen[d >> 5], 1u << (d & 31)) >> (d & 31) & 1)) bad = 1;
   }
   __syncthreads();
   for (int i = tid; i < a.n; i += kPlanThreads) {
     const int s = a.a[i];
-    if (s < 0 || s >= a.max_seqs || (seen[s >> 5] >> (s & 31) & 1)) bad = 1;
-    else if (a.lens[s] < 0 || a.lens[s] > a.max_pages * a.page) bad = 1;
+    if (s >= 0 && s < a.max_seqs && (seen[s >> 5] >> (s & 31) & 1)) bad = 1;
   }
   __syncthreads();
   cluster_sync();  // no CTA changes a length before every CTA has looked at them
@@ -252,7 +269,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid
   for (int p = tid; p < a.num_pages; p += kPlanThreads) mine += a.refs[p] != 0;
   int live;
   block_excl_scan(mine, sm, &live);
-  const int holes = find_free(a.refs, live, live, a.list, sm);
+  const int holes = find_free(a.refs, live, live, a.list, sm, nullptr);
   __syncthreads();
   int found = 0;
   for (int base = live; base < a.num_pages && found < holes; base += kPlanThreads * kU) {
@@ -653,7 +670,8 @@ bool ws_ok(const moe_paged_cache* c, int n, void* workspace, size_t bytes, Paged
   return bytes >= L->total;
 }
 
-cudaError_t launch_copy(const moe_paged_cache* c, const PageArgs& p, bool counted, bool tables, cudaStream_t s) {
+// The move of a plan (counted on the device; with the tables for a compaction), or of the caller's lists.
+CopyArgs copy_args(const moe_paged_cache* c, const PageArgs& p, bool planned, bool tables) {
   CopyArgs a;
   memset(&a, 0, sizeof a);
   a.k = static_cast<uint8_t*>(c->k);
@@ -665,7 +683,7 @@ cudaError_t launch_copy(const moe_paged_cache* c, const PageArgs& p, bool counte
   a.row_bytes = c->D * kv_size(c->kv_type);
   a.num_pages = c->num_pages;
   a.err = p.err;
-  if (counted) {
+  if (planned) {
     a.ncopy = p.ncopy;
     a.copies = p.copies;
   } else {
@@ -679,9 +697,13 @@ cudaError_t launch_copy(const moe_paged_cache* c, const PageArgs& p, bool counte
     a.bound = p.list;
     a.entries = (int64_t)c->max_seqs * c->max_pages;
   }
-  void* args[] = {&a};
-  return paged_launch(reinterpret_cast<const void*>(plane_copy_kernel), dim3(paged_sms() * 4), dim3(kCopyThreads), 0, s,
-                      args);
+  return a;
+}
+
+cudaError_t launch_copy(const CopyArgs& args, cudaStream_t s) {
+  CopyArgs a = args;
+  void* p[] = {&a};
+  return paged_launch(reinterpret_cast<const void*>(plane_copy_kernel), dim3(paged_sms() * 4), dim3(kCopyThreads), 0, s, p);
 }
 
 }  // namespace
@@ -719,7 +741,7 @@ int moe_paged_resize(const moe_paged_cache* c, const int32_t* seqs, const int32_
   e = paged_launch(reinterpret_cast<const void*>(resize_plan_kernel), dim3(1), dim3(kPlanThreads), smem,
                    (cudaStream_t)stream, args);
   if (e != cudaSuccess) return (int)e;
-  return (int)launch_copy(c, a, true, false, (cudaStream_t)stream);
+  return (int)launch_copy(copy_args(c, a, true, false), (cudaStream_t)stream);
 }
 
 int moe_paged_fork(const moe_paged_cache* c, const int32_t* src, const int32_t* dst, int n, void* workspace,
@@ -742,7 +764,7 @@ int moe_paged_compact(const moe_paged_cache* c, void* workspace, size_t workspac
   cudaError_t e = paged_launch(reinterpret_cast<const void*>(compact_plan_kernel), dim3(1), dim3(kPlanThreads), 0,
                                (cudaStream_t)stream, args);
   if (e != cudaSuccess) return (int)e;
-  return (int)launch_copy(c, a, true, true, (cudaStream_t)stream);
+  return (int)launch_copy(copy_args(c, a, true, true), (cudaStream_t)stream);
 }
 
 int moe_paged_copy(const moe_paged_cache* c, const int32_t* src, const int32_t* dst, int n, void* workspace,
@@ -751,7 +773,7 @@ int moe_paged_copy(const moe_paged_cache* c, const int32_t* src, const int32_t* 
   if (n < 0 || !ws_ok(c, 1, workspace, workspace_bytes, &L)) return (int)cudaErrorInvalidValue;
   if (n == 0) return (int)cudaSuccess;
   if (!src || !dst) return (int)cudaErrorInvalidValue;
-  return (int)launch_copy(c, page_args(c, src, dst, n, workspace, L), false, false, (cudaStream_t)stream);
+  return (int)launch_copy(copy_args(c, page_args(c, src, dst, n, workspace, L), false, false), (cudaStream_t)stream);
 }
 
 int moe_paged_append(const moe_paged_cache* c, int layer, const int32_t* seqs, int B, int Tq, const uint16_t* qkv,
