@@ -72,6 +72,7 @@ struct Cfg {
   static constexpr int kPerSm = D == 256 ? 1 : 2;         // CTAs an SM: registers (accumulator D / 2 a lane)
   static constexpr int NP = 4 / kPerSm;                   // producer warps
   static constexpr int kThreads = (kWarps + NP) * 32;
+  static constexpr int kJoin = NP == 4 ? 256 : 128;       // threads of the join: a power of two
   static constexpr int kMergeCols = D == 256 ? 64 : 32;   // columns that meet at a time at a job's end
   static constexpr int kMergeRow = kMergeCols + 4;        // floats of a row in the merge buffer, padded
   static constexpr int kMerge = kWarps * 16 * (kMergeRow + 2) * 4;  // every warp's columns; maxima and sums
@@ -142,6 +143,10 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
 __device__ __forceinline__ void mbar_arrive(uint64_t* mbar) {
   asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(smem_u32(mbar)) : "memory");
 }
+template <int kT>
+__device__ __forceinline__ void join_sync() {
+  asm volatile("bar.sync 2, %0;" ::"n"(kT) : "memory");
+}
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
 
 // Whether one of the values in w (two bf16, or four e4m3) is NaN or infinite.
@@ -153,6 +158,7 @@ __device__ __forceinline__ bool not_finite(uint32_t w) {
 
 // Keys of slot b: its sequence's length, 0 for an unused slot or a bad entry (recorded).
 __device__ __forceinline__ int slot_keys(const PAttnArgs& a, int b, int* seq) {
+  const int own = b < a.max_seqs ? a.lens[b] : 0;  // slot b is often sequence b: its length is asked for at once
   const int s = a.seqs[b];
   *seq = 0;
   if (s == -1) return 0;
@@ -161,7 +167,7 @@ __device__ __forceinline__ int slot_keys(const PAttnArgs& a, int b, int* seq) {
     return 0;
   }
   *seq = s;
-  const int n = a.lens[s];
+  const int n = s == b ? own : a.lens[s];
   if (n < 0 || n > a.max_pages * a.page) {
     atomicOr(a.err, (uint32_t)MOE_ERR_SEQ_ID);
     return 0;
@@ -176,7 +182,8 @@ enum { JOIN_PARTS = 0, JOIN_FIRST, JOIN_SECOND, JOIN_SLOT, JOIN_HEAD, JOIN_BLOCK
 // The share of one CTA: [u, end) of the flattened list, walked job by job. A job counts kSetup units of its own before
 // its units of keys: its queries, its first tile's latency and its merge cost a CTA about as much, and a batch with
 // many short sequences would otherwise pile them up in a few CTAs.
-constexpr int kSetup = 5;
+constexpr int setup_units(int MT) { return MT == 1 ? 5 : (MT == 2 ? 9 : 16); }
+template <int kSetup>
 struct Walk {
   int u, end;           // what is left of the share
   int b, job, W;        // the slot, its job (kv head and row block), units of each of its jobs
@@ -208,19 +215,19 @@ struct Walk {
   }
 };
 
-// The join, by the consumer threads of CTA c, whose share begins inside a job of CTAs c0 .. c1: they take the
+// The join, by kT threads of CTA c, whose share begins inside a job of CTAs c0 .. c1: they take the
 // (c - c0 - 1)-th of c1 - c0 equal shares of the job's (row, four columns) items. An item's parts, one per CTA of the
 // job in order, are weighted by 2^(m_i - m) and added; a share of few items has its parts spread over the threads.
 struct JoinScratch {
   static constexpr int kMaxRows = 64;
-  float4 red[kWarps * 32];
+  float4 red[256];
   // weights of the share's rows: rows * parts <= (64 / (parts - 1) + 2) * parts
   float wt[2 * kMaxRows + 2 * kPagedMaxCtas];
   float inv[kMaxRows];
 };
-template <int D>
+template <int D, int kT>
 __device__ void join_share(const PAttnArgs& a, const int (&jn)[JOIN_INTS], JoinScratch& js) {
-  constexpr int kCols = D / 4, kT = kWarps * 32;
+  constexpr int kCols = D / 4;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x;
   const int parts = jn[JOIN_PARTS], c0 = jn[JOIN_FIRST], second = jn[JOIN_SECOND], b = jn[JOIN_SLOT], h = jn[JOIN_HEAD],
             rb = jn[JOIN_BLOCK];
@@ -259,7 +266,7 @@ __device__ void join_share(const PAttnArgs& a, const int (&jn)[JOIN_INTS], JoinS
 #pragma unroll
   for (int k = 0; k < kAhead; ++k)
     ahead[k] = slices > 1 ? load(mine, sl + k * slices) : load(mine + k % kItems * kT, k / kItems);
-  for (int r = r0 + warp; r < r1; r += kWarps) {
+  for (int r = r0 + warp; r < r1; r += kT / 32) {
     constexpr int kHeld = 3;  // a lane's parts that stay in registers
     float2 x[kHeld];
     float m = -INFINITY;
@@ -292,7 +299,7 @@ __device__ void join_share(const PAttnArgs& a, const int (&jn)[JOIN_INTS], JoinS
     l = warp_sum(l);
     if (lane == 0) js.inv[r - r0] = l == 0.f ? 0.f : (a.v_scale ? a.v_scale[h] : 1.f) / l;
   }
-  consumers_sync();
+  join_sync<kT>();
   if (slices > 1) {
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -300,7 +307,7 @@ __device__ void join_share(const PAttnArgs& a, const int (&jn)[JOIN_INTS], JoinS
 #pragma unroll 4
     for (int i = sl + kAhead * slices; i < parts; i += slices) add(s, load(mine, i), weight(mine, i));
     js.red[tid] = s;
-    consumers_sync();
+    join_sync<kT>();
     if (sl != 0) return;
     for (int k = 1; k < slices; ++k) add(s, js.red[k * lanes + tid], 1.f);
     store(mine, s);
@@ -329,7 +336,7 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
     paged_attn_kernel(const __grid_constant__ PAttnArgs a, const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v) {
   using C = Cfg<D, F8>;
-  constexpr int NG = kWarps / MT, KT = C::KT, UK = NG * KT, NP = C::NP, kThreads = C::kThreads;
+  constexpr int NG = kWarps / MT, KT = C::KT, UK = NG * KT, NP = C::NP, kThreads = C::kThreads, kSetup = setup_units(MT);
   const int NS = a.ns;
   constexpr int NT = D / 8;     // accumulator tiles of 8 columns
   constexpr int KC = C::kRow / 16;  // 16-byte chunks of a cached row
@@ -379,7 +386,7 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
   }
   const int HR = a.Hkv * a.row_blocks, total = S[a.B] * HR;
   const int per = max(1, (total + a.ctas - 1) / a.ctas);
-  Walk w;
+  Walk<kSetup> w;
   w.u = min(total, (int)blockIdx.x * per);
   w.end = min(total, w.u + per);
   if (warp >= kWarps) {
@@ -453,6 +460,10 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
     if (!ok)  // no copy may still be landing when the CTA exits
       for (int j = max(0, i - NS); j < i; ++j)
         if (j % NP == warp - kWarps) bar_wait(&full[j % NS], (j / NS) & 1);
+    if (tid < C::kJoin) {  // producers that help with the join
+      join_sync<C::kJoin>();
+      if (jn[JOIN_PARTS] != 0 && joined) join_share<D, C::kJoin>(a, jn, *reinterpret_cast<JoinScratch*>(ring));
+    }
     return;
   }
 
@@ -465,7 +476,7 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
   }
   if (tid == 64) {
     int parts = 0;
-    Walk at = w;
+    Walk<kSetup> at = w;
     if (at.u < at.end) {
       at.seek(S, a.B, HR);
       const int u0 = at.base + at.job * at.W + kSetup;  // the job's first unit of keys
@@ -827,8 +838,7 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
   // launch is cooperative, so all are resident) and takes its share of that job's join. The ring is free by now.
   consumers_sync();
   if (tid == 0) asm volatile("red.release.gpu.global.add.u64 [%0], 1;" ::"l"(a.gbar) : "memory");
-  if (jn[JOIN_PARTS] == 0) return;
-  if (tid == 0) {
+  if (tid == 0 && jn[JOIN_PARTS] != 0) {
     int there = 1;
     for (long long it = 0; ld_acquire_u64(a.gbar) < gbar_base + gridDim.x;) {
       if (++it > kSpinLimit) {
@@ -840,8 +850,8 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
     }
     joined = there;
   }
-  consumers_sync();
-  if (joined) join_share<D>(a, jn, *reinterpret_cast<JoinScratch*>(ring));
+  join_sync<C::kJoin>();
+  if (jn[JOIN_PARTS] != 0 && joined) join_share<D, C::kJoin>(a, jn, *reinterpret_cast<JoinScratch*>(ring));
 }
 
 // ------------------------------------------------------------------ host side
@@ -947,7 +957,7 @@ int moe_paged_attend(const moe_paged_cache* c, int layer, const int32_t* seqs, i
   a.inv_G = 1.f / (float)a.G;
   a.ctas = 0;
   // the flattened unit list is counted in 32 bits; a unit is at least 16 keys
-  const int64_t units = ((int64_t)c->max_pages * c->page + 15) / 16 + kSetup;
+  const int64_t units = ((int64_t)c->max_pages * c->page + 15) / 16 + setup_units(4);
   if (B * units * c->Hkv * a.row_blocks >= ((int64_t)1 << 31) - kPagedMaxCtas) return (int)cudaErrorInvalidValue;
   const int kt = tile_keys(c->D * kv_size(c->kv_type));
   a.box_rows = c->page % kt == 0 ? kt : 16;
