@@ -70,9 +70,12 @@ struct Cfg {
   static constexpr int kTile = KT * kRow;                 // bytes of a k or v tile
   static constexpr int kSlot = 2 * kTile;                 // 8 KB, or 16 KB for rows of 512 bytes
   static constexpr int kPerSm = D == 256 ? 1 : 2;         // CTAs an SM: registers (accumulator D / 2 a lane)
-  static constexpr int NP = 4 / kPerSm;                   // producer warps
+  static constexpr int NP = 4;                            // producer warps
   static constexpr int kThreads = (kWarps + NP) * 32;
-  static constexpr int kJoin = NP == 4 ? 256 : 128;       // threads of the join: a power of two
+  static constexpr int kJoin = kPerSm == 1 ? 256 : 128;   // threads of the join (two CTAs an SM: the consumers)
+  // Two CTAs an SM are launched with 128 registers a thread, of which the producers hand most to the consumers.
+  static constexpr int kConsumerRegs = 216, kProducerRegs = 40;
+  static_assert(kPerSm == 1 || kConsumerRegs + kProducerRegs <= 2 * (65536 / (2 * kThreads)), "registers of a launch");
   static constexpr int kMergeCols = D == 256 ? 64 : 32;   // columns that meet at a time at a job's end
   static constexpr int kMergeRow = kMergeCols + 4;        // floats of a row in the merge buffer, padded
   static constexpr int kMerge = kWarps * 16 * (kMergeRow + 2) * 4;  // every warp's columns; maxima and sums
@@ -391,6 +394,7 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
   w.end = min(total, w.u + per);
   if (warp >= kWarps) {
     // ---------------------------------------------------------------- producer
+    if constexpr (C::kPerSm == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kProducerRegs));
     const int none = a.num_pages * a.Hkv;  // a page that is not there: outside the map, reads as zero
     const int nbox = KT / a.box_rows;
     int i = 0;      // tiles so far: slot i % NS, for the turn-th time
@@ -468,6 +472,7 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
   }
 
   // ------------------------------------------------------------------ consumers
+  if constexpr (C::kPerSm == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kConsumerRegs));
   // Off the others' way while the first tile travels: where the grid barrier stands (every launch adds one arrival a CTA,
   // so whatever is read before this CTA's own gives the launch's start), and the split job at the border before this CTA.
   if (tid == 32) {
