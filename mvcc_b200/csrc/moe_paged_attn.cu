@@ -13,8 +13,8 @@
 // each border takes an equal share of the job's rows. (The merge as a kernel of its own cost 3 us of host time and as
 // much between the kernels.)
 //
-// CTA: four consumer warps and NP producer warps, four producers an SM (a thread issues a TMA copy every 95 cycles or
-// so: one alone fetches 3.2 TB/s over the GPU in 2 KB boxes, four 6.4 TB/s). Producer w takes every NP-th of the
+// CTA: four or eight consumer warps and four producer warps (a thread issues a TMA copy every 95 cycles or so: one an SM
+// fetches 3.2 TB/s over the GPU in 2 KB boxes, four 6.4 TB/s). Producer w takes every NP-th of the
 // CTA's tiles (KT keys of k and v each), reads the page ids 32 at a time and fetches the tiles by TMA (boxes of 64 values x 16 or KT rows inside one page, 128-byte
 // swizzle) into a ring of NS slots, mbarrier-counted. Consumer warp (g, mt) holds 16 query rows as MMA fragments and
 // takes every NG-th tile: S = Q K^T, the running maximum and sum of the softmax, O += P V, all in registers; at a job's
@@ -36,7 +36,6 @@
 namespace moe {
 namespace {
 
-constexpr int kWarps = 4;                      // consumer warps
 constexpr int kSmemOne = 226 * 1024;           // dynamic shared memory of a CTA alone on its SM
 constexpr int kSmemTwo = 112 * 1024;           // of one of two
 
@@ -60,7 +59,11 @@ struct PAttnArgs {
 // whole number by 0.5 / G, far more than its rounding.
 __device__ __forceinline__ int token_of(const PAttnArgs& a, int r) { return __float2int_rd(((float)r + 0.5f) * a.inv_G); }
 
-template <int D, bool F8>
+// Three shapes of a CTA. Heads of 64 and 128: two CTAs an SM, four consumer warps each. Heads of 256, one row tile of
+// bf16: one CTA an SM, four consumer warps with queries and accumulator in 255 registers, which keep up with memory.
+// Heads of 256 otherwise ("wide"): the conversion of e4m3 or the second to fourth row tile doubles to quadruples the
+// work a byte, so eight consumer warps, which share the queries in shared memory.
+template <int D, bool F8, int MT>
 struct Cfg {
   static constexpr int kEs = F8 ? 1 : 2;
   static constexpr int kRow = D * kEs;                    // bytes of a cached row
@@ -70,13 +73,19 @@ struct Cfg {
   static constexpr int kTile = KT * kRow;                 // bytes of a k or v tile
   static constexpr int kSlot = 2 * kTile;                 // 8 KB, or 16 KB for rows of 512 bytes
   static constexpr int kPerSm = D == 256 ? 1 : 2;         // CTAs an SM: registers (accumulator D / 2 a lane)
+  static constexpr bool kWide = D == 256 && (F8 || MT > 1);
+  static constexpr int kWarps = kWide ? 8 : 4;            // consumer warps
+  static constexpr int NG = kWarps / MT;                  // key groups
   static constexpr int NP = 4;                            // producer warps
   static constexpr int kThreads = (kWarps + NP) * 32;
-  static constexpr int kJoin = kPerSm == 1 ? 256 : 128;   // threads of the join (two CTAs an SM: the consumers)
-  // Two CTAs an SM are launched with 128 registers a thread, of which the producers hand most to the consumers.
-  static constexpr int kConsumerRegs = 216, kProducerRegs = 40;
-  static_assert(kPerSm == 1 || kConsumerRegs + kProducerRegs <= 2 * (65536 / (2 * kThreads)), "registers of a launch");
-  static constexpr int kMergeCols = D == 256 ? 64 : 32;   // columns that meet at a time at a job's end
+  static constexpr int kJoin = kPerSm == 1 ? 256 : 128;   // threads of the join (narrow, alone: the producers too)
+  // But for the narrow CTA alone, the producers hand most of a launch's registers to the consumers.
+  static constexpr bool kHandOver = kPerSm == 2 || kWide;
+  static constexpr int kConsumerRegs = kWide ? 232 : 216, kProducerRegs = 40;
+  static_assert(!kHandOver || (kWarps * kConsumerRegs + NP * kProducerRegs) * 32 <=
+                                  65536 / kPerSm / kThreads / 8 * 8 * kThreads, "registers of a launch");
+  static constexpr int kQueries = kWide ? MT * (D / 16 * 512 + 64) : 0;  // bytes: fragments and row factors
+  static constexpr int kMergeCols = D == 256 && !kWide ? 64 : 32;   // columns that meet at a time at a job's end
   static constexpr int kMergeRow = kMergeCols + 4;        // floats of a row in the merge buffer, padded
   static constexpr int kMerge = kWarps * 16 * (kMergeRow + 2) * 4;  // every warp's columns; maxima and sums
   static constexpr int kMaxNS = 24;
@@ -84,12 +93,13 @@ struct Cfg {
   // At least three a key group keep two tiles on their way while one is worked on (two: 15 % less of the bandwidth).
   // A multiple of the producers and of the key groups, so that a ring slot is always filled by one producer and read by
   // one group: barrier waits tell phases apart by parity alone, and two producers on one slot could be two turns apart.
-  static int fixed_bytes(int B) { return 2048 + kMerge + (3 * B + 1) * 4; }
+  static int fixed_bytes(int B) { return 2048 + kMerge + kQueries + (3 * B + 1) * 4; }
   static int slots(int B) {
     const int fit = ((kPerSm == 1 ? kSmemOne : kSmemTwo) - fixed_bytes(B)) / kSlot;
-    return (fit > kMaxNS ? kMaxNS : fit) / kWarps * kWarps;
+    constexpr int kMul = NG > NP ? NG : NP;
+    return (fit > kMaxNS ? kMaxNS : fit) / kMul * kMul;
   }
-  static_assert(kWarps % NP == 0, "a ring slot has one producer");
+  static_assert(NG >= 1 && (NG % NP == 0 || NP % NG == 0), "a ring slot has one producer and one group");
 };
 
 // D (16x8, fp32) += A (16x16) B (16x8); bf16 or f16 operands.
@@ -150,7 +160,10 @@ template <int kT>
 __device__ __forceinline__ void join_sync() {
   asm volatile("bar.sync 2, %0;" ::"n"(kT) : "memory");
 }
-__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
+template <int kT>
+__device__ __forceinline__ void consumers_bar() {
+  asm volatile("bar.sync 1, %0;" ::"n"(kT) : "memory");
+}
 
 // Whether one of the values in w (two bf16, or four e4m3) is NaN or infinite.
 template <bool F8>
@@ -185,7 +198,7 @@ enum { JOIN_PARTS = 0, JOIN_FIRST, JOIN_SECOND, JOIN_SLOT, JOIN_HEAD, JOIN_BLOCK
 // The share of one CTA: [u, end) of the flattened list, walked job by job. A job counts kSetup units of its own before
 // its units of keys: its queries, its first tile's latency and its merge cost a CTA about as much, and a batch with
 // many short sequences would otherwise pile them up in a few CTAs.
-constexpr int setup_units(int MT) { return MT == 1 ? 5 : (MT == 2 ? 9 : 16); }
+constexpr int setup_units(int unit_keys) { return unit_keys >= 64 ? 5 : 9; }
 template <int kSetup>
 struct Walk {
   int u, end;           // what is left of the share
@@ -335,11 +348,13 @@ __device__ void join_share(const PAttnArgs& a, const int (&jn)[JOIN_INTS], JoinS
 }
 
 template <int D, bool F8, int MT>
-__global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
+__global__ void __launch_bounds__(Cfg<D, F8, MT>::kThreads, Cfg<D, F8, MT>::kPerSm)
     paged_attn_kernel(const __grid_constant__ PAttnArgs a, const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v) {
-  using C = Cfg<D, F8>;
-  constexpr int NG = kWarps / MT, KT = C::KT, UK = NG * KT, NP = C::NP, kThreads = C::kThreads, kSetup = setup_units(MT);
+  using C = Cfg<D, F8, MT>;
+  constexpr int kWarps = C::kWarps, NG = C::NG, KT = C::KT, UK = NG * KT, NP = C::NP, kThreads = C::kThreads;
+  constexpr int kSetup = setup_units(UK);
+  auto consumers_sync = [] { consumers_bar<kWarps * 32>(); };
   const int NS = a.ns;
   constexpr int NT = D / 8;     // accumulator tiles of 8 columns
   constexpr int KC = C::kRow / 16;  // 16-byte chunks of a cached row
@@ -351,7 +366,9 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   float* merge = reinterpret_cast<float*>(ring + (size_t)NS * C::kSlot);
   float2* merge_ml = reinterpret_cast<float2*>(merge + kWarps * 16 * C::kMergeRow);
-  int* S = reinterpret_cast<int*>(merge_ml + kWarps * 16);
+  uint4* q_sm = reinterpret_cast<uint4*>(merge_ml + kWarps * 16);  // wide: [row tile][k step][lane], row factors behind
+  float* q_fac = reinterpret_cast<float*>(q_sm + MT * (D / 16) * 32);
+  int* S = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(q_sm) + C::kQueries);
   int* keys = S + a.B + 1;
   int* seqs = keys + a.B;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -394,7 +411,7 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
   w.end = min(total, w.u + per);
   if (warp >= kWarps) {
     // ---------------------------------------------------------------- producer
-    if constexpr (C::kPerSm == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kProducerRegs));
+    if constexpr (C::kHandOver) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kProducerRegs));
     const int none = a.num_pages * a.Hkv;  // a page that is not there: outside the map, reads as zero
     const int nbox = KT / a.box_rows;
     int i = 0;      // tiles so far: slot i % NS, for the turn-th time
@@ -472,7 +489,7 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
   }
 
   // ------------------------------------------------------------------ consumers
-  if constexpr (C::kPerSm == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kConsumerRegs));
+  if constexpr (C::kHandOver) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kConsumerRegs));
   // Off the others' way while the first tile travels: where the grid barrier stands (every launch adds one arrival a CTA,
   // so whatever is read before this CTA's own gives the launch's start), and the split job at the border before this CTA.
   if (tid == 32) {
@@ -525,53 +542,68 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
     auto q_row = [&](int r, int t) {
       return a.q + (((int64_t)w.b * a.Tq + t) * a.Hq + h * a.G + (r - t * a.G)) * D;
     };
-    uint32_t qf[D / 16][4];
     // scores in units of log 2 are S times fA or fB, kept above zero: a negative scale turns the queries' signs, and one
     // of zero is as good as the smallest factor
     float fA = a.scale * 1.4426950408889634f, fB;
     if (a.k_scale) fA *= a.k_scale[h];
     const uint32_t flip = fA < 0.f ? 0x80008000u : 0u;
     fA = fB = fmaxf(fabsf(fA), 1.1754944e-38f);
-    {
+    uint32_t qf[C::kWide ? 1 : D / 16][4];
+    auto load_queries = [&](uint32_t (&q)[D / 16][4]) {
       const uint16_t* pA = q_row(rA < M ? rA : 0, rA < M ? tA : 0);
       const uint16_t* pB = q_row(rB < M ? rB : 0, rB < M ? tB : 0);
       if constexpr (!F8) {
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
-          qf[c][0] = *reinterpret_cast<const uint32_t*>(pA + c * 16 + 2 * ql);
-          qf[c][1] = *reinterpret_cast<const uint32_t*>(pB + c * 16 + 2 * ql);
-          qf[c][2] = *reinterpret_cast<const uint32_t*>(pA + c * 16 + 8 + 2 * ql);
-          qf[c][3] = *reinterpret_cast<const uint32_t*>(pB + c * 16 + 8 + 2 * ql);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) qf[c][e] ^= flip;
+          q[c][0] = *reinterpret_cast<const uint32_t*>(pA + c * 16 + 2 * ql) ^ flip;
+          q[c][1] = *reinterpret_cast<const uint32_t*>(pB + c * 16 + 2 * ql) ^ flip;
+          q[c][2] = *reinterpret_cast<const uint32_t*>(pA + c * 16 + 8 + 2 * ql) ^ flip;
+          q[c][3] = *reinterpret_cast<const uint32_t*>(pB + c * 16 + 8 + 2 * ql) ^ flip;
         }
       } else {
         // e4m3 keys become f16, so the queries do too: scaled by the power of two that brings the row's largest into
         // [1, 2) (exact), what then falls below f16's range is under 2^-24 of it. A 16-byte chunk of a key is one
         // k-step here: lane ql holds its values 4 ql .. + 3, and the queries are laid out to match.
-        float mA = 0.f, mB = 0.f;
+        float xA = 0.f, xB = 0.f;
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
-          const uint2 xa = *reinterpret_cast<const uint2*>(pA + c * 16 + 4 * ql);
-          const uint2 xb = *reinterpret_cast<const uint2*>(pB + c * 16 + 4 * ql);
-          qf[c][0] = xa.x ^ flip; qf[c][2] = xa.y ^ flip; qf[c][1] = xb.x ^ flip; qf[c][3] = xb.y ^ flip;
-          mA = fmaxf(fmaxf(mA, fmaxf(fabsf(lo_bf(xa.x)), fabsf(hi_bf(xa.x)))), fmaxf(fabsf(lo_bf(xa.y)), fabsf(hi_bf(xa.y))));
-          mB = fmaxf(fmaxf(mB, fmaxf(fabsf(lo_bf(xb.x)), fabsf(hi_bf(xb.x)))), fmaxf(fabsf(lo_bf(xb.y)), fabsf(hi_bf(xb.y))));
+          const uint2 va = *reinterpret_cast<const uint2*>(pA + c * 16 + 4 * ql);
+          const uint2 vb = *reinterpret_cast<const uint2*>(pB + c * 16 + 4 * ql);
+          q[c][0] = va.x ^ flip; q[c][2] = va.y ^ flip; q[c][1] = vb.x ^ flip; q[c][3] = vb.y ^ flip;
+          xA = fmaxf(fmaxf(xA, fmaxf(fabsf(lo_bf(va.x)), fabsf(hi_bf(va.x)))), fmaxf(fabsf(lo_bf(va.y)), fabsf(hi_bf(va.y))));
+          xB = fmaxf(fmaxf(xB, fmaxf(fabsf(lo_bf(vb.x)), fabsf(hi_bf(vb.x)))), fmaxf(fabsf(lo_bf(vb.y)), fabsf(hi_bf(vb.y))));
         }
         // exponents in [1, 252], so that the factor and its inverse are normal numbers
-        const uint32_t eA = min(max(__float_as_uint(quad_max(mA)) >> 23, 1u), 252u);
-        const uint32_t eB = min(max(__float_as_uint(quad_max(mB)) >> 23, 1u), 252u);
+        const uint32_t eA = min(max(__float_as_uint(quad_max(xA)) >> 23, 1u), 252u);
+        const uint32_t eB = min(max(__float_as_uint(quad_max(xB)) >> 23, 1u), 252u);
         const float iA = __uint_as_float((254u - eA) << 23), iB = __uint_as_float((254u - eB) << 23);
         fA *= __uint_as_float(eA << 23);
         fB *= __uint_as_float(eB << 23);
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
-          qf[c][0] = pack2<true>(lo_bf(qf[c][0]) * iA, hi_bf(qf[c][0]) * iA);
-          qf[c][2] = pack2<true>(lo_bf(qf[c][2]) * iA, hi_bf(qf[c][2]) * iA);
-          qf[c][1] = pack2<true>(lo_bf(qf[c][1]) * iB, hi_bf(qf[c][1]) * iB);
-          qf[c][3] = pack2<true>(lo_bf(qf[c][3]) * iB, hi_bf(qf[c][3]) * iB);
+          q[c][0] = pack2<true>(lo_bf(q[c][0]) * iA, hi_bf(q[c][0]) * iA);
+          q[c][2] = pack2<true>(lo_bf(q[c][2]) * iA, hi_bf(q[c][2]) * iA);
+          q[c][1] = pack2<true>(lo_bf(q[c][1]) * iB, hi_bf(q[c][1]) * iB);
+          q[c][3] = pack2<true>(lo_bf(q[c][3]) * iB, hi_bf(q[c][3]) * iB);
         }
       }
+    };
+    if constexpr (!C::kWide) {
+      load_queries(qf);
+    } else {  // the first group's warps share theirs (all are behind the last job's use of the buffer: its merge)
+      if (g == 0) {
+        uint32_t q[D / 16][4];
+        load_queries(q);
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) q_sm[(mt * (D / 16) + c) * 32 + lane] = make_uint4(q[c][0], q[c][1], q[c][2], q[c][3]);
+        if (ql == 0) {
+          q_fac[mt * 16 + qr] = fA;
+          q_fac[mt * 16 + qr + 8] = fB;
+        }
+      }
+      consumers_sync();
+      fA = q_fac[mt * 16 + qr];
+      fB = q_fac[mt * 16 + qr + 8];
     }
     float acc[NT][4];
 #pragma unroll
@@ -607,18 +639,30 @@ __global__ void __launch_bounds__(Cfg<D, F8>::kThreads, Cfg<D, F8>::kPerSm)
         };
 #pragma unroll
         for (int c = 0; c < KC; c += 2) {
+          // the queries of k step k: in registers, or the row tile's in shared memory
+          auto query = [&](int k, uint32_t (&q)[4]) {
+            if constexpr (!C::kWide) {
+              q[0] = qf[k][0]; q[1] = qf[k][1]; q[2] = qf[k][2]; q[3] = qf[k][3];
+            } else {
+              const uint4 x = q_sm[(mt * (D / 16) + k) * 32 + lane];
+              q[0] = x.x; q[1] = x.y; q[2] = x.z; q[3] = x.w;
+            }
+          };
+          uint32_t qa[4], qb[4];
+          query(F8 ? c : c / 2, qa);
+          if constexpr (F8) query(c + 1, qb);
 #pragma unroll
           for (int j = 0; j < KT / 16; ++j) {
             uint32_t kf[4];
             ldsm4(kf, chunk_addr(kb, j, c));
             if constexpr (!F8) {
-              mma16816<false>((c / 2) & 1 ? other(2 * j) : s[2 * j], qf[c / 2], kf[0], kf[1]);
-              mma16816<false>((c / 2) & 1 ? other(2 * j + 1) : s[2 * j + 1], qf[c / 2], kf[2], kf[3]);
+              mma16816<false>((c / 2) & 1 ? other(2 * j) : s[2 * j], qa, kf[0], kf[1]);
+              mma16816<false>((c / 2) & 1 ? other(2 * j + 1) : s[2 * j + 1], qa, kf[2], kf[3]);
             } else {
-              mma16816<true>(s[2 * j], qf[c], e4m3x2_f16x2(kf[0]), e4m3x2_f16x2(kf[0] >> 16));
-              mma16816<true>(s[2 * j + 1], qf[c], e4m3x2_f16x2(kf[2]), e4m3x2_f16x2(kf[2] >> 16));
-              mma16816<true>(other(2 * j), qf[c + 1], e4m3x2_f16x2(kf[1]), e4m3x2_f16x2(kf[1] >> 16));
-              mma16816<true>(other(2 * j + 1), qf[c + 1], e4m3x2_f16x2(kf[3]), e4m3x2_f16x2(kf[3] >> 16));
+              mma16816<true>(s[2 * j], qa, e4m3x2_f16x2(kf[0]), e4m3x2_f16x2(kf[0] >> 16));
+              mma16816<true>(s[2 * j + 1], qa, e4m3x2_f16x2(kf[2]), e4m3x2_f16x2(kf[2] >> 16));
+              mma16816<true>(other(2 * j), qb, e4m3x2_f16x2(kf[1]), e4m3x2_f16x2(kf[1] >> 16));
+              mma16816<true>(other(2 * j + 1), qb, e4m3x2_f16x2(kf[3]), e4m3x2_f16x2(kf[3] >> 16));
             }
           }
         }
@@ -895,7 +939,7 @@ bool pool_map(CUtensorMap* m, const moe_paged_cache* c, const void* base, int bo
 
 template <int D, bool F8, int MT>
 cudaError_t launch_attn(const PAttnArgs& args, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t s) {
-  using C = Cfg<D, F8>;
+  using C = Cfg<D, F8, MT>;
   const void* fn = reinterpret_cast<const void*>(paged_attn_kernel<D, F8, MT>);
   static SmemGrant granted;
   PAttnArgs a = args;
@@ -962,7 +1006,7 @@ int moe_paged_attend(const moe_paged_cache* c, int layer, const int32_t* seqs, i
   a.inv_G = 1.f / (float)a.G;
   a.ctas = 0;
   // the flattened unit list is counted in 32 bits; a unit is at least 16 keys
-  const int64_t units = ((int64_t)c->max_pages * c->page + 15) / 16 + setup_units(4);
+  const int64_t units = ((int64_t)c->max_pages * c->page + 15) / 16 + setup_units(16);
   if (B * units * c->Hkv * a.row_blocks >= ((int64_t)1 << 31) - kPagedMaxCtas) return (int)cudaErrorInvalidValue;
   const int kt = tile_keys(c->D * kv_size(c->kv_type));
   a.box_rows = c->page % kt == 0 ? kt : 16;
