@@ -124,11 +124,11 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
 }
-// Two e4m3 values (the low 16 bits of w) as two f16, exactly.
-__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t w) {
-  uint32_t r;
-  asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(w));
-  return r;
+// Four e4m3 values as f16 pairs (bytes 0 and 1, 2 and 3), exactly.
+__device__ __forceinline__ void e4m3x4_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -659,10 +659,13 @@ __global__ void __launch_bounds__(Cfg<D, F8, MT>::kThreads, Cfg<D, F8, MT>::kPer
               mma16816<false>((c / 2) & 1 ? other(2 * j) : s[2 * j], qa, kf[0], kf[1]);
               mma16816<false>((c / 2) & 1 ? other(2 * j + 1) : s[2 * j + 1], qa, kf[2], kf[3]);
             } else {
-              mma16816<true>(s[2 * j], qa, e4m3x2_f16x2(kf[0]), e4m3x2_f16x2(kf[0] >> 16));
-              mma16816<true>(s[2 * j + 1], qa, e4m3x2_f16x2(kf[2]), e4m3x2_f16x2(kf[2] >> 16));
-              mma16816<true>(other(2 * j), qb, e4m3x2_f16x2(kf[1]), e4m3x2_f16x2(kf[1] >> 16));
-              mma16816<true>(other(2 * j + 1), qb, e4m3x2_f16x2(kf[3]), e4m3x2_f16x2(kf[3] >> 16));
+              uint32_t b[4][2];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) e4m3x4_f16(kf[e], b[e][0], b[e][1]);
+              mma16816<true>(s[2 * j], qa, b[0][0], b[0][1]);
+              mma16816<true>(s[2 * j + 1], qa, b[2][0], b[2][1]);
+              mma16816<true>(other(2 * j), qb, b[1][0], b[1][1]);
+              mma16816<true>(other(2 * j + 1), qb, b[3][0], b[3][1]);
             }
           }
         }
@@ -734,9 +737,11 @@ __global__ void __launch_bounds__(Cfg<D, F8, MT>::kThreads, Cfg<D, F8, MT>::kPer
                 // a 16-bit unit holds two columns of one key: even columns to one MMA, odd ones to the next
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                  const uint32_t b0 = __byte_perm(vf[2 * e], 0, 0x3120), b1 = __byte_perm(vf[2 * e + 1], 0, 0x3120);
-                  add(acc[2 * (c + e)], pf[ks], e4m3x2_f16x2(b0), e4m3x2_f16x2(b1));
-                  add(acc[2 * (c + e) + 1], pf[ks], e4m3x2_f16x2(b0 >> 16), e4m3x2_f16x2(b1 >> 16));
+                  uint32_t even0, odd0, even1, odd1;  // keys 0-7 and 8-15
+                  e4m3x4_f16(__byte_perm(vf[2 * e], 0, 0x3120), even0, odd0);
+                  e4m3x4_f16(__byte_perm(vf[2 * e + 1], 0, 0x3120), even1, odd1);
+                  add(acc[2 * (c + e)], pf[ks], even0, even1);
+                  add(acc[2 * (c + e) + 1], pf[ks], odd0, odd1);
                 }
               }
             }
