@@ -46,8 +46,9 @@ typedef struct moe_paged_cache {
   int32_t layers, num_pages, page, Hkv, D, kv_type, max_seqs, max_pages;
 } moe_paged_cache;
 
-/* Bits of the paged workspace's error word (moe_paged_workspace_error). MOE_ERR_TIMEOUT (include/moe_block.h) is set
- * too when a bounded wait of the attention kernel gave up; that call's output is then invalid. */
+/* Bits of the paged workspace's error word (moe_paged_workspace_error). MOE_ERR_TIMEOUT or MOE_ERR_BARRIER
+ * (include/moe_block.h) is set too when a bounded wait of the attention kernel gave up; that call's output is then
+ * invalid. */
 enum {
   MOE_ERR_PAGE_ID = 1 << 8,   /* a page id outside [0, num_pages): its keys read as zero, its rows are not written */
   MOE_ERR_SEQ_ID = 1 << 9,    /* a list entry outside [0, max_seqs) (-1 marks an unused slot where a call says so), a
@@ -79,8 +80,9 @@ MOE_API int moe_paged_workspace_error(void* workspace, size_t workspace_bytes, m
 /* Sets the length of each of the n listed sequences (distinct): shrinking releases the pages behind the new end (0
  * releases all of them), growing takes free pages, and a partly filled page at the end of what stays that other
  * sequences hold too is replaced by a copy of its filled rows, in every layer, in a page of its own (of k listed
- * sequences that end in one page, all its holders but the last in list order copy). Pages released by a call can be
- * taken by the same call. seqs, new_lens: device int32 [n]. n <= 2048 and at most the workspace's max_batch. */
+ * sequences that end in one page, all its holders but the last in list order copy). That copy takes a free page, of a
+ * sequence that shrinks too; releasing a whole sequence never does. Pages released by a call can be taken by the same
+ * call. seqs, new_lens: device int32 [n]. n <= 2048 and at most the workspace's max_batch. */
 MOE_API int moe_paged_resize(const moe_paged_cache* c, const int32_t* seqs, const int32_t* new_lens, int n,
                              void* workspace, size_t workspace_bytes, moe_stream_t stream);
 

@@ -44,7 +44,8 @@ MOE_API size_t moe_spec_workspace_bytes(int max_B, int V);
  *   with sum_{j <= v} w_j > u[b][K] sum_j w_j. Where w is zero everywhere, w = p_a.
  * tokens int32 [B][K + 1] = the a accepted tokens, the drawn one, then -1; accepted int32 [B] = a. Products and sums
  * are in fp64. Entries of p and q that are NaN, negative or infinite count as zero; a draft outside [0, V) is rejected;
- * if no entry of p_a is positive, the drawn token is -1. K >= 1 (up to 64), B <= max_B of the workspace. */
+ * if no entry of p_a is positive, the drawn token is -1. K up to 64, B <= max_B of the workspace. K = 0 (drafted NULL)
+ * draws one token a sequence from its probabilities. */
 MOE_API int moe_spec_verify(const float* target, int64_t ld_target, const float* draft, int64_t ld_draft,
                             const int32_t* drafted, const int32_t* n_drafted, const float* u, int B, int K, int V,
                             int32_t* tokens, int32_t* accepted, void* workspace, size_t workspace_bytes,

@@ -51,12 +51,13 @@ def _dense(t, dtype, n, dev):
 
 
 class SpecVerifier:
-    """Verification of up to K drafted tokens for up to max_B sequences over V tokens; owns the call's workspace."""
+    """Verification of up to K drafted tokens for up to max_B sequences over V tokens; owns the call's workspace. With
+    K = 0 it draws one token a sequence (draft and drafted are None then)."""
 
     def __init__(self, max_B, K, V, device="cuda"):
         self.max_B, self.K, self.V = max_B, K, V
         n = _lib.moe_spec_workspace_bytes(max_B, V)
-        if n == 0 or not 1 <= K <= 64:
+        if n == 0 or not 0 <= K <= 64:
             raise ValueError("unsupported sizes for the verification of drafts")
         self.ws = torch.zeros(n, dtype=torch.uint8, device=device)
         self.device, self._dev = self.ws.device, self.ws.get_device()
@@ -73,9 +74,9 @@ class SpecVerifier:
             raise ValueError(f"target {tuple(target.shape)}: the verifier takes up to {self.max_B} x {K + 1} x {self.V}")
         ldp = self._rows(target, "target", B, K1)
         ldq, q = 0, None
-        if draft is not None:
+        if draft is not None and K:
             ldq, q = self._rows(draft, "draft", B, K), draft.data_ptr()
-        if not (_dense(drafted, _I32, B * K, dev) and _dense(u, _F32, B * K1, dev) and _dense(tokens, _I32, B * K1, dev)
+        if not ((_dense(drafted, _I32, B * K, dev) if K else drafted is None) and _dense(u, _F32, B * K1, dev) and _dense(tokens, _I32, B * K1, dev)
                 and _dense(accepted, _I32, B, dev)):
             raise ValueError(f"expected contiguous drafted int32 ({B}, {K}), u float32 ({B}, {K1}), tokens int32 "
                              f"({B}, {K1}) and accepted int32 ({B},) on {self.device}")
@@ -83,7 +84,7 @@ class SpecVerifier:
         if n_drafted is not None:
             _need(_dense(n_drafted, _I32, B, dev), f"n_drafted: expected contiguous int32 ({B},) on {self.device}")
             n = n_drafted.data_ptr()
-        rc = _lib.moe_spec_verify(target.data_ptr(), ldp, q, ldq, drafted.data_ptr(), n, u.data_ptr(), B, K, V,
+        rc = _lib.moe_spec_verify(target.data_ptr(), ldp, q, ldq, drafted.data_ptr() if K else None, n, u.data_ptr(), B, K, V,
                                   tokens.data_ptr(), accepted.data_ptr(), *self._ws, raw_stream(dev, stream))
         if rc:
             _check(rc, "moe_spec_verify")

@@ -187,17 +187,67 @@ class DecodeStack:
         self.head.argmax(self.normed[T - 1], self.next, logits=logits, stream=stream)
 
 
+def paged_steps(stk, batch, length, new, steps, temperature=0.0, seed=7):
+    """`steps` steps of `batch` sequences of `length` cached tokens over a paged cache (mvcc_b200.paged), a token of each
+    sequence drawn from the step's probabilities at `temperature` (0: the likeliest one; mvcc_b200.spec). With new > 1
+    each step takes `new` - 1 drafted tokens a sequence too, here random ones, which are verified and rolled back to what
+    was accepted. Yields (tokens [batch, new], accepted [batch]) on the host after each step; the residuals fed in are
+    seeded random rows (there is no embedding table here)."""
+    from .paged import PagedDecodeStack
+    from .spec import SpecVerifier, softmax_rows
+    dev, H, V, page, K = stk.final_norm.device, stk.attn_shape.H, stk.V, 64, new - 1
+    pages = -(-(length + steps * new) // page)
+    ps = PagedDecodeStack(stk, num_pages=batch * pages, page=page, max_seqs=batch, max_pages=pages, max_batch=batch,
+                          max_new=new)
+    g = torch.Generator(device=dev).manual_seed(seed)
+    for t in (ps.cache.k, ps.cache.v):  # as if `length` tokens had been decoded
+        t.copy_(_normal_bf16(tuple(t.shape), g, 1.0, device=dev))
+    seqs = torch.arange(batch, dtype=torch.int32, device=dev)
+    lens = torch.full((batch,), length, dtype=torch.int32, device=dev)
+    ps.cache.resize(seqs, lens)
+    T = batch * new
+    probs, tokens = torch.empty(batch, new, V, device=dev), torch.empty(batch, new, dtype=torch.int32, device=dev)
+    accepted, temps = torch.empty(batch, dtype=torch.int32, device=dev), torch.full((T,), temperature, device=dev)
+    ver = SpecVerifier(batch, K, V, device=dev)
+    for _ in range(steps):
+        lens = lens + new
+        ps.cache.resize(seqs, lens)
+        ps.step(torch.randn(T, H, generator=g, device=dev), seqs, Tq=new, logits=probs)
+        softmax_rows(probs.view(T, V), probs.view(T, V), temperature=temps)
+        drafted = torch.randint(V, (batch, K), generator=g, device=dev).to(torch.int32) if K else None
+        ver.verify(probs, None, drafted, torch.rand(batch, new, generator=g, device=dev), tokens, accepted)
+        if K:
+            lens = lens - K + accepted
+            ps.cache.resize(seqs, lens)
+        err = ps.error_words()
+        if err:
+            raise RuntimeError(f"paged step: error word {err:#x}")
+        yield tokens.cpu(), accepted.cpu()
+
+
 def main(argv=None):
     """`python -m mvcc_b200.stack [--steps N] [--layers L]`: N plain decode steps (no CUDA graph) of BASELINE config 3
     on cuda:0 -- seeded synthetic weights and a 4096-token cache, each step at position 4095 from the same residual --
-    printing the next token of each. Used to capture the step's kernel launch list with a profiler."""
+    printing the next token of each. Used to capture the step's kernel launch list with a profiler. With `--batch B` the
+    steps run over a paged cache, B sequences at once; `--draft K` adds K drafted tokens a sequence, verified each step."""
     import argparse
     ap = argparse.ArgumentParser(prog="python -m mvcc_b200.stack")
     ap.add_argument("--steps", type=int, default=3)
     ap.add_argument("--layers", type=int, default=40)
+    ap.add_argument("--batch", type=int, default=0, help="sequences of a paged step (0: the single-sequence stack)")
+    ap.add_argument("--draft", type=int, default=0, help="drafted tokens a sequence, up to 7 (with --batch)")
     args = ap.parse_args(argv)
+    if args.batch < 0 or not 0 <= args.draft <= 7 or (args.draft and not args.batch):
+        ap.error("--draft needs --batch and takes 0 to 7")
     s = torch.cuda.Stream()
-    stk = DecodeStack(L=args.layers, ctx=4096, vocab=151936, seed=5)
+    # a paged run keeps its keys and values elsewhere
+    stk = DecodeStack(L=args.layers, ctx=64 if args.batch else 4096, vocab=151936, seed=5)
+    if args.batch:
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            for tok, acc in paged_steps(stk, args.batch, 4095, 1 + args.draft, args.steps):
+                print("tokens", tok.tolist(), "accepted", acc.tolist(), flush=True)
+        return
     h0, _ = synth_activations(stk.moe_shape, 1, seed=41, stream=s)
     h = h0.clone()
     torch.cuda.synchronize()

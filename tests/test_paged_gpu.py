@@ -723,3 +723,138 @@ def test_drafts_are_verified_and_rolled_back():
         lens = kept
     assert K in seen and 0 in seen
     assert int(ps.cache.refs.sum()) == sum(-(-int(n) // 16) for n in lens)
+
+
+def test_the_stack_command_decodes_a_batch_with_and_without_drafts():
+    from mvcc_b200 import stack
+    st = small_stack(L=2, vocab=700)
+    for new in (1, 3):
+        got = list(stack.paged_steps(st, batch=3, length=130, new=new, steps=3))
+        again = list(stack.paged_steps(st, batch=3, length=130, new=new, steps=3))
+        assert len(got) == 3
+        for (tok, acc), (tok2, acc2) in zip(got, again):
+            assert torch.equal(tok, tok2) and torch.equal(acc, acc2)  # the same inputs give the same tokens
+            for b in range(3):
+                a = int(acc[b])
+                assert 0 <= a < new and bool((tok[b, :a + 1] >= 0).all()) and bool((tok[b, a + 1:] == -1).all())
+                assert int(tok[b].max()) < 700
+
+
+# ------------------------------------------------------------------ several at once, far offsets, the largest lists
+
+def test_two_caches_on_two_streams_at_once():
+    """Calls of two caches (different heads, so different grids) overlap on two streams; each gives what it gives alone."""
+    a = filled([3000, 17, 900], Tq=2, Hq=8, Hkv=2, D=256, page=32, seed=1)
+    b = filled([5000, 1200, 64, 1], Hq=8, Hkv=4, D=128, page=16, seed=2)
+    qa, qb = queries(a, 3, 2), queries(b, 4, 1)
+    sa, sb = i32([0, 1, 2]), i32([3, 0, 2, 1])
+    wa, wb = torch.zeros_like(qa), torch.zeros_like(qb)
+    a.attend(0, sa, qa, wa, Tq=2)
+    b.attend(0, sb, qb, wb)
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    outs_a, outs_b = [torch.zeros_like(qa) for _ in range(30)], [torch.zeros_like(qb) for _ in range(30)]
+    torch.cuda.synchronize()
+    for x, y in zip(outs_a, outs_b):
+        a.attend(0, sa, qa, x, Tq=2, stream=s1)
+        b.attend(0, sb, qb, y, stream=s2)
+    torch.cuda.synchronize()
+    assert a.error_word() == 0 and b.error_word() == 0
+    assert all(torch.equal(x, wa) for x in outs_a) and all(torch.equal(y, wb) for y in outs_b)
+
+
+def test_two_graphs_of_one_stream_share_a_workspace():
+    c = filled([700, 90, 33], Tq=4, Hq=16, Hkv=2, D=256, page=64)
+    q1, q4 = queries(c, 3, 1), queries(c, 3, 4, seed=6)
+    o1, o4 = torch.zeros_like(q1), torch.zeros_like(q4)
+    seqs = i32([2, 0, 1])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        c.attend(0, seqs, q1, o1)
+        c.attend(0, seqs, q4, o4, Tq=4)
+        s.synchronize()
+        w1, w4 = o1.clone(), o4.clone()
+        g1, g4 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g1, stream=s):
+            c.attend(0, seqs, q1, o1)
+        with torch.cuda.graph(g4, stream=s):
+            c.attend(0, seqs, q4, o4, Tq=4)
+        for _ in range(5):
+            o1.zero_()
+            o4.zero_()
+            g1.replay()
+            g4.replay()
+            g4.replay()
+            g1.replay()
+            s.synchronize()
+            assert torch.equal(o1, w1) and torch.equal(o4, w4)
+        assert c.error_word(s) == 0
+
+
+def test_offsets_past_32_bits():
+    """A layer of 2.6 GB pools: pages whose byte offsets pass 2^31 and, in the second layer, 2^32."""
+    Hkv, D, page, pages = 2, 256, 64, 40000
+    c = P().PagedCache.empty(2, pages, page, Hkv, D, 8, 3, 3, 4, 2)
+    free = list(range(pages - 1, pages - 4, -1)) + [pages // 2, pages - 7]
+    lens = [130, 65]
+    for s, n in enumerate(lens):
+        for j in range(-(-n // page)):
+            p = free.pop(0)
+            c.tables[s, j], c.refs[p] = p, 1
+    c.lens[:2] = i32(lens)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    for s, n in enumerate(lens):
+        for p in c.tables[s][c.tables[s] >= 0].tolist():
+            for t in (c.k, c.v):
+                t[1, p] = bits(torch.randn(Hkv, page, D, generator=g, device="cuda"))
+    qkv = bits(torch.randn(2, 12 * D, generator=g, device="cuda"))
+    q = torch.zeros(2, 8 * D, dtype=torch.int16, device="cuda")
+    c.append(1, i32([0, 1]), qkv, q)
+    for s, n in enumerate(lens):
+        pid = int(c.tables[s, (n - 1) // page])
+        assert torch.equal(c.v[1, pid, :, (n - 1) % page], qkv[s].view(12, D)[10:])
+    check_attend(c, [1, 0], 2, layer=1)
+    src, dst = [int(c.tables[0, 0]), int(c.tables[1, 0])], [pages - 10, 3]
+    want = c.k[:, src].clone()
+    c.copy_pages(i32(src), i32(dst))
+    assert torch.equal(c.k[:, dst], want)
+    before = c.k[1, c.tables[0, :3].long()].clone()
+    c.compact()
+    assert c.error_word() == 0 and sorted(c.tables[:2].flatten().tolist()) == [-1, 0, 1, 2, 3, 4]
+    assert torch.equal(c.k[1, c.tables[0, :3].long()], before)
+
+
+def test_a_batch_of_the_largest_size_over_one_shared_prompt():
+    """2048 slots of 2048 sequences that share one prompt's pages, each with a token of its own."""
+    c = make(layers=1, pages=2100, page=16, Hkv=1, D=128, max_seqs=2048, max_pages=8, Hq=2, max_batch=2048)
+    c.resize(i32([0]), i32([100]))
+    rest = list(range(1, 2048))
+    c.fork(i32([0] * 2047), i32(rest))
+    allseq = i32(list(range(2048)))
+    c.resize(allseq, i32([101] * 2048))
+    assert c.error_word() == 0 and c.refs.max() == 2048
+    qkv = bits(torch.randn(2048, 4 * 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)))
+    q, out = torch.zeros(2048, 256, dtype=torch.int16, device="cuda"), torch.zeros(2048, 256, dtype=torch.int16, device="cuda")
+    c.append(0, allseq, qkv, q)
+    c.attend(0, allseq, q, out)
+    assert c.error_word() == 0
+    pick = [0, 1, 7, 1000, 2047]
+    want, tol = attend64(c, 0, pick, q[pick].contiguous(), 1, 128 ** -0.5, "bf16")
+    assert bool(((vals(out[pick]) - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("kv,D,Hkv,G,Tq", [("bf16", 256, 1, 8, 8), ("e4m3", 256, 2, 16, 2), ("bf16", 64, 2, 1, 7),
+                                          ("bf16", 128, 1, 128, 8), ("e4m3", 128, 4, 2, 8), ("bf16", 256, 2, 3, 1)])
+def test_attention_of_random_batches(kv, D, Hkv, G, Tq):
+    r = random.Random(D + G)
+    for seed in range(4):
+        lens = [max(0, int(r.expovariate(1 / 150))) if r.random() < 0.9 else r.randint(500, 2500)
+                for _ in range(r.randint(1, 14))]
+        kw = {} if kv == "bf16" else dict(k_scale=torch.full((1, Hkv), 0.02, device="cuda"),
+                                          v_scale=torch.full((1, Hkv), 0.03, device="cuda"))
+        c = filled(lens, Tq=Tq, Hq=G * Hkv, Hkv=Hkv, D=D, page=r.choice((16, 32, 48, 64, 128, 1024)), kv=kv, seed=seed,
+                   max_batch=20, **kw)
+        seqs = list(range(len(lens))) + [-1] * r.randint(0, 2)
+        r.shuffle(seqs)
+        check_attend(c, seqs, Tq, kv)

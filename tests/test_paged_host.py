@@ -121,8 +121,8 @@ def test_spec_calls_refuse_before_launch():
 
     def verify(t=PTR, ldt=100, d=PTR, ldd=100, x=PTR, u=PTR, B=4, K=3, V=100, tok=PTR, acc=PTR, ws=PTR, n=big):
         return L.moe_spec_verify(t, ldt, d, ldd, x, None, u, B, K, V, tok, acc, ws, n, None)
-    assert verify(B=0) == 0
-    for kw in ({"t": None}, {"ldt": 99}, {"ldd": 99}, {"x": None}, {"u": None}, {"B": -1}, {"B": 65536}, {"K": 0},
+    assert verify(B=0) == 0 and verify(K=0, d=None, x=None, tok=None) == BAD
+    for kw in ({"t": None}, {"ldt": 99}, {"ldd": 99}, {"x": None}, {"u": None}, {"B": -1}, {"B": 65536}, {"K": -1},
                {"K": 65}, {"V": 0}, {"tok": None}, {"acc": None}, {"ws": None}, {"ws": PTR + 4}, {"n": 256}):
         assert verify(**kw) == BAD, kw
     for args in ((None, PTR, 100, 64, 1, PTR), (PTR, None, 100, 64, 1, PTR), (PTR, PTR, 0, 64, 1, PTR),
@@ -138,3 +138,10 @@ def test_refused_calls_count_no_launch():
     test_attention_calls_refuse_before_launch()
     test_spec_calls_refuse_before_launch()
     assert m.stats()["launches"] == 0
+
+
+@pytest.mark.parametrize("argv", [["--draft", "2"], ["--batch", "2", "--draft", "8"], ["--batch", "-1"]])
+def test_stack_command_refuses_its_arguments(argv):
+    from mvcc_b200 import stack
+    with pytest.raises(SystemExit):
+        stack.main(argv)

@@ -277,3 +277,48 @@ def test_verify_of_rows_apart_on_another_stream_and_in_a_graph():
                 lambda: ver.verify(p.repeat(2, 1, 1), q, x, u, tt, aa), lambda: ver.verify(p, q, x, u, tt[:, :2], aa)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_softmax_of_many_short_rows_and_two_streams_of_long_ones():
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = 3 * torch.randn(70000, 9, generator=g, device="cuda")
+    out = torch.empty_like(x)
+    S().softmax_rows(x, out)
+    want = torch.softmax(x.double(), -1)
+    assert float((out.double() - want).abs().max()) <= 2.0 ** -19
+    a, b = torch.randn(40, 100000, generator=g, device="cuda"), torch.randn(30, 151936, generator=g, device="cuda")
+    oa, ob = torch.empty_like(a), torch.empty_like(b)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(10):
+        S().softmax_rows(a, oa, stream=s1)
+        S().softmax_rows(b, ob, stream=s2)
+    torch.cuda.synchronize()
+    near(oa, a, torch.ones(40, device="cuda"))
+    near(ob, b, torch.ones(30, device="cuda"))
+
+
+def test_one_verifier_serves_batches_of_every_size_in_turn():
+    K, V = 3, 4000
+    ver = S().SpecVerifier(70, K, V)
+    for B in (1, 70, 2, 33, 70, 1):
+        p, q, x, u = drafts(B, K, V, seed=B)
+        compare(p, q, x, u, ver=ver, least=0.0)
+
+
+@pytest.mark.parametrize("B,V", [(1, 1), (7, 5), (64, 4096), (5, 151936)])
+def test_a_token_is_drawn_without_drafts(B, V):
+    """K = 0: one draw a sequence, by the running sum; at temperature 0 the likeliest token."""
+    g = torch.Generator(device="cuda").manual_seed(B)
+    z = 3 * torch.randn(B, V, generator=g, device="cuda")
+    p, u = torch.empty_like(z), torch.rand(B, 1, generator=g, device="cuda")
+    ver = S().SpecVerifier(B, 0, V)
+    tok, acc = torch.zeros(B, 1, dtype=torch.int32, device="cuda"), torch.full((B,), 9, dtype=torch.int32, device="cuda")
+    for t in (0.8, 0.0):
+        S().softmax_rows(z, p, temperature=torch.full((B,), t, device="cuda"))
+        ver.verify(p.view(B, 1, V), None, None, u, tok, acc)
+        want, _, gap = verify64(p.view(B, 1, V).double().cpu().numpy(), None, None, u.double().cpu().numpy(), None)
+        safe = gap > 1e-13 if t else np.ones(B, bool)
+        assert np.array_equal(tok.cpu().numpy()[safe], want[safe]) and not bool(acc.any())
+        if t == 0:
+            assert tok[:, 0].tolist() == z.argmax(-1).tolist()
