@@ -5,7 +5,7 @@
 //                        copy brings the next row's share into shared memory while this row's, in registers, is
 //                        reduced and stored. The CTAs' (maximum, sum of 2^((x - max) c)) pairs meet through distributed
 //                        shared memory behind one cluster barrier a row, and each CTA rescales what it holds. Two CTAs
-//                        an SM: one's barriers hide behind the other's stores (192 rows of 151936: 51 us; one CTA an SM
+//                        an SM: one's barriers hide behind the other's stores (192 rows of 151936: 50 us; one CTA an SM
 //                        with two buffers 60 us; a CTA per row share without the walk 95 us). Bound by the row's bytes,
 //                        8 V.
 //   verify_kernel        CTA (chunk, sequence): which drafts are accepted (a few gathered values, found by every warp
@@ -67,15 +67,19 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// 2^((v - m) c), one at the maximum itself (infinite ones included), zero for a NaN.
-__device__ __forceinline__ float soft_weight(float v, float m, float c) {
-  const float e = ex2((v - m) * c);
-  return v == m ? 1.f : (e == e ? e : 0.f);
+// 2^((v - m) c) for v <= m, neither a NaN. Where m or c is infinite the difference or the product may be no number: then
+// one at the maximum itself, zero below it.
+__device__ __forceinline__ float soft_weight(float v, float m, float c) { return ex2((v - m) * c); }
+__device__ __forceinline__ float soft_weight_any(float v, float m, float c) {
+  return v == m ? 1.f : ex2((v - m) * c);
 }
+__device__ __forceinline__ bool soft_plain(float m, float c) { return fabsf(m) < INFINITY && c < INFINITY; }
+// A NaN never wins: it counts as -infinity.
+__device__ __forceinline__ float soft_clean(float v) { return fmaxf(v, -INFINITY); }
 
 // VEC floats a load (4 when rows and length allow it), N loads a thread; N = 0 reads the row again in every pass.
 template <int VEC, int N>
-__global__ void __launch_bounds__(kSmThreads, N * VEC <= 40 ? 2 : 1) softmax_rows_kernel(
+__global__ void __launch_bounds__(kSmThreads, VEC == 4 ? 2 : 1) softmax_rows_kernel(
     const __grid_constant__ SoftmaxArgs a) {
   __shared__ float red[2][kSmWarps];
   __shared__ float peer[3][kSmMaxCluster];  // of each CTA of the row: maximum, sum, index of the maximum
@@ -91,7 +95,7 @@ __global__ void __launch_bounds__(kSmThreads, N * VEC <= 40 ? 2 : 1) softmax_row
   const float c = greedy ? 0.f : 1.4426950408889634f / t;
   const int chunk = ((a.V + CL - 1) / CL + 3) & ~3;
   const int b0 = min(a.V, rank * chunk), b1 = min(a.V, b0 + chunk);
-  auto weight = [&](float v, float m) { return soft_weight(v, m, c); };
+  auto weight = [&](float v, float m) { return soft_weight_any(v, m, c); };
 
   float r[N ? N * VEC : 1];
   float m = -INFINITY;
@@ -110,7 +114,10 @@ __global__ void __launch_bounds__(kSmThreads, N * VEC <= 40 ? 2 : 1) softmax_row
       }
     }
 #pragma unroll
-    for (int k = 0; k < N * VEC; ++k) m = fmaxf(m, r[k]);
+    for (int k = 0; k < N * VEC; ++k) {
+      r[k] = soft_clean(r[k]);
+      m = fmaxf(m, r[k]);
+    }
   } else {
     for (int i = b0 + tid; i < b1; i += kSmThreads) m = fmaxf(m, x[i]);
   }
@@ -127,13 +134,20 @@ __global__ void __launch_bounds__(kSmThreads, N * VEC <= 40 ? 2 : 1) softmax_row
   if (!greedy) {
     s = 0.f;
     if constexpr (N > 0) {
+      float z = m, cz = c;
+      if (!soft_plain(m, c)) {  // one at the maximum, zero below it (or everywhere): exponents 0 and -infinity
+#pragma unroll
+        for (int k = 0; k < N * VEC; ++k) r[k] = r[k] == m && m != -INFINITY ? 0.f : -INFINITY;
+        z = 0.f;
+        cz = 1.f;
+      }
 #pragma unroll
       for (int k = 0; k < N * VEC; ++k) {
-        r[k] = m == -INFINITY ? 0.f : weight(r[k], m);
+        r[k] = soft_weight(r[k], z, cz);
         s += r[k];
       }
     } else {
-      for (int i = b0 + tid; i < b1; i += kSmThreads) s += m == -INFINITY ? 0.f : weight(x[i], m);
+      for (int i = b0 + tid; i < b1; i += kSmThreads) s += m == -INFINITY ? 0.f : weight(soft_clean(x[i]), m);
     }
     s = warp_sum(s);
   } else {
@@ -180,7 +194,7 @@ __global__ void __launch_bounds__(kSmThreads, N * VEC <= 40 ? 2 : 1) softmax_row
         }
       }
     } else {
-      for (int i = b0 + tid; i < b1; i += kSmThreads) y[i] = f == 0.f ? 0.f : weight(x[i], m) * f;
+      for (int i = b0 + tid; i < b1; i += kSmThreads) y[i] = f == 0.f ? 0.f : weight(soft_clean(x[i]), m) * f;
     }
   } else {
     float best = (float)(1 << 24);
@@ -250,12 +264,11 @@ __global__ void __launch_bounds__(kSmThreads, N <= 10 ? 2 : 1) softmax_ring_kern
         r[k] = i < n ? sh[i] : -INFINITY;
       }
     }
-    if (!ok) {  // the copy never came: the row and those after it are no numbers, and say so
 #pragma unroll
-      for (int k = 0; k < N * 4; ++k) r[k] = __int_as_float(0x7fc00000);
+    for (int k = 0; k < N * 4; ++k) {
+      r[k] = soft_clean(r[k]);
+      m = fmaxf(m, r[k]);
     }
-#pragma unroll
-    for (int k = 0; k < N * 4; ++k) m = fmaxf(m, r[k]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) red[0][warp] = m;
@@ -270,14 +283,20 @@ __global__ void __launch_bounds__(kSmThreads, N <= 10 ? 2 : 1) softmax_ring_kern
     const float c = greedy ? 0.f : 1.4426950408889634f / t;
     float s;
     if (!greedy) {
-      const float z = m == -INFINITY ? 0.f : m;
-      s = 0.f;
+      float z = m, cz = c;
+      if (!soft_plain(m, c)) {  // one at the maximum, zero below it (or everywhere): exponents 0 and -infinity
+#pragma unroll
+        for (int k = 0; k < N * 4; ++k) r[k] = r[k] == m && m != -INFINITY ? 0.f : -INFINITY;
+        z = 0.f;
+        cz = 1.f;
+      }
+      float ss[2] = {0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < N * 4; ++k) {
-        r[k] = soft_weight(r[k], z, c);
-        s += r[k];
+        r[k] = soft_weight(r[k], z, cz);
+        ss[k & 1] += r[k];
       }
-      s = warp_sum(s);
+      s = warp_sum(ss[0] + ss[1]);
     } else {
       int at = 1 << 24;
 #pragma unroll
@@ -307,8 +326,8 @@ __global__ void __launch_bounds__(kSmThreads, N <= 10 ? 2 : 1) softmax_ring_kern
     if (!greedy) {
       float total = 0.f;
       for (int k = 0; k < CL; ++k)
-        if (pr[0][k] != -INFINITY) total += pr[1][k] * soft_weight(pr[0][k], M, c);
-      f = M == -INFINITY || m == -INFINITY ? 0.f : soft_weight(m, M, c) / total;
+        if (pr[0][k] != -INFINITY) total += pr[1][k] * soft_weight_any(pr[0][k], M, c);
+      f = M == -INFINITY || m == -INFINITY ? 0.f : soft_weight_any(m, M, c) / total;
     } else {
       for (int k = CL - 1; k >= 0; --k)
         if (pr[0][k] == M && M != -INFINITY) at = (int)pr[1][k] - b0;
@@ -316,7 +335,7 @@ __global__ void __launch_bounds__(kSmThreads, N <= 10 ? 2 : 1) softmax_ring_kern
       for (int k = 0; k < N * 4; ++k) r[k] = (k / VEC * kSmThreads + tid) * VEC + k % VEC == at ? 1.f : 0.f;
       f = 1.f;
     }
-    if (!ok) f = __int_as_float(0x7fc00000);
+    if (!ok) f = __int_as_float(0x7fc00000);  // the copy never came: the row and those after it are no numbers, and say so
 #pragma unroll
     for (int k = 0; k < N * 4 / VEC; ++k) {
       const int i = (k * kSmThreads + tid) * VEC;
