@@ -46,9 +46,8 @@ typedef struct moe_paged_cache {
   int32_t layers, num_pages, page, Hkv, D, kv_type, max_seqs, max_pages;
 } moe_paged_cache;
 
-/* Bits of the paged workspace's error word (moe_paged_workspace_error). MOE_ERR_TIMEOUT or MOE_ERR_BARRIER
- * (include/moe_block.h) is set too when a bounded wait of the attention kernel gave up; that call's output is then
- * invalid. */
+/* Bits of the paged workspace's error word (moe_paged_workspace_error). MOE_ERR_TIMEOUT (include/moe_block.h) is set
+ * too when a bounded wait of the attention kernel gave up; that call's output is then invalid. */
 enum {
   MOE_ERR_PAGE_ID = 1 << 8,   /* a page id outside [0, num_pages): its keys read as zero, its rows are not written */
   MOE_ERR_SEQ_ID = 1 << 9,    /* a list entry outside [0, max_seqs) (-1 marks an unused slot where a call says so), a

@@ -28,12 +28,11 @@ inline int paged_block_rows(int G, int Tq) {
 // Offsets (bytes) of the caller-owned workspace's sections, each 256-byte aligned. The error word leads; what the page
 // calls and the attention keep shares the space behind it, since one workspace serves one call at a time.
 struct PagedWs {
-  // arrivals at the attention's grid barrier, one counter for each size of grid: one CTA an SM, two
-  size_t err, gbar1, gbar2;
+  size_t err;
   // page calls: number of page copies, their (source, destination, rows) triples, the free-page list and the page map
   size_t ncopy, copies, list, map;
-  // attention: partial maxima and sums, partial accumulators
-  size_t ml, acc;
+  // attention: the split jobs at the borders of its CTAs, partial maxima and sums, partial accumulators
+  size_t joins, ml, acc;
   size_t total;
 };
 
@@ -41,7 +40,6 @@ inline PagedWs paged_ws(const moe_paged_cache* c, int Hq, int max_batch, int max
   PagedWs L;
   size_t o = 0;
   L.err = o;    o = ws_align(o + 4);
-  L.gbar1 = o;  L.gbar2 = o + 64;  o = ws_align(o + 128);
   const size_t base = o;
   L.ncopy = o;  o = ws_align(o + 4);
   L.copies = o; o = ws_align(o + 12 * (size_t)(c->num_pages > max_batch ? c->num_pages : max_batch));
@@ -50,6 +48,7 @@ inline PagedWs paged_ws(const moe_paged_cache* c, int Hq, int max_batch, int max
   const size_t pages_end = o;
   o = base;
   const int rows = paged_block_rows(Hq / c->Hkv, max_new < kPagedMaxNew ? max_new : kPagedMaxNew);
+  L.joins = o;  o = ws_align(o + 32 * (size_t)kPagedMaxCtas);
   L.ml = o;     o = ws_align(o + sizeof(float) * 2 * kPagedMaxCtas * 2 * (size_t)rows);
   L.acc = o;    o = ws_align(o + sizeof(float) * kPagedMaxCtas * 2 * (size_t)rows * c->D);
   L.total = o > pages_end ? o : pages_end;
@@ -79,9 +78,8 @@ inline int64_t paged_layer_bytes(const moe_paged_cache* c) {
 
 // Launch as a programmatic dependent of the stream's previous kernel: every kernel launched here waits for it
 // (griddepcontrol.wait, in every thread) before it touches memory.
-// `cooperative`: its CTAs wait for one another, so all of them have to be resident.
 inline cudaError_t paged_launch(const void* fn, dim3 grid, dim3 block, size_t smem, cudaStream_t s, void** args,
-                                int cluster = 1, bool cooperative = false) {
+                                int cluster = 1) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -94,12 +92,8 @@ inline cudaError_t paged_launch(const void* fn, dim3 grid, dim3 block, size_t sm
   attr[1].val.clusterDim.x = cluster;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
-  if (cooperative) {
-    attr[1].id = cudaLaunchAttributeCooperative;
-    attr[1].val.cooperative = 1;
-  }
   cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 || cooperative ? 2 : 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return launched(cudaLaunchKernelExC(&cfg, fn, args));
 }
 

@@ -4,25 +4,34 @@
 // o = sum_j softmax_j(scale q . k_j) v_j for the G = Hq / Hkv query heads and Tq new tokens that share a kv head: each
 // cached value is read once and used by G Tq rows, so up to 64 rows the call is bound by the cache's bytes.
 //
-// Work split: a unit is NG x KT keys of one (sequence, kv head, row block) job, and a job costs a few units more. Every CTA of a persistent grid counts
-// the batch's units itself (a scan over the lengths, which only the device knows) and takes an equal, contiguous share
-// of the flattened list, whatever the lengths: a long cache is split over many CTAs, many short ones share a CTA. A CTA
-// has partial results for its first and its last job at most; they go to the workspace as (max, sum, accumulator), and
-// behind a barrier over the grid each split job's parts are merged in CTA order, so the result does not depend on timing.
-// A job that lies in one CTA is finished there. A job of n parts holds n - 1 of the borders between CTAs: the CTA behind
-// each border takes an equal share of the job's rows. (The merge as a kernel of its own cost 3 us of host time and as
-// much between the kernels.)
+// Work split: a unit is NG x KT keys of one (sequence, kv head, row block) job, and a job costs a few units more. Every
+// CTA of a persistent grid counts the batch's units itself (a scan over the lengths, which only the device knows) and
+// takes an equal, contiguous share of the flattened list, whatever the lengths: a long cache is split over many CTAs,
+// many short ones share a CTA. A CTA has partial results for its first and its last job at most; they go to the workspace
+// as (max, sum, accumulator), and paged_join_kernel merges each split job's parts in CTA order, so the result does not
+// depend on timing. A job that lies in one CTA is finished there. A job of n parts holds n - 1 of the borders between
+// CTAs: the join runs a CTA a border, and those of one job share its rows. (Joined by the same launch behind a barrier
+// over the grid, a call took 3 us less of the host but 2 us more of the GPU: a cooperative launch does not overlap the
+// kernel before it.)
 //
 // CTA: four or eight consumer warps and four producer warps (a thread issues a TMA copy every 95 cycles or so: one an SM
-// fetches 3.2 TB/s over the GPU in 2 KB boxes, four 6.4 TB/s). Producer w takes every NP-th of the
-// CTA's tiles (KT keys of k and v each), reads the page ids 32 at a time and fetches the tiles by TMA (boxes of 64 values x 16 or KT rows inside one page, 128-byte
-// swizzle) into a ring of NS slots, mbarrier-counted. Consumer warp (g, mt) holds 16 query rows as MMA fragments and
-// takes every NG-th tile: S = Q K^T, the running maximum and sum of the softmax, O += P V, all in registers; at a job's
-// end the NG warps of a row tile merge through shared memory.
+// fetches 3.2 TB/s over the GPU in 2 KB boxes, four 6.4 TB/s). Producer w takes every NP-th of the CTA's tiles (KT keys of
+// k and v each), reads the page ids 32 at a time and fetches the tiles by TMA (boxes of 128 bytes x 16 or KT rows inside
+// one page, 128-byte swizzle) into a ring of NS slots, mbarrier-counted. Consumer warp (g, mt) holds 16 query rows as MMA
+// fragments and takes every NG-th tile: S = Q K^T, the running maximum and sum of the softmax, O += P V, all in
+// registers; at a job's end the NG warps of a row tile merge through shared memory.
 //
 // mma.sync and not tcgen05: with 16 to 64 rows a tcgen05.mma (at least 64 rows of the cache as M, and P through TMEM)
 // would leave its tensor core as idle as the register MMA does, and add two TMEM round trips to the softmax of each
 // tile; at 16 rows the register MMA needs under a third of the cycles that the tile's bytes take to arrive.
+//
+// Measured on a B200 (16 query and 2 kv heads of 256, bf16, unless said otherwise; the device copy moves 6.45 TB/s): one
+// sequence of 131071 keys 51 us (5.2 TB/s), 48 ragged sequences of up to 8192 keys 69 us (5.4 TB/s), with 4 and 8 new
+// tokens each 82 and 128 us; 24 sequences of up to 16000 keys, 32 over 8 heads of 128, 4 tokens: 123 us in bf16
+// (5.9 TB/s), 79 us in e4m3 with pages of 16 (4.6 TB/s). The loop over the tiles runs at the read bandwidth for bf16 and
+// one row tile; around it lie 2 us for the units, 1.5 us for the first queries and pages, 2 us for the last merge, 1 to
+// 4 us for the slowest CTA and 3 us for the join. With e4m3 or several row tiles the consumers' latency a tile (2000
+// cycles, two warps a scheduler) bounds it.
 #include <algorithm>
 #include <cstring>
 #include <mutex>
@@ -47,7 +56,7 @@ struct PAttnArgs {
   const int32_t* seqs;
   const int32_t* tables;
   const int32_t* lens;
-  unsigned long long* gbar;  // arrivals at the end of the work, over all launches
+  int32_t* joins;  // [ctas][JOIN_INTS]: the split job at the border before each CTA
   float* ml;       // [2 ctas][rows][2]
   float* acc;      // [2 ctas][rows][D]
   uint32_t* err;
@@ -78,7 +87,6 @@ struct Cfg {
   static constexpr int NG = kWarps / MT;                  // key groups
   static constexpr int NP = 4;                            // producer warps
   static constexpr int kThreads = (kWarps + NP) * 32;
-  static constexpr int kJoin = kPerSm == 1 ? 256 : 128;   // threads of the join (narrow, alone: the producers too)
   // But for the narrow CTA alone, the producers hand most of a launch's registers to the consumers.
   static constexpr bool kHandOver = kPerSm == 2 || kWide;
   static constexpr int kConsumerRegs = kWide ? 232 : 216, kProducerRegs = 40;
@@ -157,10 +165,6 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* mbar) {
   asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.shared::cta.b64 st, [%0];\n\t}" ::"r"(smem_u32(mbar)) : "memory");
 }
 template <int kT>
-__device__ __forceinline__ void join_sync() {
-  asm volatile("bar.sync 2, %0;" ::"n"(kT) : "memory");
-}
-template <int kT>
 __device__ __forceinline__ void consumers_bar() {
   asm volatile("bar.sync 1, %0;" ::"n"(kT) : "memory");
 }
@@ -193,7 +197,7 @@ __device__ __forceinline__ int slot_keys(const PAttnArgs& a, int b, int* seq) {
 
 // The split job at the border before a CTA: its parts (0: none), its first CTA, whether its part is that CTA's second,
 // slot, kv head and row block.
-enum { JOIN_PARTS = 0, JOIN_FIRST, JOIN_SECOND, JOIN_SLOT, JOIN_HEAD, JOIN_BLOCK, JOIN_INTS };
+enum { JOIN_PARTS = 0, JOIN_FIRST, JOIN_SECOND, JOIN_SLOT, JOIN_HEAD, JOIN_BLOCK, JOIN_INTS = 8 };
 
 // The share of one CTA: [u, end) of the flattened list, walked job by job. A job counts kSetup units of its own before
 // its units of keys: its queries, its first tile's latency and its merge cost a CTA about as much, and a batch with
@@ -231,122 +235,6 @@ struct Walk {
   }
 };
 
-// The join, by kT threads of CTA c, whose share begins inside a job of CTAs c0 .. c1: they take the
-// (c - c0 - 1)-th of c1 - c0 equal shares of the job's (row, four columns) items. An item's parts, one per CTA of the
-// job in order, are weighted by 2^(m_i - m) and added; a share of few items has its parts spread over the threads.
-struct JoinScratch {
-  static constexpr int kMaxRows = 64;
-  float4 red[256];
-  // weights of the share's rows: rows * parts <= (64 / (parts - 1) + 2) * parts
-  float wt[2 * kMaxRows + 2 * kPagedMaxCtas];
-  float inv[kMaxRows];
-};
-template <int D, int kT>
-__device__ void join_share(const PAttnArgs& a, const int (&jn)[JOIN_INTS], JoinScratch& js) {
-  constexpr int kCols = D / 4;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x;
-  const int parts = jn[JOIN_PARTS], c0 = jn[JOIN_FIRST], second = jn[JOIN_SECOND], b = jn[JOIN_SLOT], h = jn[JOIN_HEAD],
-            rb = jn[JOIN_BLOCK];
-  const int rows = min(a.rows, a.G * a.Tq - rb * a.rows), all = rows * kCols, share = c - c0 - 1;
-  const int i0 = all * share / (parts - 1), i1 = all * (share + 1) / (parts - 1);  // all <= 2^12, parts <= 320
-  if (i0 >= i1) return;
-  const int r0 = i0 / kCols, r1 = (i1 - 1) / kCols + 1;
-  auto part = [&](int i) { return (int64_t)(c0 + i) * 2 + (i == 0 ? second : 0); };
-  // Few items (many parts): the parts of an item over `slices` threads, a power of two up to 32. Many items (few parts):
-  // kItems items a thread at a time. Either way each thread's first kAhead values are on their way while the weights are
-  // found: eight parts of one item, or two of each of four.
-  constexpr int kAhead = 8, kItems = 4;
-  int lg = 0;
-  while (lg < 5 && (i1 - i0) << (lg + 1) <= kT) ++lg;
-  const int slices = 1 << lg, lanes = kT >> lg, sl = (tid << lg) / kT, mine = i0 + (tid & (lanes - 1));
-  auto load = [&](int it, int i) {
-    const int r = it / kCols, col = it % kCols;
-    return it < i1 && i < parts ? __ldcg(reinterpret_cast<const float4*>(a.acc + (part(i) * a.rows + r) * D + col * 4))
-                                : make_float4(0.f, 0.f, 0.f, 0.f);
-  };
-  auto weight = [&](int it, int i) { return it < i1 && i < parts ? js.wt[(it / kCols - r0) * parts + i] : 0.f; };
-  auto add = [](float4& s, const float4& x, float f) {
-    s.x = fmaf(x.x, f, s.x);
-    s.y = fmaf(x.y, f, s.y);
-    s.z = fmaf(x.z, f, s.z);
-    s.w = fmaf(x.w, f, s.w);
-  };
-  auto store = [&](int it, const float4& s) {
-    if (it >= i1) return;
-    const int r = it / kCols, col = it % kCols, q = rb * a.rows + r, t = token_of(a, q);
-    const float d = js.inv[r - r0];
-    *reinterpret_cast<uint2*>(a.out + (((int64_t)b * a.Tq + t) * a.Hq + h * a.G + (q - t * a.G)) * D + col * 4) =
-        make_uint2(pack2<false>(s.x * d, s.y * d), pack2<false>(s.z * d, s.w * d));
-  };
-  float4 ahead[kAhead];
-#pragma unroll
-  for (int k = 0; k < kAhead; ++k)
-    ahead[k] = slices > 1 ? load(mine, sl + k * slices) : load(mine + k % kItems * kT, k / kItems);
-  for (int r = r0 + warp; r < r1; r += kT / 32) {
-    constexpr int kHeld = 3;  // a lane's parts that stay in registers
-    float2 x[kHeld];
-    float m = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < kHeld; ++k) {
-      const int i = lane + 32 * k;
-      x[k] = i < parts ? __ldcg(reinterpret_cast<const float2*>(a.ml + (part(i) * a.rows + r) * 2))
-                       : make_float2(-INFINITY, 0.f);
-    }
-#pragma unroll
-    for (int k = 0; k < kHeld; ++k) m = fmaxf(m, x[k].x);
-    for (int i = lane + 32 * kHeld; i < parts; i += 32) m = fmaxf(m, __ldcg(a.ml + (part(i) * a.rows + r) * 2));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float z = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-#pragma unroll
-    for (int k = 0; k < kHeld; ++k) {
-      const int i = lane + 32 * k;
-      const float f = ex2(x[k].x - z);
-      if (i < parts) js.wt[(r - r0) * parts + i] = f;
-      l = fmaf(x[k].y, f, l);
-    }
-    for (int i = lane + 32 * kHeld; i < parts; i += 32) {
-      const float2 v = __ldcg(reinterpret_cast<const float2*>(a.ml + (part(i) * a.rows + r) * 2));
-      const float f = ex2(v.x - z);
-      js.wt[(r - r0) * parts + i] = f;
-      l = fmaf(v.y, f, l);
-    }
-    l = warp_sum(l);
-    if (lane == 0) js.inv[r - r0] = l == 0.f ? 0.f : (a.v_scale ? a.v_scale[h] : 1.f) / l;
-  }
-  join_sync<kT>();
-  if (slices > 1) {
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) add(s, ahead[k], weight(mine, sl + k * slices));
-#pragma unroll 4
-    for (int i = sl + kAhead * slices; i < parts; i += slices) add(s, load(mine, i), weight(mine, i));
-    js.red[tid] = s;
-    join_sync<kT>();
-    if (sl != 0) return;
-    for (int k = 1; k < slices; ++k) add(s, js.red[k * lanes + tid], 1.f);
-    store(mine, s);
-  } else {
-    for (int base = mine; base < i1; base += kItems * kT) {
-      float4 s[kItems];
-#pragma unroll
-      for (int k = 0; k < kItems; ++k) s[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int i = 0; i < parts; i += 2) {
-        if (i > 0 || base != mine) {
-#pragma unroll
-          for (int k = 0; k < kAhead; ++k) ahead[k] = load(base + k % kItems * kT, i + k / kItems);
-        }
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k)
-          add(s[k % kItems], ahead[k], weight(base + k % kItems * kT, i + k / kItems));
-      }
-#pragma unroll
-      for (int k = 0; k < kItems; ++k) store(base + k * kT, s[k]);
-    }
-  }
-}
-
 template <int D, bool F8, int MT>
 __global__ void __launch_bounds__(Cfg<D, F8, MT>::kThreads, Cfg<D, F8, MT>::kPerSm)
     paged_attn_kernel(const __grid_constant__ PAttnArgs a, const __grid_constant__ CUtensorMap map_k,
@@ -361,8 +249,6 @@ __global__ void __launch_bounds__(Cfg<D, F8, MT>::kThreads, Cfg<D, F8, MT>::kPer
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[C::kMaxNS], empty[C::kMaxNS];
   __shared__ int sm[32];
-  __shared__ int jn[JOIN_INTS], joined;
-  __shared__ unsigned long long gbar_base;
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   float* merge = reinterpret_cast<float*>(ring + (size_t)NS * C::kSlot);
   float2* merge_ml = reinterpret_cast<float2*>(merge + kWarps * 16 * C::kMergeRow);
@@ -481,38 +367,27 @@ __global__ void __launch_bounds__(Cfg<D, F8, MT>::kThreads, Cfg<D, F8, MT>::kPer
     if (!ok)  // no copy may still be landing when the CTA exits
       for (int j = max(0, i - NS); j < i; ++j)
         if (j % NP == warp - kWarps) bar_wait(&full[j % NS], (j / NS) & 1);
-    if (tid < C::kJoin) {  // producers that help with the join
-      join_sync<C::kJoin>();
-      if (jn[JOIN_PARTS] != 0 && joined) join_share<D, C::kJoin>(a, jn, *reinterpret_cast<JoinScratch*>(ring));
-    }
     return;
   }
 
   // ------------------------------------------------------------------ consumers
   if constexpr (C::kHandOver) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kConsumerRegs));
-  // Off the others' way while the first tile travels: where the grid barrier stands (every launch adds one arrival a CTA,
-  // so whatever is read before this CTA's own gives the launch's start), and the split job at the border before this CTA.
-  if (tid == 32) {
-    const unsigned long long v = ld_relaxed_u64(a.gbar);
-    gbar_base = v - v % gridDim.x;
-  }
+  // The split job at the border before this CTA, for the join; off the others' way while the first tile travels.
   if (tid == 64) {
-    int parts = 0;
+    int4 j0 = make_int4(0, 0, 0, 0);
     Walk<kSetup> at = w;
     if (at.u < at.end) {
       at.seek(S, a.B, HR);
       const int u0 = at.base + at.job * at.W + kSetup;  // the job's first unit of keys
       if (u0 < at.u) {
         const int c0 = u0 / per;
-        parts = (u0 - kSetup + at.W - 1) / per - c0 + 1;
-        jn[JOIN_FIRST] = c0;
-        jn[JOIN_SECOND] = u0 - kSetup > c0 * per;  // another job's units lie before it in that CTA
-        jn[JOIN_SLOT] = at.b;
-        jn[JOIN_HEAD] = at.job / a.row_blocks;
-        jn[JOIN_BLOCK] = at.job % a.row_blocks;
+        // its part in CTA c0 is that CTA's second if another job's units lie before it there
+        j0 = make_int4((u0 - kSetup + at.W - 1) / per - c0 + 1, c0, u0 - kSetup > c0 * per, at.b);
+        *reinterpret_cast<int2*>(a.joins + blockIdx.x * JOIN_INTS + 4) =
+            make_int2(at.job / a.row_blocks, at.job % a.row_blocks);
       }
     }
-    jn[JOIN_PARTS] = parts;
+    *reinterpret_cast<int4*>(a.joins + blockIdx.x * JOIN_INTS) = j0;
   }
 
   const int g = warp / MT, mt = warp % MT, qr = lane >> 2, ql = lane & 3;
@@ -888,24 +763,124 @@ __global__ void __launch_bounds__(Cfg<D, F8, MT>::kThreads, Cfg<D, F8, MT>::kPer
       const int t = k < slot ? turn : turn - 1;  // the slot's last turn
       if (t >= 0) bar_wait(&full[k], t & 1);
     }
-  // The split jobs. Every CTA arrives once its parts are written; one whose share began inside a job waits for all (the
-  // launch is cooperative, so all are resident) and takes its share of that job's join. The ring is free by now.
-  consumers_sync();
-  if (tid == 0) asm volatile("red.release.gpu.global.add.u64 [%0], 1;" ::"l"(a.gbar) : "memory");
-  if (tid == 0 && jn[JOIN_PARTS] != 0) {
-    int there = 1;
-    for (long long it = 0; ld_acquire_u64(a.gbar) < gbar_base + gridDim.x;) {
-      if (++it > kSpinLimit) {
-        atomicOr(a.err, (uint32_t)MOE_ERR_BARRIER);
-        there = 0;
-        break;
-      }
-      if (it > 64) __nanosleep(20);
+}
+
+// The join. CTA c, of the border before the attention's CTA c, takes the (c - c0 - 1)-th of c1 - c0 equal shares of the
+// (row, four columns) items of the job that lies across it, the work of CTAs c0 .. c1. An item's parts, one per CTA of the
+// job in order, are weighted by 2^(m_i - m) and added; a share of few items has its parts spread over the threads.
+constexpr int kJoinThreads = 256;
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PAttnArgs a) {
+  constexpr int kCols = D / 4, kT = kJoinThreads, kMaxRows = 64;
+  __shared__ float4 red[kT];
+  // weights of the share's rows: rows * parts <= (64 / (parts - 1) + 2) * parts
+  __shared__ float wt[2 * kMaxRows + 2 * kPagedMaxCtas];
+  __shared__ float inv[kMaxRows];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x + 1;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int4 j0 = *reinterpret_cast<const int4*>(a.joins + c * JOIN_INTS);
+  const int2 j1 = *reinterpret_cast<const int2*>(a.joins + c * JOIN_INTS + 4);
+  const int parts = j0.x, c0 = j0.y, second = j0.z, b = j0.w, h = j1.x, rb = j1.y;
+  if (parts == 0) return;
+  const int rows = min(a.rows, a.G * a.Tq - rb * a.rows), all = rows * kCols, share = c - c0 - 1;
+  const int i0 = all * share / (parts - 1), i1 = all * (share + 1) / (parts - 1);  // all <= 2^12, parts <= 320
+  if (i0 >= i1) return;
+  const int r0 = i0 / kCols, r1 = (i1 - 1) / kCols + 1;
+  auto part = [&](int i) { return (int64_t)(c0 + i) * 2 + (i == 0 ? second : 0); };
+  // Few items (many parts): the parts of an item over `slices` threads, a power of two up to 32. Many items (few parts):
+  // kItems items a thread at a time. Either way each thread's first kAhead values are on their way while the weights are
+  // found: eight parts of one item, or two of each of four.
+  constexpr int kAhead = 8, kItems = 4;
+  int lg = 0;
+  while (lg < 5 && (i1 - i0) << (lg + 1) <= kT) ++lg;
+  const int slices = 1 << lg, lanes = kT >> lg, sl = (tid << lg) / kT, mine = i0 + (tid & (lanes - 1));
+  auto load = [&](int it, int i) {
+    const int r = it / kCols, col = it % kCols;
+    return it < i1 && i < parts ? __ldcg(reinterpret_cast<const float4*>(a.acc + (part(i) * a.rows + r) * D + col * 4))
+                                : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  auto weight = [&](int it, int i) { return it < i1 && i < parts ? wt[(it / kCols - r0) * parts + i] : 0.f; };
+  auto add = [](float4& s, const float4& x, float f) {
+    s.x = fmaf(x.x, f, s.x);
+    s.y = fmaf(x.y, f, s.y);
+    s.z = fmaf(x.z, f, s.z);
+    s.w = fmaf(x.w, f, s.w);
+  };
+  auto store = [&](int it, const float4& s) {
+    if (it >= i1) return;
+    const int r = it / kCols, col = it % kCols, q = rb * a.rows + r, t = token_of(a, q);
+    const float d = inv[r - r0];
+    *reinterpret_cast<uint2*>(a.out + (((int64_t)b * a.Tq + t) * a.Hq + h * a.G + (q - t * a.G)) * D + col * 4) =
+        make_uint2(pack2<false>(s.x * d, s.y * d), pack2<false>(s.z * d, s.w * d));
+  };
+  float4 ahead[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k)
+    ahead[k] = slices > 1 ? load(mine, sl + k * slices) : load(mine + k % kItems * kT, k / kItems);
+  for (int r = r0 + warp; r < r1; r += kT / 32) {
+    constexpr int kHeld = 3;  // a lane's parts that stay in registers
+    float2 x[kHeld];
+    float m = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+      const int i = lane + 32 * k;
+      x[k] = i < parts ? __ldcg(reinterpret_cast<const float2*>(a.ml + (part(i) * a.rows + r) * 2))
+                       : make_float2(-INFINITY, 0.f);
     }
-    joined = there;
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) m = fmaxf(m, x[k].x);
+    for (int i = lane + 32 * kHeld; i < parts; i += 32) m = fmaxf(m, __ldcg(a.ml + (part(i) * a.rows + r) * 2));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float z = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+      const int i = lane + 32 * k;
+      const float f = ex2(x[k].x - z);
+      if (i < parts) wt[(r - r0) * parts + i] = f;
+      l = fmaf(x[k].y, f, l);
+    }
+    for (int i = lane + 32 * kHeld; i < parts; i += 32) {
+      const float2 v = __ldcg(reinterpret_cast<const float2*>(a.ml + (part(i) * a.rows + r) * 2));
+      const float f = ex2(v.x - z);
+      wt[(r - r0) * parts + i] = f;
+      l = fmaf(v.y, f, l);
+    }
+    l = warp_sum(l);
+    if (lane == 0) inv[r - r0] = l == 0.f ? 0.f : (a.v_scale ? a.v_scale[h] : 1.f) / l;
   }
-  join_sync<C::kJoin>();
-  if (jn[JOIN_PARTS] != 0 && joined) join_share<D, C::kJoin>(a, jn, *reinterpret_cast<JoinScratch*>(ring));
+  __syncthreads();
+  if (slices > 1) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) add(s, ahead[k], weight(mine, sl + k * slices));
+#pragma unroll 4
+    for (int i = sl + kAhead * slices; i < parts; i += slices) add(s, load(mine, i), weight(mine, i));
+    red[tid] = s;
+    __syncthreads();
+    if (sl != 0) return;
+    for (int k = 1; k < slices; ++k) add(s, red[k * lanes + tid], 1.f);
+    store(mine, s);
+  } else {
+    for (int base = mine; base < i1; base += kItems * kT) {
+      float4 s[kItems];
+#pragma unroll
+      for (int k = 0; k < kItems; ++k) s[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int i = 0; i < parts; i += 2) {
+        if (i > 0 || base != mine) {
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k) ahead[k] = load(base + k % kItems * kT, i + k / kItems);
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+          add(s[k % kItems], ahead[k], weight(base + k % kItems * kT, i + k / kItems));
+      }
+#pragma unroll
+      for (int k = 0; k < kItems; ++k) store(base + k * kT, s[k]);
+    }
+  }
 }
 
 // ------------------------------------------------------------------ host side
@@ -955,7 +930,10 @@ cudaError_t launch_attn(const PAttnArgs& args, const CUtensorMap& mk, const CUte
   a.ctas = std::min(kPagedMaxCtas, paged_sms() * C::kPerSm);
   CUtensorMap k = mk, v = mv;
   void* p[] = {&a, &k, &v};
-  return paged_launch(fn, dim3(a.ctas), dim3(C::kThreads), smem, s, p, 1, true);
+  e = paged_launch(fn, dim3(a.ctas), dim3(C::kThreads), smem, s, p);
+  if (e != cudaSuccess) return e;
+  void* j[] = {&a};
+  return paged_launch(reinterpret_cast<const void*>(paged_join_kernel<D>), dim3(a.ctas - 1), dim3(kJoinThreads), 0, s, j);
 }
 
 template <int D, bool F8>
@@ -992,7 +970,7 @@ int moe_paged_attend(const moe_paged_cache* c, int layer, const int32_t* seqs, i
   a.seqs = seqs;
   a.tables = c->tables;
   a.lens = c->lens;
-  a.gbar = reinterpret_cast<unsigned long long*>(ws + (c->D == 256 ? L.gbar1 : L.gbar2));
+  a.joins = reinterpret_cast<int32_t*>(ws + L.joins);
   a.ml = reinterpret_cast<float*>(ws + L.ml);
   a.acc = reinterpret_cast<float*>(ws + L.acc);
   a.err = reinterpret_cast<uint32_t*>(ws + L.err);

@@ -4,9 +4,13 @@
 // A page call is a plan and a move. The plan (which pages change hands) is integer work over lists, tables and the
 // holder counts: one CTA of 1024 threads, so that its steps are separated by block barriers and its result depends on
 // the inputs alone. The move is pure traffic: the plan's (source, destination, rows) triples times layers times {k, v},
-// cut into 16 KB pieces that the whole GPU takes in turn. The move is a launch of its own, programmatically dependent on
-// the plan's: as one cooperative launch with a barrier between them, forking 32 sequences and growing them took 36 us
-// instead of 22.
+// cut into 16 KB pieces that the whole GPU takes in turn. The move is a launch of its own, programmatically dependent
+// on the plan's: as one cooperative launch with a barrier between them, forking 32 sequences and growing them took 36 us
+// instead of 24.
+//
+// Measured on a B200: 32 children forked from 4 sequences of 2087 tokens, freed, and grown by a token over 10 layers
+// (25 MB copied) 24 us: 10 us of it the move, the rest the latency of three plans; compaction of a pool of 3001 pages,
+// 40 % live, over 4 layers (377 MB moved) 131 us, 5.8 TB/s read and written.
 #include <algorithm>
 #include <cstring>
 
@@ -169,7 +173,9 @@ __global__ void __launch_bounds__(kPlanThreads) resize_plan_kernel(const __grid_
     if (base > a.num_pages) break;  // more than there can be: no sum may pass the list
   }
   const int want_all = base;
-  const int found = want_all > a.num_pages ? -1 : find_free(a.refs, a.num_pages, want_all, a.list, sm, released ? nullptr : &ahead);
+  const int found = want_all > a.num_pages ? -1
+                                           : find_free(a.refs, a.num_pages, want_all, a.list, sm,
+                                                       released ? nullptr : &ahead);
   __syncthreads();
   if (found < want_all) {  // nothing is changed: the holders come back
     for (int i = warp; i < n; i += nw) {
@@ -428,7 +434,8 @@ __device__ __forceinline__ u64 fma2(u64 x, u64 y, u64 z) {
 // L = D / 16 lanes of 16 values, the chunks of eight lane and lane + L; a warp takes 32 / L heads of a token at a time
 // and fetches the next ones before it works on these. The pairs of the rotation meet by shuffles, in one lane (rope_dim
 // = D), or in shared memory where they lie at different places of two lanes. TT = 1 and several CTAs a token where the
-// CTAs of TT = 4 would not fill the GPU twice.
+// CTAs of TT = 4 would not fill the GPU twice. 4095 tokens of 16 + 2 + 2 heads of 256 take 20 us (4.1 TB/s; about 170
+// instructions a warp for every two heads bound it, not memory), 64 tokens 3.4 us.
 template <int D, bool F8, int TT>
 __global__ void __launch_bounds__(kAppendWarps * 32, 4) append_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int L = D / 16, kHeads = 32 / L;
@@ -440,7 +447,8 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 4) append_kernel(const __gr
   const int heads = a.Hq + 2 * a.Hkv, half = a.rope_dim >> 1;
   // this CTA's share of the (token, group of heads) items, token by token, a warp every kAppendWarps-th
   const int groups = (heads + kHeads - 1) / kHeads, items = here * groups;
-  const int begin = (int)((int64_t)items * blockIdx.y / gridDim.y), end = (int)((int64_t)items * (blockIdx.y + 1) / gridDim.y);
+  const int begin = (int)((int64_t)items * blockIdx.y / gridDim.y);
+  const int end = (int)((int64_t)items * (blockIdx.y + 1) / gridDim.y);
   struct Item {
     int k, g, left;  // token, group, items from this one to the end
     __device__ __forceinline__ void on(int groups) {
@@ -620,7 +628,8 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 4) append_kernel(const __gr
           q[i] = 0;
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            q[i] |= (uint32_t)__nv_cvt_float_to_fp8(__fdiv_rn(v[c][4 * i + j], sc), __NV_SATFINITE, __NV_E4M3) << (8 * j);
+            q[i] |= (uint32_t)__nv_cvt_float_to_fp8(__fdiv_rn(v[c][4 * i + j], sc), __NV_SATFINITE, __NV_E4M3)
+                    << (8 * j);
         }
         reinterpret_cast<uint2*>(dst)[hl + c * L] = make_uint2(q[0], q[1]);
       }
@@ -703,7 +712,8 @@ CopyArgs copy_args(const moe_paged_cache* c, const PageArgs& p, bool planned, bo
 cudaError_t launch_copy(const CopyArgs& args, cudaStream_t s) {
   CopyArgs a = args;
   void* p[] = {&a};
-  return paged_launch(reinterpret_cast<const void*>(plane_copy_kernel), dim3(paged_sms() * 4), dim3(kCopyThreads), 0, s, p);
+  return paged_launch(reinterpret_cast<const void*>(plane_copy_kernel), dim3(paged_sms() * 4), dim3(kCopyThreads), 0, s,
+                      p);
 }
 
 }  // namespace
@@ -785,8 +795,8 @@ int moe_paged_append(const moe_paged_cache* c, int layer, const int32_t* seqs, i
       Hq % c->Hkv != 0 || rope_dim < 0 || rope_dim > c->D || rope_dim % 2 != 0)
     return (int)cudaErrorInvalidValue;
   if (B == 0) return (int)cudaSuccess;
-  if (!seqs || !qkv || !q_out || !paged_al16(qkv) || !paged_al16(q_out) || !paged_al16(q_norm) || !paged_al16(k_norm) || (q_norm == nullptr) != (k_norm == nullptr) ||
-      (rope_dim > 0) != (inv_freq != nullptr))
+  if (!seqs || !qkv || !q_out || !paged_al16(qkv) || !paged_al16(q_out) || !paged_al16(q_norm) ||
+      !paged_al16(k_norm) || (q_norm == nullptr) != (k_norm == nullptr) || (rope_dim > 0) != (inv_freq != nullptr))
     return (int)cudaErrorInvalidValue;
   const int64_t off = layer * paged_layer_bytes(c);
   AppendArgs a;

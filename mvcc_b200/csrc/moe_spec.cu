@@ -1,8 +1,8 @@
 // moe_spec.cu -- probabilities of a step's logits and the verification of drafted tokens (include/moe_spec.h).
 //
 //   softmax_rows_kernel  short rows: a CTA (or a cluster) a row, its values in registers; one read, one write.
-//   softmax_ring_kernel  long rows: a row is a cluster of up to 8 CTAs. Each CTA walks its share of row after row: a bulk
-//                        copy brings the next row's share into shared memory while this row's, in registers, is
+//   softmax_ring_kernel  long rows: a row is a cluster of up to 8 CTAs. Each CTA walks its share of row after row: a
+//                        bulk copy brings the next row's share into shared memory while this row's, in registers, is
 //                        reduced and stored. The CTAs' (maximum, sum of 2^((x - max) c)) pairs meet through distributed
 //                        shared memory behind one cluster barrier a row, and each CTA rescales what it holds. Two CTAs
 //                        an SM: one's barriers hide behind the other's stores (192 rows of 151936: 50 us; one CTA an SM
@@ -10,10 +10,12 @@
 //                        8 V.
 //   verify_kernel        CTA (chunk, sequence): which drafts are accepted (a few gathered values, found by every warp
 //                        alone), then each warp's fp64 sum of the weights of its stretch of the chunk; the sequence's
-//                        last CTA to finish finds the stretch and, in it, the token whose running sum passes u times the
-//                        total. Only the row that the token is drawn from is read: 8 V bytes a sequence. fp64, because a
+//                        last CTA to finish finds the stretch and, in it, the token whose running sum passes u times
+//                        the total. Only the row that the token is drawn from is read: 8 V bytes a sequence. fp64, because a
 //                        running sum in fp32 is off by more than the smallest gap between two tokens of a large
-//                        vocabulary, and the choice would depend on the order of the sum.
+//                        vocabulary, and the choice would depend on the order of the sum. 64 sequences of 4 drafts
+//                        over 151936 tokens: 19 to 21 us (12 us of them bytes, 5 us the two chains of dependent loads
+//                        before and after); one sequence 7 us.
 #include <algorithm>
 #include <atomic>
 
