@@ -121,9 +121,10 @@ MOE_API int moe_paged_append(const moe_paged_cache* c, int layer, const int32_t*
 /* Causal attention of the new tokens over the cached keys and values of layer `layer`, theirs included: query head h
  * reads kv head h / (Hq / Hkv), softmax(scale q . k) . v in fp32, out bf16 [B Tq][Hq D]. Rows of unused slots, of
  * empty sequences and of no token are zero. What lies in a page behind a sequence's end, and what a token may not see,
- * has no influence, NaN and infinities included. Hq / Hkv any whole number with Hq <= 128; Tq <= 8; B <= 2048. q, out
- * 16-byte aligned. The batch's work is shared out over the GPU by keys, whatever the lengths, and the parts of a
- * sequence joined in order: the same call gives the same bits. */
+ * has no influence, NaN and infinities included. G = Hq / Hkv any whole number with Hq <= 128; Tq <= 8; B <= 2048;
+ * B Hkv ceil(G Tq / 64) max_pages page at most 2^34 (the work is counted in 32 bits); q, out 16-byte aligned. The
+ * batch's work is shared out over the GPU by keys, whatever the lengths, and the parts of a sequence joined in order:
+ * the same call gives the same bits. */
 MOE_API int moe_paged_attend(const moe_paged_cache* c, int layer, const int32_t* seqs, int B, int Tq,
                              const uint16_t* q, int Hq, float scale, uint16_t* out, void* workspace,
                              size_t workspace_bytes, moe_stream_t stream);

@@ -24,9 +24,9 @@ MOE_API int moe_lm_head_logits(const uint16_t* normed, const uint16_t* lm_head, 
 /* probs[r][v] = exp((x_v - m) / t_r) / sum_w exp((x_w - m) / t_r), m the row's largest logit, for R rows of V fp32
  * logits; rows lie ld_logits and ld_probs floats apart (at least V; what lies between rows is left alone). temperature
  * fp32 [R] (NULL = 1): a row with t_r = 0 (or negative or NaN) puts everything on its largest logit, the lowest index
- * of a tie. NaN logits and -infinity get probability zero (a NaN never wins, as in moe_lm_head_argmax); +infinity
- * takes all (shared by several); a row with no logit above -infinity is all zeros. probs may be logits itself (with
- * the same ld), but not overlap it otherwise. 1 <= V < 2^24, R >= 0. */
+ * of a tie, and an infinite one shares equally. NaN logits and -infinity get probability zero (a NaN never wins, as in
+ * moe_lm_head_argmax); +infinity takes all (shared by several); a row with no logit above -infinity is all zeros. probs
+ * may be logits itself (with the same ld), but not overlap it otherwise. 1 <= V < 2^24, R >= 0. */
 MOE_API int moe_softmax_rows(const float* logits, int64_t ld_logits, int R, int V, const float* temperature,
                              float* probs, int64_t ld_probs, moe_stream_t stream);
 

@@ -5,17 +5,17 @@
 //                        bulk copy brings the next row's share into shared memory while this row's, in registers, is
 //                        reduced and stored. The CTAs' (maximum, sum of 2^((x - max) c)) pairs meet through distributed
 //                        shared memory behind one cluster barrier a row, and each CTA rescales what it holds. Two CTAs
-//                        an SM: one's barriers hide behind the other's stores (192 rows of 151936: 50 us; one CTA an SM
+//                        an SM: one's barriers hide behind the other's stores (192 rows of 151936: 52 us; one CTA an SM
 //                        with two buffers 60 us; a CTA per row share without the walk 95 us). Bound by the row's bytes,
 //                        8 V.
 //   verify_kernel        CTA (chunk, sequence): which drafts are accepted (a few gathered values, found by every warp
 //                        alone), then each warp's fp64 sum of the weights of its stretch of the chunk; the sequence's
 //                        last CTA to finish finds the stretch and, in it, the token whose running sum passes u times
-//                        the total. Only the row that the token is drawn from is read: 8 V bytes a sequence. fp64, because a
-//                        running sum in fp32 is off by more than the smallest gap between two tokens of a large
-//                        vocabulary, and the choice would depend on the order of the sum. 64 sequences of 4 drafts
-//                        over 151936 tokens: 19 to 21 us (12 us of them bytes, 5 us the two chains of dependent loads
-//                        before and after); one sequence 7 us.
+//                        the total. Only the row that the token is drawn from is read: 8 V bytes a sequence. fp64,
+//                        because a running sum in fp32 is off by more than the smallest gap between two tokens of a
+//                        large vocabulary, and the choice would depend on the order of the sum. 64 sequences of 4
+//                        drafts over 151936 tokens: 19 us (12 us of them bytes, 5 us the two chains of dependent
+//                        loads before and after); one sequence 7 us.
 #include <algorithm>
 #include <atomic>
 
@@ -69,6 +69,8 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// log2(e) / t, but never zero: at an infinite temperature a logit of -infinity keeps its weight of zero.
+__device__ __forceinline__ float soft_factor(float t) { return fmaxf(1.4426950408889634f / t, 1.4e-45f); }
 // 2^((v - m) c) for v <= m, neither a NaN. Where m or c is infinite the difference or the product may be no number: then
 // one at the maximum itself, zero below it.
 __device__ __forceinline__ float soft_weight(float v, float m, float c) { return ex2((v - m) * c); }
@@ -94,7 +96,7 @@ __global__ void __launch_bounds__(kSmThreads, VEC == 4 ? 2 : 1) softmax_rows_ker
   float* y = a.y + row * a.ldy;
   const float t = a.temperature ? a.temperature[row] : 1.f;
   const bool greedy = !(t > 0.f);
-  const float c = greedy ? 0.f : 1.4426950408889634f / t;
+  const float c = greedy ? 0.f : soft_factor(t);
   const int chunk = ((a.V + CL - 1) / CL + 3) & ~3;
   const int b0 = min(a.V, rank * chunk), b1 = min(a.V, b0 + chunk);
   auto weight = [&](float v, float m) { return soft_weight_any(v, m, c); };
@@ -282,7 +284,7 @@ __global__ void __launch_bounds__(kSmThreads, N <= 10 ? 2 : 1) softmax_ring_kern
     for (int o = kSmWarps / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float t = a.temperature ? a.temperature[row] : 1.f;
     const bool greedy = !(t > 0.f);
-    const float c = greedy ? 0.f : 1.4426950408889634f / t;
+    const float c = greedy ? 0.f : soft_factor(t);
     float s;
     if (!greedy) {
       float z = m, cz = c;

@@ -102,10 +102,11 @@ def test_layer_call_refuses_before_launch():
     assert n(ctypes.byref(w), ctypes.byref(cache(Hkv=4)), 4, 1) == 0 and n(ctypes.byref(w), ctypes.byref(cache(D=128)), 4,
                                                                          1) == 0
 
-    def call(rms=PTR, h=PTR, cc=c, seqs=PTR, B=4, Tq=1, f=PTR, out=PTR, ws=PTR, size=big):
-        return L.moe_attn_paged_forward_rms(ctypes.byref(w), rms, h, cc, 0, seqs, B, Tq, f, out, ws, size, None)
+    def call(rms=PTR, h=PTR, cc=c, layer=0, seqs=PTR, B=4, Tq=1, f=PTR, out=PTR, ws=PTR, size=big):
+        return L.moe_attn_paged_forward_rms(ctypes.byref(w), rms, h, cc, layer, seqs, B, Tq, f, out, ws, size, None)
     for kw in ({"rms": None}, {"h": None}, {"h": PTR + 4}, {"seqs": None}, {"B": 0}, {"Tq": 9}, {"f": None},
-               {"out": None}, {"ws": None}, {"size": 256}, {"cc": ctypes.byref(cache(Hkv=4))}):
+               {"out": None}, {"ws": None}, {"size": 256}, {"cc": ctypes.byref(cache(Hkv=4))},
+               {"layer": -1}, {"layer": cache().layers}, {"cc": ctypes.byref(cache(k=None))}):
         assert call(**kw) == BAD, kw
 
 

@@ -106,6 +106,22 @@ def test_softmax_of_masked_and_infinite_rows(V):
             near(out, x, tt)
 
 
+@pytest.mark.parametrize("V", [1, 37, 4096, 50001, 151936, 270000])
+def test_softmax_at_an_infinite_temperature_shares_equally(V):
+    x = 9 * torch.randn(5, V, device="cuda", generator=torch.Generator(device="cuda").manual_seed(V))
+    x[1, ::3] = -math.inf
+    x[2, V // 2] = math.nan
+    x[3] = -math.inf
+    x[4, V - 1] = math.inf
+    out = torch.full_like(x, 9.0)
+    S().softmax_rows(x, out, temperature=torch.full((5,), math.inf, device="cuda"))
+    on = x > -math.inf  # False for a NaN
+    on[4, :V - 1] = False
+    want = on.double() / on.sum(1, keepdim=True).clamp(min=1).double()
+    # the sum of up to V ones: its rounding, a chain's and a tree's, then the division's and the product's
+    assert bool(((out.double() - want).abs() <= 2.0 ** -20 * want).all())
+
+
 def test_softmax_keeps_what_lies_between_rows():
     x = torch.randn(6, 1000, device="cuda")
     y = torch.full((6, 1003), 5.0, device="cuda")
