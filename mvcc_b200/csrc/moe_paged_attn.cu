@@ -16,7 +16,7 @@
 //
 // CTA: four or eight consumer warps and four producer warps (a thread issues a TMA copy every 95 cycles or so: one an SM
 // fetches 3.2 TB/s over the GPU in 2 KB boxes, four 6.4 TB/s). Producer w takes every NP-th of the CTA's tiles (KT keys of
-// k and v each), reads the page ids 32 at a time and fetches the tiles by TMA (boxes of 128 bytes x 16 or KT rows inside
+// k and v each), looks up their pages eight tiles ahead and fetches them by TMA (boxes of 128 bytes x 16 or KT rows inside
 // one page, 128-byte swizzle) into a ring of NS slots, mbarrier-counted. Consumer warp (g, mt) holds 16 query rows as MMA
 // fragments and takes every NG-th tile: S = Q K^T, the running maximum and sum of the softmax, O += P V, all in
 // registers; at a job's end the NG warps of a row tile merge through shared memory.
@@ -26,9 +26,9 @@
 // tile; at 16 rows the register MMA needs under a third of the cycles that the tile's bytes take to arrive.
 //
 // Measured on a B200 (16 query and 2 kv heads of 256, bf16, unless said otherwise; the device copy moves 6.45 TB/s): one
-// sequence of 131071 keys 51 us (5.2 TB/s), 48 ragged sequences of up to 8192 keys 69 us (5.4 TB/s), with 4 and 8 new
+// sequence of 131071 keys 52 us (5.2 TB/s), 48 ragged sequences of up to 8192 keys 70 us (5.4 TB/s), with 4 and 8 new
 // tokens each 82 and 128 us; 24 sequences of up to 16000 keys, 32 over 8 heads of 128, 4 tokens: 123 us in bf16
-// (5.9 TB/s), 79 us in e4m3 with pages of 16 (4.6 TB/s). The loop over the tiles runs at the read bandwidth for bf16 and
+// (5.9 TB/s), 77 us in e4m3 with pages of 16 (4.7 TB/s). The loop over the tiles runs at the read bandwidth for bf16 and
 // one row tile; around it lie 2 us for the units, 1.5 us for the first queries and pages, 2 us for the last merge, 1 to
 // 4 us for the slowest CTA and 3 us for the join. With e4m3 or several row tiles the consumers' latency a tile (2000
 // cycles, two warps a scheduler) bounds it.
@@ -299,27 +299,21 @@ __global__ void __launch_bounds__(Cfg<D, F8, MT>::kThreads, Cfg<D, F8, MT>::kPer
     // ---------------------------------------------------------------- producer
     if constexpr (C::kHandOver) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kProducerRegs));
     const int none = a.num_pages * a.Hkv;  // a page that is not there: outside the map, reads as zero
-    const int nbox = KT / a.box_rows;
-    int i = 0;      // tiles so far: slot i % NS, for the turn-th time
-    int slot = 0, turn = 0;
-    auto on = [&] {
-      ++i;
-      if (++slot == NS) {
-        slot = 0;
-        ++turn;
-      }
-    };
+    const int nbox = KT / a.box_rows;      // 1 or 2
+    const int own = warp - kWarps;
+    int slot = own, turn = 0;              // of this warp's next tile, the slot for the turn-th time
+    int next = own, before = 0;            // that tile's number; tiles of the jobs so far
     bool ok = true;
     while (ok && w.next(S, a.B, HR)) {
       const int lu = w.lu, run = w.run, h = w.job / a.row_blocks;
       const int n = keys[w.b];
       const int32_t* row = a.tables + (int64_t)seqs[w.b] * a.max_pages;
       const int key_end = (lu + run) * UK;
-      int z = 0, y = 0;
-      int fetched = lu * UK;  // first key whose box no lane holds yet
-      int held = 0;           // first key of lane 0's box
-      for (int key = lu * UK; key < key_end && ok; key += KT, on()) {
-        if (i % NP != warp - kWarps) continue;
+      // Pages of this warp's next eight tiles, a lane a box, and the lane of the next box. (32 at a time: 52.3 us for one
+      // sequence of 131071 keys, 8: 51.8.)
+      int z = 0, y = 0, at = 8 * nbox;
+      for (; next < before + run * NG; next += NP) {
+        const int key = lu * UK + (next - before) * KT;
         if (turn > 0) {
           ok = bar_wait(&empty[slot], (turn - 1) & 1);
           if (!ok) {
@@ -329,44 +323,50 @@ __global__ void __launch_bounds__(Cfg<D, F8, MT>::kThreads, Cfg<D, F8, MT>::kPer
         }
         if (key >= n) {  // a unit's tile behind the sequence's end
           if (lane == 0) mbar_arrive(&full[slot]);
-          continue;
-        }
-        while (key >= fetched) {  // the next 32 boxes' pages
-          held = fetched;
-          const int k = fetched + lane * a.box_rows;
-          z = none;
-          y = 0;
-          if (k < n && k < key_end) {
-            const int pid = row[k / a.page];
-            if (pid >= 0 && pid < a.num_pages) z = pid * a.Hkv + h;
-            else atomicOr(a.err, (uint32_t)MOE_ERR_PAGE_ID);
-            y = k % a.page;
-          }
-          fetched += 32 * a.box_rows;
-        }
-        const int boxes = min(nbox, (n - key + a.box_rows - 1) / a.box_rows);
-        uint8_t* dst = ring + (size_t)slot * C::kSlot;
-        if (lane == 0) expect_tx(&full[slot], (uint32_t)(2 * boxes * a.box_rows * C::kRow));
-        __syncwarp();
-        for (int x = 0; x < boxes; ++x) {
-          const int from = (key - held) / a.box_rows + x;
-          const int bz = __shfl_sync(0xffffffffu, z, from), by = __shfl_sync(0xffffffffu, y, from);
-          // one lane issues every copy: the operands of a TMA instruction are uniform, lanes would take turns
-          if (lane == 0) {
-#pragma unroll
-            for (int sg = 0; sg < C::kSegs; ++sg) {
-              uint8_t* at = dst + sg * C::kSeg + x * a.box_rows * 128;
-              tma_load_3d(at, &map_k, sg * (128 / C::kEs), by, bz, &full[slot]);
-              tma_load_3d(at + C::kTile, &map_v, sg * (128 / C::kEs), by, bz, &full[slot]);
+        } else {
+          if (at == 8 * nbox) {
+            at = 0;
+            const int k = key + (nbox == 2 ? (lane >> 1) * NP * KT + (lane & 1) * a.box_rows : lane * NP * KT);
+            z = none;
+            y = 0;
+            if (lane < 8 * nbox && k < n && k < key_end) {
+              const int pid = row[k / a.page];
+              if (pid >= 0 && pid < a.num_pages) z = pid * a.Hkv + h;
+              else atomicOr(a.err, (uint32_t)MOE_ERR_PAGE_ID);
+              y = k % a.page;
             }
           }
+          const int boxes = min(nbox, (n - key + a.box_rows - 1) / a.box_rows);
+          uint8_t* dst = ring + (size_t)slot * C::kSlot;
+          if (lane == 0) expect_tx(&full[slot], (uint32_t)(2 * boxes * a.box_rows * C::kRow));
+          __syncwarp();
+          for (int x = 0; x < boxes; ++x) {
+            const int bz = __shfl_sync(0xffffffffu, z, at + x), by = __shfl_sync(0xffffffffu, y, at + x);
+            // one lane issues every copy: the operands of a TMA instruction are uniform, lanes would take turns
+            if (lane == 0) {
+#pragma unroll
+              for (int sg = 0; sg < C::kSegs; ++sg) {
+                uint8_t* to = dst + sg * C::kSeg + x * a.box_rows * 128;
+                tma_load_3d(to, &map_k, sg * (128 / C::kEs), by, bz, &full[slot]);
+                tma_load_3d(to + C::kTile, &map_v, sg * (128 / C::kEs), by, bz, &full[slot]);
+              }
+            }
+          }
+          __syncwarp();
+          at += nbox;
         }
-        __syncwarp();
+        if ((slot += NP) >= NS) {
+          slot = own;
+          ++turn;
+        }
       }
+      before += run * NG;
     }
-    if (!ok)  // no copy may still be landing when the CTA exits
-      for (int j = max(0, i - NS); j < i; ++j)
-        if (j % NP == warp - kWarps) bar_wait(&full[j % NS], (j / NS) & 1);
+    if (!ok)  // no copy may still be landing when the CTA exits: this warp's last tiles
+      for (int k = own; k < NS; k += NP) {
+        const int t = k < slot ? turn : turn - 1;  // the slot's last turn
+        if (t >= 0) bar_wait(&full[k], t & 1);
+      }
     return;
   }
 
