@@ -408,11 +408,13 @@ struct AppendArgs {
   const int32_t* lens;
   uint32_t* err;
   int32_t B, Tq, Hq, Hkv, page, num_pages, max_seqs, max_pages, rope_dim;
+  int32_t per;  // tokens a CTA
   float eps;
 };
 
 constexpr int kAppendWarps = 8;
-constexpr int kAppendMany = 4;  // tokens a CTA where there are many
+constexpr int kAppendCtas = 4;  // an SM
+constexpr int kAppendMany = 8;  // tokens a CTA at most, where there are many
 
 // Packed pairs of fp32 (sm_100a): two roundings to nearest an instruction.
 __device__ __forceinline__ u64 pair(float lo, float hi) {
@@ -429,21 +431,22 @@ __device__ __forceinline__ u64 fma2(u64 x, u64 y, u64 z) {
   return r;
 }
 
-// A CTA takes TT tokens: their positions are looked up and their angles formed once (in fp64: position times frequency,
+// A CTA takes up to TT tokens: their positions are looked up and their angles formed once (in fp64: position times frequency,
 // in half turns, reduced to [-1, 1] before the fp32 sine and cosine), while the first rows are on their way. A head is
 // L = D / 16 lanes of 16 values, the chunks of eight lane and lane + L; a warp takes 32 / L heads of a token at a time
 // and fetches the next ones before it works on these. The pairs of the rotation meet by shuffles, in one lane (rope_dim
-// = D), or in shared memory where they lie at different places of two lanes. TT = 1 and several CTAs a token where the
-// CTAs of TT = 4 would not fill the GPU twice. 4095 tokens of 16 + 2 + 2 heads of 256 take 20 us (4.1 TB/s; about 170
-// instructions a warp for every two heads bound it, not memory), 64 tokens 3.4 us.
+// = D), or in shared memory where they lie at different places of two lanes. TT = 1 and several CTAs a token where two
+// tokens a CTA would be too few for every SM; else every CTA takes the same share, in as few full rounds of the GPU as
+// eight tokens a CTA allow (four a CTA and a last round of any size: 8 to 10 % slower). 4095 tokens of 16 + 2 + 2 heads
+// of 256 take 18.6 us (4.5 TB/s; about 170 instructions a warp for every two heads bound it, not memory), 64 tokens 3.5.
 template <int D, bool F8, int TT>
-__global__ void __launch_bounds__(kAppendWarps * 32, 4) append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(kAppendWarps * 32, kAppendCtas) append_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int L = D / 16, kHeads = 32 / L;
   __shared__ __align__(16) float cs[TT][D / 2], sn[TT][D / 2];
   __shared__ __align__(16) float rows[kAppendWarps][kHeads][D];
   __shared__ int seq_s[TT], pos_s[TT];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hl = lane % L, hw = lane / L;
-  const int tok0 = blockIdx.x * TT, T = a.B * a.Tq, here = min(TT, T - tok0);
+  const int per = TT == 1 ? 1 : a.per, tok0 = blockIdx.x * per, T = a.B * a.Tq, here = min(per, T - tok0);
   const int heads = a.Hq + 2 * a.Hkv, half = a.rope_dim >> 1;
   // this CTA's share of the (token, group of heads) items, token by token, a warp every kAppendWarps-th
   const int groups = (heads + kHeads - 1) / kHeads, items = here * groups;
@@ -475,10 +478,10 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 4) append_kernel(const __gr
   uint4 next[2];
   fetch(ahead, next);
   // the tokens: sequence and position (-1: none, or a fault)
-  if (tid < TT) {
+  if (tid < here) {
     const int tok = tok0 + tid, b = tok / a.Tq, t = tok - b * a.Tq;
     int pos = -1;
-    const int s = tok < T ? a.seqs[b] : -1;
+    const int s = a.seqs[b];
     if (s >= 0 && s < a.max_seqs) {
       const int len = a.lens[s];
       if (len >= 0 && len <= a.max_pages * a.page) pos = max(-1, len - a.Tq + t);
@@ -490,7 +493,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 4) append_kernel(const __gr
     pos_s[tid] = pos;
   }
   __syncthreads();
-  for (int i = tid; i < TT * half; i += kAppendWarps * 32) {
+  for (int i = tid; i < here * half; i += kAppendWarps * 32) {
     const int k = i / half, d = i - k * half;
     double x = (double)pos_s[k] * a.inv_freq[d] * 0.31830988618379067154;  // 1 / pi
     x -= 2.0 * rint(0.5 * x);
@@ -642,11 +645,13 @@ cudaError_t launch_append(const AppendArgs& a, cudaStream_t s) {
   AppendArgs arg = a;
   void* args[] = {&arg};
   const int T = a.B * a.Tq, per_token = (a.Hq + 2 * a.Hkv + 512 / D - 1) / (512 / D);
-  const bool many = T > paged_sms() * 2 * kAppendMany;
+  // whole rounds of the CTAs that the GPU holds at once, with equal shares
+  const int slots = paged_sms() * kAppendCtas, rounds = (T + slots * kAppendMany - 1) / (slots * kAppendMany);
+  const bool many = T > slots * 2;
+  arg.per = many ? (T + slots * rounds - 1) / (slots * rounds) : 1;
   const void* fn = many ? reinterpret_cast<const void*>(append_kernel<D, F8, kAppendMany>)
                         : reinterpret_cast<const void*>(append_kernel<D, F8, 1>);
-  const dim3 grid(many ? (T + kAppendMany - 1) / kAppendMany : T,
-                  many ? 1 : (per_token + kAppendWarps - 1) / kAppendWarps);
+  const dim3 grid((T + arg.per - 1) / arg.per, many ? 1 : (per_token + kAppendWarps - 1) / kAppendWarps);
   return paged_launch(fn, grid, dim3(kAppendWarps * 32), 0, s, args);
 }
 
@@ -823,6 +828,7 @@ int moe_paged_append(const moe_paged_cache* c, int layer, const int32_t* seqs, i
   a.max_seqs = c->max_seqs;
   a.max_pages = c->max_pages;
   a.rope_dim = rope_dim;
+  a.per = 1;
   a.eps = eps;
   const cudaStream_t s = (cudaStream_t)stream;
   if (c->kv_type == MOE_KV_E4M3)

@@ -241,7 +241,9 @@ def rotate64(x, w, pos, inv_freq, eps=1e-6):
 
 @pytest.mark.parametrize("D,page,Hq,Hkv,rope,Tq,norm", [
     (256, 64, 16, 2, 64, 1, True), (256, 16, 8, 8, 256, 3, True), (128, 48, 10, 2, 6, 37, True), (64, 32, 3, 1, 2, 5, True),
-    (64, 16, 4, 4, 0, 1, True), (128, 64, 8, 1, 128, 130, False), (256, 32, 4, 2, 0, 2, False)])
+    (64, 16, 4, 4, 0, 1, True), (128, 64, 8, 1, 128, 130, False), (256, 32, 4, 2, 0, 2, False),
+    # several tokens a CTA, and several rounds of them
+    (128, 64, 4, 2, 128, 301, True), (256, 128, 2, 2, 64, 300, True), (64, 256, 2, 1, 6, 1001, True)])
 def test_append_against_64_bits(D, page, Hq, Hkv, rope, Tq, norm):
     far = 200_000 // page
     c = make(layers=2, pages=60, page=page, Hkv=Hkv, D=D, max_seqs=6, max_pages=far, Hq=Hq, max_new=Tq)
