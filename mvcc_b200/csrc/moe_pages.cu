@@ -413,7 +413,7 @@ struct AppendArgs {
 };
 
 constexpr int kAppendWarps = 8;
-constexpr int kAppendCtas = 4;  // an SM
+constexpr int kAppendCtas = 4;  // an SM (five, with 48 registers a thread: 22.8 us instead of 18.6 for the prompt below)
 constexpr int kAppendMany = 8;  // tokens a CTA at most, where there are many
 
 // Packed pairs of fp32 (sm_100a): two roundings to nearest an instruction.
