@@ -27,8 +27,8 @@
 //
 // Measured on a B200 (16 query and 2 kv heads of 256, bf16, unless said otherwise; the device copy moves 6.45 TB/s): one
 // sequence of 131071 keys 52 us (5.2 TB/s), 48 ragged sequences of up to 8192 keys 70 us (5.4 TB/s), with 4 and 8 new
-// tokens each 82 and 128 us; 24 sequences of up to 16000 keys, 32 over 8 heads of 128, 4 tokens: 123 us in bf16
-// (5.9 TB/s), 77 us in e4m3 with pages of 16 (4.7 TB/s). The loop over the tiles runs at the read bandwidth for bf16 and
+// tokens each 81 and 126 us; 24 sequences of up to 16000 keys, 32 over 8 heads of 128, 4 tokens: 123 us in bf16
+// (5.9 TB/s), 75 us in e4m3 with pages of 16 (4.8 TB/s). The loop over the tiles runs at the read bandwidth for bf16 and
 // one row tile; around it lie 2 us for the units, 1.5 us for the first queries and pages, 2 us for the last merge, 1 to
 // 4 us for the slowest CTA and 3 us for the join. With e4m3 or several row tiles the consumers' latency a tile (2000
 // cycles, two warps a scheduler) bounds it.
@@ -567,12 +567,14 @@ __global__ void __launch_bounds__(Cfg<D, F8, MT>::kThreads, Cfg<D, F8, MT>::kPer
         }
         nA = quad_max(nA);
         nB = quad_max(nB);
-        // f16 weights carry a common factor 2^15 (it cancels in the division): what a long row's many small weights
-        // lose below f16's normal range then stays under 2^-40 of the largest each.
-        constexpr float kLift = F8 ? 15.f : 0.f;
-        const float zA = nA == -INFINITY ? 0.f : nA * fA, zB = nB == -INFINITY ? 0.f : nB * fB;
-        if (__any_sync(0xffffffffu, nA != mA || nB != mB)) {
-          const float cA = ex2(fmaf(mA, fA, -zA)), cB = ex2(fmaf(mB, fB, -zB));
+        // The maximum that the weights refer to moves only when a row's grows by more than kSlack (in units of log 2), for
+        // moving it rescales the whole accumulator: with the true maximum, every other tile does for some row of a warp.
+        // A weight is then 2^kSlack at most, which costs no accuracy. f16 weights carry a common factor 2^11 besides (it
+        // cancels in the division), so that they end below 2^15 and what a long row's many small weights lose below f16's
+        // normal range stays under 2^-35 of the largest each.
+        constexpr float kSlack = 4.f, kLift = F8 ? 11.f : 0.f;
+        if (__any_sync(0xffffffffu, (nA - mA) * fA > kSlack || (nB - mB) * fB > kSlack)) {
+          const float cA = mA == nA ? 1.f : ex2((mA - nA) * fA), cB = mB == nB ? 1.f : ex2((mB - nB) * fB);
           lsum[0] *= cA;
           lsum[2] *= cB;
 #pragma unroll
@@ -585,6 +587,7 @@ __global__ void __launch_bounds__(Cfg<D, F8, MT>::kThreads, Cfg<D, F8, MT>::kPer
           mA = nA;
           mB = nB;
         }
+        const float zA = mA == -INFINITY ? 0.f : mA * fA, zB = mB == -INFINITY ? 0.f : mB * fB;
         // P in the cache's MMA type; the sums take the rounded weights, so that a row's weights still add up to one
         uint32_t pf[KT / 16][4];
         const float yA = kLift - zA, yB = kLift - zB;

@@ -500,6 +500,23 @@ def test_attention_scores_of_any_size():
         assert bool(((vals(out) - want).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("kv,D,Tq", [("bf16", 64, 1), ("bf16", 128, 4), ("bf16", 256, 1), ("e4m3", 128, 2), ("e4m3", 256, 3)])
+def test_attention_of_scores_that_climb_and_fall(kv, D, Tq):
+    """Scores that rise over 2000 keys by 50 powers of two, evenly, in steps, or falling: the running maximum moves in
+    every tile, in a few, or never."""
+    n, page = 2000, 16
+    c = filled([n] * 3, Hq=4, Hkv=2, D=D, page=page, kv=kv, Tq=Tq)
+    j = torch.arange(n, device="cuda")
+    for s, ramp in enumerate((8.0 * j / n, 0.8 * (j // 200), 8.0 - 8.0 * j / n)):
+        ids = c.tables[s, :n // page].long()
+        at = ramp.view(-1, 1, page).expand(-1, 2, -1)
+        k = c.k.view(torch.bfloat16 if kv == "bf16" else torch.float8_e4m3fn)
+        k[0, ids, :, :, 0] = at.to(k.dtype)
+    q = vals(queries(c, 3, Tq, std=0.5)).view(-1, D).float()
+    q[:, 0] = 4.4 * D ** 0.5
+    check_attend(c, [0, 1, 2], Tq, kv, q=bits(q.view(3 * Tq, -1)))
+
+
 def test_attention_with_bad_pages_and_sequences_is_recorded_and_bounded():
     c = filled([100, 40], Hq=2, Hkv=2, D=64, page=16, max_batch=8)
     q = queries(c, 2, 1)
