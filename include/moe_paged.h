@@ -62,7 +62,7 @@ enum {
 MOE_API int moe_paged_check(const moe_paged_cache* c);
 
 /* Bytes of caller-owned workspace for the calls below with Hq query heads, lists of up to max_batch entries
- * (1 .. 2048) and up to max_new new tokens a sequence (1 .. 8 for moe_paged_attend; more for moe_paged_append only); 0
+ * (1 .. 4096) and up to max_new new tokens a sequence (1 .. 8 for moe_paged_attend; more for moe_paged_append only); 0
  * for unsupported sizes. One workspace per concurrently running call, on the cache's device. Zero it once before its
  * first call. Calls that share one (two captured graphs of the same stream, say) must not overlap. */
 MOE_API size_t moe_paged_workspace_bytes(const moe_paged_cache* c, int Hq, int max_batch, int max_new);
@@ -81,7 +81,7 @@ MOE_API int moe_paged_workspace_error(void* workspace, size_t workspace_bytes, m
  * sequences hold too is replaced by a copy of its filled rows, in every layer, in a page of its own (of k listed
  * sequences that end in one page, all its holders but the last in list order copy). That copy takes a free page, of a
  * sequence that shrinks too; releasing a whole sequence never does. Pages released by a call can be taken by the same
- * call. seqs, new_lens: device int32 [n]. n <= 2048 and at most the workspace's max_batch. */
+ * call. seqs, new_lens: device int32 [n]. n <= 4096 and at most the workspace's max_batch. */
 MOE_API int moe_paged_resize(const moe_paged_cache* c, const int32_t* seqs, const int32_t* new_lens, int n,
                              void* workspace, size_t workspace_bytes, moe_stream_t stream);
 
@@ -111,7 +111,7 @@ MOE_API int moe_paged_copy(const moe_paged_cache* c, const int32_t* src, const i
  * (d, d + rope_dim / 2), d < rope_dim / 2, are rotated by the angle position * inv_freq[d] (fp64 [rope_dim / 2], for
  * this model theta^(-2 d / rope_dim); the angle is formed and reduced in fp64, so far positions keep their accuracy;
  * rope_dim 0 with inv_freq NULL = no rotation). q goes to q_out bf16 [B Tq][Hq D]; k and v go into the pages at the
- * tokens' positions, for e4m3 as x / scale rounded to nearest even and saturated. B <= 2048, B * Tq < 2^24, rope_dim
+ * tokens' positions, for e4m3 as x / scale rounded to nearest even and saturated. B <= 4096, B * Tq < 2^24, rope_dim
  * even and <= D; qkv, q_out and the norms 16-byte aligned. Rows of unused slots and of no token are left as they were. */
 MOE_API int moe_paged_append(const moe_paged_cache* c, int layer, const int32_t* seqs, int B, int Tq,
                              const uint16_t* qkv, int Hq, const uint16_t* q_norm, const uint16_t* k_norm,
@@ -121,7 +121,7 @@ MOE_API int moe_paged_append(const moe_paged_cache* c, int layer, const int32_t*
 /* Causal attention of the new tokens over the cached keys and values of layer `layer`, theirs included: query head h
  * reads kv head h / (Hq / Hkv), softmax(scale q . k) . v in fp32, out bf16 [B Tq][Hq D]. Rows of unused slots, of
  * empty sequences and of no token are zero. What lies in a page behind a sequence's end, and what a token may not see,
- * has no influence, NaN and infinities included. G = Hq / Hkv any whole number with Hq <= 128; Tq <= 8; B <= 2048;
+ * has no influence, NaN and infinities included. G = Hq / Hkv any whole number with Hq <= 128; Tq <= 8; B <= 4096;
  * B Hkv ceil(G Tq / 64) max_pages page at most 2^34 (the work is counted in 32 bits); q, out 16-byte aligned. The
  * batch's work is shared out over the GPU by keys, whatever the lengths, and the parts of a sequence joined in order:
  * the same call gives the same bits. */

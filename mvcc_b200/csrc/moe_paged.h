@@ -12,7 +12,7 @@
 
 namespace moe {
 
-constexpr int kPagedMaxBatch = 2048;   // list entries of one call
+constexpr int kPagedMaxBatch = 4096;   // list entries of one call
 constexpr int kPagedMaxNew = 8;        // new tokens a sequence that the attention takes
 constexpr int kPagedMaxPages = 1 << 20;
 constexpr int kPagedMaxCtas = 320;     // CTAs of the attention grid at most (its partials are sized by it)

@@ -101,8 +101,8 @@ struct Cfg {
   // At least three a key group keep two tiles on their way while one is worked on (two: 15 % less of the bandwidth).
   // A multiple of the producers and of the key groups, so that a ring slot is always filled by one producer and read by
   // one group: barrier waits tell phases apart by parity alone, and two producers on one slot could be two turns apart.
-  static int fixed_bytes(int B) { return 2048 + kMerge + kQueries + (3 * B + 1) * 4; }
-  static int slots(int B) {
+  static constexpr int fixed_bytes(int B) { return 2048 + kMerge + kQueries + (3 * B + 1) * 4; }
+  static constexpr int slots(int B) {
     const int fit = ((kPerSm == 1 ? kSmemOne : kSmemTwo) - fixed_bytes(B)) / kSlot;
     constexpr int kMul = NG > NP ? NG : NP;
     return (fit > kMaxNS ? kMaxNS : fit) / kMul * kMul;
@@ -923,6 +923,7 @@ bool pool_map(CUtensorMap* m, const moe_paged_cache* c, const void* base, int bo
 template <int D, bool F8, int MT>
 cudaError_t launch_attn(const PAttnArgs& args, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t s) {
   using C = Cfg<D, F8, MT>;
+  static_assert(C::slots(kPagedMaxBatch) >= std::max(C::NG, C::NP), "each group and producer has a slot");
   const void* fn = reinterpret_cast<const void*>(paged_attn_kernel<D, F8, MT>);
   static SmemGrant granted;
   PAttnArgs a = args;

@@ -844,22 +844,25 @@ def test_offsets_past_32_bits():
     assert torch.equal(c.k[1, c.tables[0, :3].long()], before)
 
 
-def test_a_batch_of_the_largest_size_over_one_shared_prompt():
-    """2048 slots of 2048 sequences that share one prompt's pages, each with a token of its own."""
-    c = make(layers=1, pages=2100, page=16, Hkv=1, D=128, max_seqs=2048, max_pages=8, Hq=2, max_batch=2048)
+@pytest.mark.parametrize("N,kv,D,Hq", [(2048, "bf16", 128, 2), (4096, "bf16", 128, 4), (4096, "bf16", 64, 2),
+                                       (4096, "e4m3", 256, 2), (4096, "bf16", 256, 64)])
+def test_a_batch_of_the_largest_size_over_one_shared_prompt(N, kv, D, Hq):
+    """N slots of N sequences that share one prompt's pages, each with a token of its own."""
+    c = make(layers=1, pages=N + 52, page=16, Hkv=1, D=D, max_seqs=N, max_pages=8, Hq=Hq, max_batch=N, kv=kv)
     c.resize(i32([0]), i32([100]))
-    rest = list(range(1, 2048))
-    c.fork(i32([0] * 2047), i32(rest))
-    allseq = i32(list(range(2048)))
-    c.resize(allseq, i32([101] * 2048))
-    assert c.error_word() == 0 and c.refs.max() == 2048
-    qkv = bits(torch.randn(2048, 4 * 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)))
-    q, out = torch.zeros(2048, 256, dtype=torch.int16, device="cuda"), torch.zeros(2048, 256, dtype=torch.int16, device="cuda")
+    rest = list(range(1, N))
+    c.fork(i32([0] * (N - 1)), i32(rest))
+    allseq = i32(list(range(N)))
+    c.resize(allseq, i32([101] * N))
+    assert c.error_word() == 0 and c.refs.max() == N
+    g = torch.Generator(device="cuda").manual_seed(3)
+    qkv = bits(torch.randn(N, (Hq + 2) * D, device="cuda", generator=g))
+    q, out = (torch.zeros(N, Hq * D, dtype=torch.int16, device="cuda") for _ in range(2))
     c.append(0, allseq, qkv, q)
     c.attend(0, allseq, q, out)
     assert c.error_word() == 0
-    pick = [0, 1, 7, 1000, 2047]
-    want, tol = attend64(c, 0, pick, q[pick].contiguous(), 1, 128 ** -0.5, "bf16")
+    pick = [0, 1, 7, 1000, N - 1]
+    want, tol = attend64(c, 0, pick, q[pick].contiguous(), 1, D ** -0.5, kv)
     assert bool(((vals(out[pick]) - want).abs() <= tol).all())
 
 

@@ -39,8 +39,8 @@ def test_workspace_bytes():
     c = ctypes.byref(cache())
     assert n(c, 16, 8, 1) > 0 and n(c, 16, 8, 1) % 256 == 0
     assert n(c, 16, 8, 8) >= n(c, 16, 8, 2) >= n(c, 16, 8, 1)
-    assert n(c, 16, 2048, 1) > 0 and n(c, 16, 8, 4096) == n(c, 16, 8, 8)  # long appends need nothing more
-    assert n(c, 15, 8, 1) == 0 and n(c, 130, 8, 1) == 0 and n(c, 16, 0, 1) == 0 and n(c, 16, 2049, 1) == 0
+    assert n(c, 16, 4096, 1) > 0 and n(c, 16, 8, 4096) == n(c, 16, 8, 8)  # long appends need nothing more
+    assert n(c, 15, 8, 1) == 0 and n(c, 130, 8, 1) == 0 and n(c, 16, 0, 1) == 0 and n(c, 16, 4097, 1) == 0
     assert n(c, 16, 8, 0) == 0 and n(ctypes.byref(cache(D=100)), 16, 8, 1) == 0
     s = lib().moe_spec_workspace_bytes
     assert s(1, 151936) > 0 and s(64, 151936) > s(1, 151936)
@@ -61,8 +61,8 @@ def test_page_calls_refuse_before_launch():
         assert call(bad, PTR, PTR, 4, ws, big, None) == BAD
         assert call(None, PTR, PTR, 4, ws, big, None) == BAD
         assert call(c, None, None, 0, ws, big, None) == 0            # an empty list: nothing to do
-    assert L.moe_paged_resize(c, PTR, PTR, 2049, ws, big, None) == BAD
-    assert L.moe_paged_fork(c, PTR, PTR, 2049, ws, big, None) == BAD
+    assert L.moe_paged_resize(c, PTR, PTR, 4097, ws, big, None) == BAD
+    assert L.moe_paged_fork(c, PTR, PTR, 4097, ws, big, None) == BAD
     assert L.moe_paged_compact(c, ws, 256, None) == BAD and L.moe_paged_compact(bad, ws, big, None) == BAD
 
 
@@ -78,12 +78,12 @@ def test_attention_calls_refuse_before_launch():
 
     for call in (append, attend):
         assert call(B=0) == 0
-        for kw in ({"layer": 2}, {"layer": -1}, {"seqs": None}, {"B": -1}, {"B": 2049}, {"Tq": 0}, {"Hq": 15},
+        for kw in ({"layer": 2}, {"layer": -1}, {"seqs": None}, {"B": -1}, {"B": 4097}, {"Tq": 0}, {"Hq": 15},
                    {"Hq": 0}, {"Hq": 130}, {"q": None}, {"q": PTR + 2}, {"ws": None}, {"ws": PTR + 4}, {"n": 256},
                    {"cc": None}, {"cc": ctypes.byref(cache(D=80))}):
             assert call(**kw) == BAD, kw
     for kw in ({"qn": None}, {"kn": None}, {"rope": 0}, {"f": None}, {"rope": 7}, {"rope": 258}, {"rope": -2},
-               {"qkv": None}, {"qkv": PTR + 8}, {"B": 2048, "Tq": 1 << 13}):
+               {"qkv": None}, {"qkv": PTR + 8}, {"B": 4096, "Tq": 1 << 12}):
         assert append(**kw) == BAD, kw
     for kw in ({"Tq": 9}, {"out": None}, {"out": PTR + 8}):
         assert attend(**kw) == BAD, kw
