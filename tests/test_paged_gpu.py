@@ -500,6 +500,16 @@ def test_attention_scores_of_any_size():
         assert bool(((vals(out) - want).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("D,Hq,Tq", [(128, 4, 1), (128, 8, 3), (256, 4, 3), (256, 16, 8)])
+def test_attention_over_8_bits_with_scores_too_small_to_tell(D, Hq, Tq):
+    """A scale of zero with tiny queries, and queries of zero with tiny key scales: equal scores, so a row is the mean of
+    the values that it sees, whatever the factors' product comes to in fp32."""
+    c = filled([130, 9, 2, 33], Hq=Hq, Hkv=2, D=D, page=16, kv="e4m3", Tq=Tq,
+               k_scale=torch.full((1, 2), 1e-9, device="cuda"), v_scale=torch.full((1, 2), 0.03, device="cuda"))
+    for std, scale in ((0.0, None), (2.0 ** -30, 0.0), (2.0, 0.0), (2.0 ** -126, 1e-3)):
+        check_attend(c, [2, 0, 3, 1], Tq, "e4m3", scale=scale, q=queries(c, 4, Tq, std=std))
+
+
 @pytest.mark.parametrize("kv,D,Tq", [("bf16", 64, 1), ("bf16", 128, 4), ("bf16", 256, 1), ("e4m3", 128, 2), ("e4m3", 256, 3)])
 def test_attention_of_scores_that_climb_and_fall(kv, D, Tq):
     """Scores that rise over 2000 keys by 50 powers of two, evenly, in steps, or falling: the running maximum moves in
