@@ -21,17 +21,17 @@
 // fragments and takes every NG-th tile: S = Q K^T, the running maximum and sum of the softmax, O += P V, all in
 // registers; at a job's end the NG warps of a row tile merge through shared memory.
 //
-// mma.sync and not tcgen05: with 16 to 64 rows a tcgen05.mma (at least 64 rows of the cache as M, and P through TMEM)
-// would leave its tensor core as idle as the register MMA does, and add two TMEM round trips to the softmax of each
-// tile; at 16 rows the register MMA needs under a third of the cycles that the tile's bytes take to arrive.
+// mma.sync and not tcgen05: at 16 rows the register MMA needs under a half of the cycles that a tile's bytes take to
+// arrive, so a tcgen05.mma (at least 64 rows of the cache as M, and P through TMEM) would only add two TMEM round trips to
+// the softmax of each tile. At 64 rows that no longer holds: there the register MMAs bound the call.
 //
 // Measured on a B200 (16 query and 2 kv heads of 256, bf16, unless said otherwise; the device copy moves 6.45 TB/s): one
-// sequence of 131071 keys 52 us (5.2 TB/s), 48 ragged sequences of up to 8192 keys 70 us (5.4 TB/s), with 4 and 8 new
-// tokens each 81 and 126 us; 24 sequences of up to 16000 keys, 32 over 8 heads of 128, 4 tokens: 123 us in bf16
-// (5.9 TB/s), 75 us in e4m3 with pages of 16 (4.8 TB/s). The loop over the tiles runs at the read bandwidth for bf16 and
+// sequence of 131071 keys 51 us (5.3 TB/s), 48 ragged sequences of up to 8192 keys 68 us (5.5 TB/s), with 4 and 8 new
+// tokens each 83 and 146 us; 24 sequences of up to 16000 keys, 32 over 8 heads of 128, 4 tokens: 123 us in bf16
+// (5.9 TB/s), 69 us in e4m3 with pages of 16 (5.2 TB/s). The loop over the tiles runs at the read bandwidth for bf16 and
 // one row tile; around it lie 2 us for the units, 1.5 us for the first queries and pages, 2 us for the last merge, 1 to
-// 4 us for the slowest CTA and 3 us for the join. With e4m3 or several row tiles the consumers' latency a tile (2000
-// cycles, two warps a scheduler) bounds it.
+// 4 us for the slowest CTA and 3 us for the join. With e4m3 the consumers' latency a tile (2000 cycles, two warps a
+// scheduler) bounds it, with four row tiles their products, and the k and v fragments that every row tile loads again.
 #include <algorithm>
 #include <cstring>
 #include <mutex>
@@ -589,16 +589,29 @@ __global__ void __launch_bounds__(Cfg<D, F8, MT>::kThreads, Cfg<D, F8, MT>::kPer
           mB = nB;
         }
         const float zA = mA == -INFINITY ? 0.f : mA * fA, zB = mB == -INFINITY ? 0.f : mB * fB;
-        // P in the cache's MMA type; the sums take the rounded weights, so that a row's weights still add up to one
-        uint32_t pf[KT / 16][4];
+        // P in the cache's MMA type; the sums take the same weights, so that a row's still add up to one. f16 keeps 11 bits
+        // of a weight, finer than the output. bf16 keeps 8, as few as the output, which would show in rows whose values
+        // nearly cancel (the error's mean square over 48 ragged sequences 1.35 times that of the output's rounding alone):
+        // what it leaves over goes into a second operand and a second product, 16 bits together. Up to 16 rows a kv head
+        // that costs nothing (48 sequences: 68.1 against 69.0 us), with four tokens 83.0 against 81.0, with eight, where
+        // the products bound the call, 146 against 126.
+        uint32_t pf[KT / 16][4], pr[F8 ? 1 : KT / 16][4];
         const float yA = kLift - zA, yB = kLift - zB;
+        auto weights = [&](int j, int e, float x, float y) {
+          const uint32_t w = pack2<F8>(x, y);
+          pf[j >> 1][(j & 1) * 2 + e] = w;
+          if constexpr (!F8) pr[j >> 1][(j & 1) * 2 + e] = pack2<false>(x - lo_bf(w), y - hi_bf(w));
+        };
 #pragma unroll
         for (int j = 0; j < KT / 8; ++j) {
-          pf[j >> 1][(j & 1) * 2] = pack2<F8>(ex2(fmaf(s[j][0], fA, yA)), ex2(fmaf(s[j][1], fA, yA)));
-          pf[j >> 1][(j & 1) * 2 + 1] = pack2<F8>(ex2(fmaf(s[j][2], fB, yB)), ex2(fmaf(s[j][3], fB, yB)));
+          weights(j, 0, ex2(fmaf(s[j][0], fA, yA)), ex2(fmaf(s[j][1], fA, yA)));
+          weights(j, 1, ex2(fmaf(s[j][2], fB, yB)), ex2(fmaf(s[j][3], fB, yB)));
         }
 #pragma unroll
-        for (int ks = 0; ks < KT / 16; ++ks) mma16816<F8>(lsum, pf[ks], kOnes, kOnes);
+        for (int ks = 0; ks < KT / 16; ++ks) {
+          mma16816<F8>(lsum, pf[ks], kOnes, kOnes);
+          if constexpr (!F8) mma16816<false>(lsum, pr[ks], kOnes, kOnes);
+        }
         // O += P V. B fragments of the 16 keys from key0 + 16 ks, the columns of chunk pair c
         auto pv = [&](auto&& keep, auto&& add) {
 #pragma unroll
@@ -612,6 +625,8 @@ __global__ void __launch_bounds__(Cfg<D, F8, MT>::kThreads, Cfg<D, F8, MT>::kPer
               if constexpr (!F8) {
                 add(acc[c], pf[ks], vf[0], vf[1]);
                 add(acc[c + 1], pf[ks], vf[2], vf[3]);
+                add(acc[c], pr[ks], vf[0], vf[1]);
+                add(acc[c + 1], pr[ks], vf[2], vf[3]);
               } else {
                 // a 16-bit unit holds two columns of one key: even columns to one MMA, odd ones to the next
 #pragma unroll

@@ -500,6 +500,30 @@ def test_attention_scores_of_any_size():
         assert bool(((vals(out) - want).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("D,Hq,Tq", [(64, 4, 1), (64, 16, 3), (128, 8, 1), (128, 32, 4), (256, 16, 1), (256, 16, 4), (256, 16, 8)])
+def test_attention_keeps_more_of_a_weight_than_its_output_shows(D, Hq, Tq):
+    """Rows of values that nearly cancel, where a weight of 8 bits would show: within the output's rounding (2^-8 of it) and
+    2^-16 of sum p |v| for the weights' two bf16 parts, beside what attend64 allows for the scores and the sums in fp32."""
+    lens = [9, 17, 24, 40, 57]
+    c = filled(lens, Hq=Hq, Hkv=2, D=D, page=16, Tq=Tq)
+    B, G = len(lens), Hq // 2
+    q = queries(c, B, Tq, std=0.25)
+    out = torch.zeros_like(q)
+    c.attend(0, i32(list(range(B))), q, out, Tq=Tq)
+    got, qq = vals(out).view(B, Tq, Hq, D), vals(q).view(B, Tq, Hq, D)
+    for b, n in enumerate(lens):
+        ids = c.tables[b, :-(-n // 16)].long()
+        for t in range(Tq):
+            m = n - Tq + t + 1
+            for h in range(Hq):
+                k, v = (vals(x[0, ids, h // G]).reshape(-1, D)[:m] for x in (c.k, c.v))
+                p = torch.softmax(k @ qq[b, t, h] * D ** -0.5, 0)
+                o, mag = p @ v, p @ v.abs()
+                ds = (D + 4) * F32 * float((k.abs() @ qq[b, t, h].abs()).max()) * D ** -0.5 + 2.0 ** -20
+                tol = BF * o.abs() + (2.0 ** -16 + 2 * ds + 72 * F32) * (mag + o.abs())
+                assert bool(((got[b, t, h] - o).abs() <= tol).all()), (b, t, h)
+
+
 @pytest.mark.parametrize("D,Hq,Tq", [(128, 4, 1), (128, 8, 3), (256, 4, 3), (256, 16, 8)])
 def test_attention_over_8_bits_with_scores_too_small_to_tell(D, Hq, Tq):
     """A scale of zero with tiny queries, and queries of zero with tiny key scales: equal scores, so a row is the mean of
