@@ -500,6 +500,28 @@ def test_attention_scores_of_any_size():
         assert bool(((vals(out) - want).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("D,Hq,Tq", [(64, 4, 1), (128, 8, 2), (256, 4, 1), (256, 16, 4)])
+def test_attention_of_values_near_the_largest_of_their_type(D, Hq, Tq):
+    """Even scores, and one key late in the sequence a few powers of two above them whose value is 3e38: the mean is finite,
+    and so is every sum of p v with p relative to the row's largest weight."""
+    n, at, B = 600, 400, 400  # enough sequences that one warp meets a sequence's even keys before the high one
+    for up in (1.0, 2.5, 3.5, 3.9, 4.5):
+        c = filled([n] + [0] * (B - 1), Hq=Hq, Hkv=2, D=D, page=16, Tq=Tq)
+        c.tables[1:] = c.tables[0]
+        c.lens[:] = n
+        pid = int(c.tables[0, at // 16])
+        c.k.zero_()
+        c.k.view(torch.bfloat16)[0, pid, :, at % 16, 0] = up / math.log2(math.e)
+        c.v.view(torch.bfloat16)[0, pid, :, at % 16] = 3e38
+        q = torch.zeros(B * Tq * Hq, D, device="cuda")
+        q[:, 0] = 1.0
+        q = bits(q).view(B * Tq, -1)
+        out = torch.zeros_like(q)
+        c.attend(0, i32(list(range(B))), q, out, Tq=Tq, scale=1.0)
+        want, tol = attend64(c, 0, [0], q[:Tq], Tq, 1.0, "bf16")
+        assert bool(((vals(out).view(B, Tq, -1) - want).abs() <= tol).all())
+
+
 @pytest.mark.parametrize("D,Hq,Tq", [(64, 4, 1), (64, 16, 3), (128, 8, 1), (128, 32, 4), (256, 16, 1), (256, 16, 4), (256, 16, 8)])
 def test_attention_keeps_more_of_a_weight_than_its_output_shows(D, Hq, Tq):
     """Rows of values that nearly cancel, where a weight of 8 bits would show: within the output's rounding (2^-8 of it) and
