@@ -65,8 +65,11 @@ __device__ __forceinline__ void store_peer(float* p, uint32_t rank, float v) {
                "r"(rank), "f"(v)
                : "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_arrive();
+  cluster_wait();
 }
 
 // log2(e) / t, but never zero: at an infinite temperature a logit of -infinity keeps its weight of zero.
@@ -89,6 +92,7 @@ __global__ void __launch_bounds__(kSmThreads, VEC == 4 ? 2 : 1) softmax_rows_ker
   __shared__ float peer[3][kSmMaxCluster];  // of each CTA of the row: maximum, sum, index of the maximum
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int CL = (int)cluster_size(), rank = (int)cluster_rank();
+  cluster_arrive();  // a CTA's shared memory may be written by the others once it has started: waited for before they do
   pdl_wait();
   pdl_launch_dependents();
   const int64_t row = blockIdx.x / CL;
@@ -174,6 +178,7 @@ __global__ void __launch_bounds__(kSmThreads, VEC == 4 ? 2 : 1) softmax_rows_ker
     const float v = __shfl_xor_sync(0xffffffffu, s, o);
     s = greedy ? fminf(s, v) : s + v;
   }
+  cluster_wait();  // every CTA of the cluster has started
   if (tid < CL) {
     store_peer(&peer[0][rank], tid, m);
     store_peer(&peer[1][rank], tid, s);
@@ -232,6 +237,7 @@ __global__ void __launch_bounds__(kSmThreads, N <= 10 ? 2 : 1) softmax_ring_kern
   const int first = blockIdx.x / CL, step = gridDim.x / CL;
   const int chunk = ((a.V + CL - 1) / CL + 3) & ~3;
   const int b0 = min(a.V, rank * chunk), n = min(a.V, b0 + chunk) - b0;
+  cluster_arrive();
   if (tid == 0) {
     mbar_init(&full, 1);
     mbar_fence_init();
@@ -317,6 +323,7 @@ __global__ void __launch_bounds__(kSmThreads, N <= 10 ? 2 : 1) softmax_ring_kern
       s = greedy ? fminf(s, v) : s + v;
     }
     float(*pr)[kSmMaxCluster] = peer[turn & 1];
+    if (turn == 0) cluster_wait();  // every CTA of the cluster has started
     if (tid < CL) {
       store_peer(&pr[0][rank], tid, m);
       store_peer(&pr[1][rank], tid, s);

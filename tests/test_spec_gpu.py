@@ -122,6 +122,28 @@ def test_softmax_at_an_infinite_temperature_shares_equally(V):
     assert bool(((out.double() - want).abs() <= 2.0 ** -20 * want).all())
 
 
+@pytest.mark.parametrize("R,V", [(64, 40961), (16, 151936), (2, 20484), (300, 163844), (3, 270000)])
+def test_softmax_of_clusters_that_start_beside_other_work(R, V):
+    """Rows shared by clusters of 2 to 8 CTAs, launched back to back on two streams beside a kernel that keeps the GPU's
+    places busy, so that a cluster's CTAs start as room comes: the same bits every time."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = 3 * torch.randn(R, V, generator=g, device="cuda")
+    want = torch.empty_like(x)
+    S().softmax_rows(x, want)
+    near(want, x, torch.ones(R, device="cuda"))
+    busy = torch.randn(2048, 2048, device="cuda")
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = [torch.full_like(x, 9.0) for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        with torch.cuda.stream(streams[2]):
+            torch.mm(busy, busy)
+        for out, s in zip(outs, streams):
+            S().softmax_rows(x, out, stream=s)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
 def test_softmax_keeps_what_lies_between_rows():
     x = torch.randn(6, 1000, device="cuda")
     y = torch.full((6, 1003), 5.0, device="cuda")
