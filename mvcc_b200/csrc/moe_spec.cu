@@ -232,6 +232,7 @@ __global__ void __launch_bounds__(kSmThreads, N <= 10 ? 2 : 1) softmax_ring_kern
   __shared__ __align__(8) uint64_t full;
   __shared__ float red[2][kSmWarps];
   __shared__ float peer[2][2][kSmMaxCluster];  // by row parity: maxima and sums (or indices) of the row's CTAs
+  __shared__ int broken;  // a wait for a copy gave up: this row and those after it are no numbers
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int CL = (int)cluster_size(), rank = (int)cluster_rank();
   const int first = blockIdx.x / CL, step = gridDim.x / CL;
@@ -239,14 +240,17 @@ __global__ void __launch_bounds__(kSmThreads, N <= 10 ? 2 : 1) softmax_ring_kern
   const int b0 = min(a.V, rank * chunk), n = min(a.V, b0 + chunk) - b0;
   cluster_arrive();
   if (tid == 0) {
+    broken = 0;
     mbar_init(&full, 1);
     mbar_fence_init();
   }
   __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
-  auto fetch = [&](int64_t row) {  // one thread
+  int issued = 0;  // copies that thread 0 has started
+  auto fetch = [&](int64_t row) {  // thread 0
     if (row >= a.R || n == 0) return;
+    ++issued;
     const float* src = a.x + row * a.ldx + b0;
     expect_tx(&full, span_bytes(src, n * 4));
     bulk_span(smem, src, n * 4, &full);
@@ -282,8 +286,9 @@ __global__ void __launch_bounds__(kSmThreads, N <= 10 ? 2 : 1) softmax_ring_kern
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) red[0][warp] = m;
+    if (!ok) broken = 1;
     __syncthreads();  // the buffer has been read
-    if (tid == 0 && ok) fetch((int64_t)row + step);
+    if (tid == 0 && !broken) fetch((int64_t)row + step);
     __syncwarp();
     m = red[0][lane & (kSmWarps - 1)];
 #pragma unroll
@@ -325,8 +330,9 @@ __global__ void __launch_bounds__(kSmThreads, N <= 10 ? 2 : 1) softmax_ring_kern
     float(*pr)[kSmMaxCluster] = peer[turn & 1];
     if (turn == 0) cluster_wait();  // every CTA of the cluster has started
     if (tid < CL) {
-      store_peer(&pr[0][rank], tid, m);
-      store_peer(&pr[1][rank], tid, s);
+      // a copy that never came: a maximum that takes part everywhere, and a sum (or index) that is no number
+      store_peer(&pr[0][rank], tid, broken ? INFINITY : m);
+      store_peer(&pr[1][rank], tid, broken ? __int_as_float(0x7fc00000) : s);
     }
     cluster_sync();  // the other parity's values are written again only after the next row's barrier
     float M = -INFINITY;
@@ -340,13 +346,14 @@ __global__ void __launch_bounds__(kSmThreads, N <= 10 ? 2 : 1) softmax_ring_kern
         if (pr[0][k] != -INFINITY) total += pr[1][k] * soft_weight_any(pr[0][k], M, c);
       f = M == -INFINITY || m == -INFINITY ? 0.f : soft_weight_any(m, M, c) / total;
     } else {
+      float index = -1.f;
       for (int k = CL - 1; k >= 0; --k)
-        if (pr[0][k] == M && M != -INFINITY) at = (int)pr[1][k] - b0;
+        if (pr[0][k] == M && M != -INFINITY) index = pr[1][k];
+      f = index == index ? 1.f : index;
+      at = (int)index - b0;
 #pragma unroll
       for (int k = 0; k < N * 4; ++k) r[k] = (k / VEC * kSmThreads + tid) * VEC + k % VEC == at ? 1.f : 0.f;
-      f = 1.f;
     }
-    if (!ok) f = __int_as_float(0x7fc00000);  // the copy never came: the row and those after it are no numbers, and say so
 #pragma unroll
     for (int k = 0; k < N * 4 / VEC; ++k) {
       const int i = (k * kSmThreads + tid) * VEC;
@@ -358,7 +365,7 @@ __global__ void __launch_bounds__(kSmThreads, N <= 10 ? 2 : 1) softmax_ring_kern
       }
     }
   }
-  if (!ok && tid == 0) bar_wait(&full, (turn - 1) & 1);  // no copy may still be landing when the CTA exits
+  if (tid == 0 && issued > 0) bar_wait(&full, (issued - 1) & 1);  // the last copy may still be landing, if a wait gave up
 }
 
 template <int VEC, int N>
