@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <mutex>
 
 #include "../../include/moe_block.h"
 
@@ -168,15 +169,20 @@ inline cudaError_t launched(cudaError_t e) {
 // launches there (including those inside CUDA-graph capture) make no attribute call. Kernel attributes belong to
 // each device's context, so what was granted is recorded per device: a process that drives several GPUs raises each
 // kernel's limit on each of them. One SmemGrant per kernel instantiation, as a function-local static (zero at start).
+// Requests of different sizes from several host threads take turns: an attribute set to less after one set to more would
+// leave the record above the attribute, and every later launch in between would fail.
 struct SmemGrant {
   static constexpr int kDevices = 64;
   std::atomic<size_t> dev[kDevices];
+  std::mutex turn;
 };
 inline cudaError_t grant_smem(const void* kern, size_t bytes, size_t floor_bytes, SmemGrant& g) {
   int d = 0;
   cudaError_t e = cudaGetDevice(&d);
   if (e != cudaSuccess) return e;
   const bool kept = d >= 0 && d < SmemGrant::kDevices;  // devices past the table are raised on every launch
+  if (kept && bytes <= g.dev[d].load(std::memory_order_relaxed)) return cudaSuccess;
+  std::lock_guard<std::mutex> lock(g.turn);
   if (kept && bytes <= g.dev[d].load(std::memory_order_relaxed)) return cudaSuccess;
   const size_t want = bytes > floor_bytes ? bytes : floor_bytes;
   e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)want);

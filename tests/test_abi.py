@@ -215,3 +215,15 @@ def test_tensor_stats_follow_the_reference_debug_report():
     b = torch.tensor([0.5, -0.25], dtype=torch.bfloat16).view(torch.int16)
     sb = mvcc_b200.tensor_stats(b)
     assert sb["absmax"] == 0.5 and sb["mean"] == 0.125 and sb["nonfinite"] == 0
+
+
+def test_shared_memory_grants_of_two_threads_keep_the_larger(tmp_path):
+    """Two host threads that raise one kernel's shared-memory limit at once, by different sizes, leave the larger."""
+    import subprocess
+    exe = str(tmp_path / "smem_grant")
+    cmd = [os.environ.get("NVCC", "nvcc"), "-std=c++17", "-O1", "-x", "cu", "-gencode", "arch=compute_100a,code=sm_100a",
+           os.path.join(ROOT, "tests", "cpp", "smem_grant.cpp"), "-o", exe, "-lpthread"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    run = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert run.returncode == 0, run.stdout
