@@ -25,6 +25,16 @@ inline int paged_block_rows(int G, int Tq) {
   return m <= 16 ? 16 : (m <= 32 ? 32 : 64);
 }
 
+// Units of work that a job of the attention counts beside its units of unit_keys keys (moe_paged_attn.cu).
+constexpr int setup_units(int unit_keys) { return unit_keys >= 64 ? 5 : 9; }
+
+// The attention counts its flattened list of units in 32 bits; a unit is at least 16 keys.
+inline bool paged_work_fits(const moe_paged_cache* c, int Hq, int B, int Tq) {
+  const int G = Hq / c->Hkv, rows = paged_block_rows(G, Tq), blocks = (G * Tq + rows - 1) / rows;
+  const int64_t units = ((int64_t)c->max_pages * c->page + 15) / 16 + setup_units(16);
+  return B * units * c->Hkv * blocks < ((int64_t)1 << 31) - kPagedMaxCtas;
+}
+
 // Offsets (bytes) of the caller-owned workspace's sections, each 256-byte aligned. The error word leads; what the page
 // calls and the attention keep shares the space behind it, since one workspace serves one call at a time.
 struct PagedWs {

@@ -201,8 +201,7 @@ enum { JOIN_PARTS = 0, JOIN_FIRST, JOIN_SECOND, JOIN_SLOT, JOIN_HEAD, JOIN_BLOCK
 
 // The share of one CTA: [u, end) of the flattened list, walked job by job. A job counts kSetup units of its own before
 // its units of keys: its queries, its first tile's latency and its merge cost a CTA about as much, and a batch with
-// many short sequences would otherwise pile them up in a few CTAs.
-constexpr int setup_units(int unit_keys) { return unit_keys >= 64 ? 5 : 9; }
+// many short sequences would otherwise pile them up in a few CTAs. (setup_units, moe_paged.h)
 template <int kSetup>
 struct Walk {
   int u, end;           // what is left of the share
@@ -976,7 +975,7 @@ extern "C" {
 int moe_paged_attend(const moe_paged_cache* c, int layer, const int32_t* seqs, int B, int Tq, const uint16_t* q, int Hq,
                      float scale, uint16_t* out, void* workspace, size_t workspace_bytes, moe_stream_t stream) {
   if (!paged_ok(c) || layer < 0 || layer >= c->layers || B < 0 || B > kPagedMaxBatch || Tq < 1 || Tq > kPagedMaxNew ||
-      Hq < 1 || Hq > 128 || Hq % c->Hkv != 0 || !workspace || !paged_al16(workspace))
+      Hq < 1 || Hq > 128 || Hq % c->Hkv != 0 || !workspace || !paged_al16(workspace) || !paged_work_fits(c, Hq, B, Tq))
     return (int)cudaErrorInvalidValue;
   if (B == 0) return (int)cudaSuccess;
   if (!seqs || !q || !out || !paged_al16(q) || !paged_al16(out)) return (int)cudaErrorInvalidValue;
@@ -1009,9 +1008,6 @@ int moe_paged_attend(const moe_paged_cache* c, int layer, const int32_t* seqs, i
   a.scale = scale;
   a.inv_G = 1.f / (float)a.G;
   a.ctas = 0;
-  // the flattened unit list is counted in 32 bits; a unit is at least 16 keys
-  const int64_t units = ((int64_t)c->max_pages * c->page + 15) / 16 + setup_units(16);
-  if (B * units * c->Hkv * a.row_blocks >= ((int64_t)1 << 31) - kPagedMaxCtas) return (int)cudaErrorInvalidValue;
   const int kt = tile_keys(c->D * kv_size(c->kv_type));
   a.box_rows = c->page % kt == 0 ? kt : 16;
   CUtensorMap mk, mv;

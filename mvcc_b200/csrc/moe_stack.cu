@@ -829,8 +829,11 @@ int moe_attn_paged_forward_rms(const moe_attn_weights* w, const uint16_t* rms1, 
                                const moe_paged_cache* c, int layer, const int32_t* seqs, int B, int Tq,
                                const double* inv_freq, uint16_t* attn_out, void* workspace, size_t workspace_bytes,
                                moe_stream_t stream) {
-  if (!attn_paged_ok(w, c, B, Tq) || !paged_ok(c) || layer < 0 || layer >= c->layers || !rms1 || !hidden || !seqs || !inv_freq || !attn_out || !workspace ||
-      !al16(rms1) || !al16(hidden) || !al16(workspace) || !al16(w->qkv) || !al16(w->o) || (w->gate && !al16(w->gate)))
+  // every check of the append and the attention too: once the first projection is launched nothing is refused
+  if (!attn_paged_ok(w, c, B, Tq) || !paged_ok(c) || layer < 0 || layer >= c->layers || !rms1 || !hidden || !seqs ||
+      !inv_freq || !attn_out || !workspace || !al16(rms1) || !al16(hidden) || !al16(workspace) || !al16(w->qkv) ||
+      !al16(w->o) || (w->gate && !al16(w->gate)) || !al16(w->q_norm) || !al16(w->k_norm) ||
+      !paged_work_fits(c, w->Hq, B, Tq))
     return (int)cudaErrorInvalidValue;
   const AttnPagedWs L = attn_paged_ws(w, c, B, Tq);
   if (workspace_bytes < L.total) return (int)cudaErrorInvalidValue;

@@ -110,6 +110,22 @@ def test_layer_call_refuses_before_launch():
         assert call(**kw) == BAD, kw
 
 
+@pytest.mark.parametrize("what", ["work", "q_norm", "k_norm"])
+def test_layer_call_refuses_what_its_parts_would_before_any_launch(what):
+    """A batch whose key units pass 32 bits (the attention's limit) and a misaligned norm (the append's): refused at once,
+    not after the projections."""
+    import mvcc_b200 as m
+    L, big = lib(), 1 << 40
+    w = m.MoeAttnWeights(PTR, None, PTR, PTR, PTR, 2048, 32, 32, 256, 64, 1e7, 1e-6)
+    if what != "work":
+        setattr(w, what, PTR + 8)
+    cc = cache(Hkv=32, **({"max_pages": 1 << 13, "page": 64} if what == "work" else {}))
+    m.reset_stats()
+    assert L.moe_attn_paged_forward_rms(ctypes.byref(w), PTR, PTR, ctypes.byref(cc), 0, PTR, 4096, 1, PTR, PTR, PTR, big,
+                                        None) == BAD
+    assert m.stats()["launches"] == 0
+
+
 def test_spec_calls_refuse_before_launch():
     L, big = lib(), 1 << 40
 
