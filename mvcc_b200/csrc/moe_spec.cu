@@ -462,9 +462,14 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
 }
 
 // A non-negative finite fp32 as fp64, by moving its fields (a conversion instruction has an eighth of the rate). Zero
-// becomes 2^-127 and subnormals are off by less than that: the weights below are differences of two such values, in
-// which equal ones cancel exactly and the rest is far below what a sum of probabilities holds.
+// becomes 2^-127 and values below 2^-126 are off by less than that. The weights below are differences of two such values:
+// equal ones cancel exactly, and a row's sum is off by less than 2^24 2^-126, which 53 bits do not show unless the sum
+// itself is below kTiny. Such a row is weighed again by conversion (18.9 us for 64 x 4 drafts; with the small values put
+// right in every weight, 26.8).
+constexpr double kTiny = 0x1p-40;
+template <bool EXACT>
 __device__ __forceinline__ double widen(float v) {
+  if (EXACT) return (double)v;
   const uint32_t u = __float_as_uint(v);
   return __hiloint2double((int)((u >> 3) + 0x38000000u), (int)(u << 29));
 }
@@ -475,12 +480,13 @@ struct Weights {
   const float* p;
   const float* q;  // null: q is zero but for `hit`, where it is one
   int hit;
+  template <bool EXACT>
   __device__ __forceinline__ void of(int i, const float4& pv, const float4& qv, double (&w)[4]) const {
     const float a[4] = {pv.x, pv.y, pv.z, pv.w}, b[4] = {qv.x, qv.y, qv.z, qv.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const float y = q ? prob(b[k]) : (i + k == hit ? 1.f : 0.f);
-      w[k] = widen(fmaxf(prob(a[k]), y)) - widen(y);
+      w[k] = widen<EXACT>(fmaxf(prob(a[k]), y)) - widen<EXACT>(y);
     }
   }
 };
@@ -501,9 +507,22 @@ __device__ double stretch_sum(const Weights& W, int i0, int i1, int V, int lane)
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       double w[4];
-      W.of(base + u * 128 + lane * 4, p[u], q[u], w);
+      W.of<false>(base + u * 128 + lane * 4, p[u], q[u], w);
       s += (w[0] + w[1]) + (w[2] + w[3]);
     }
+  }
+  return warp_sum_f64(s);
+}
+
+// The same by conversion, for rows whose sum is tiny: out of line, so that its instructions are not among those of the rest.
+template <bool VEC>
+__device__ __noinline__ double stretch_sum_exact(const Weights& W, int i0, int i1, int V, int lane) {
+  double s = 0.0;
+#pragma unroll 1
+  for (int i = i0 + lane * 4; i < i1; i += 128) {
+    double w[4];
+    W.of<true>(i, load_probs<VEC>(W.p, i, V), W.q ? load_probs<VEC>(W.q, i, V) : make_float4(0.f, 0.f, 0.f, 0.f), w);
+    s += (w[0] + w[1]) + (w[2] + w[3]);
   }
   return warp_sum_f64(s);
 }
@@ -512,7 +531,7 @@ template <bool VEC>
 __global__ void __launch_bounds__(kVfThreads) verify_kernel(const __grid_constant__ VerifyArgs a) {
   __shared__ double wsum[kVfWarps];
   __shared__ int last, found, stretch_s, some_s;
-  __shared__ double base_s, target_s;
+  __shared__ double base_s, target_s, total_s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.y, K = a.K;
   pdl_wait();
   pdl_launch_dependents();
@@ -605,21 +624,31 @@ __global__ void __launch_bounds__(kVfThreads) verify_kernel(const __grid_constan
     if (pick >= k0 && pick < k1) base_s = none ? some_base : hit_base;
     if (tid == 0) {
       target_s = target;
+      total_s = total;
       found = 0x7fffffff;
     }
     __syncthreads();
     return pick;
   };
-  int stretch = choose();
-  if (stretch < 0 && rejected) {  // no residual anywhere: the row itself
-    W.q = nullptr;
-    W.hit = -1;
+  int stretch;
+  bool exact = false, residual = rejected;
+  while (true) {
+    stretch = choose();
+    if (stretch < 0 && residual) {  // no residual anywhere: the row itself
+      residual = false;
+      W.q = nullptr;
+      W.hit = -1;
+    } else if (stretch >= 0 && total_s < kTiny && !exact) {
+      exact = true;
+    } else {
+      break;
+    }
     for (int k = warp; k < a.stretches; k += kVfWarps) {
-      const double s = stretch_sum<VEC>(W, k * a.stretch, min(a.V, (k + 1) * a.stretch), a.V, lane);
+      const int i0 = k * a.stretch, i1 = min(a.V, i0 + a.stretch);
+      const double s = exact ? stretch_sum_exact<VEC>(W, i0, i1, a.V, lane) : stretch_sum<VEC>(W, i0, i1, a.V, lane);
       if (lane == 0) __stcg(sums + k, s);
     }
     __syncthreads();
-    stretch = choose();
   }
   int token = -1;
   if (stretch >= 0) {
@@ -633,7 +662,8 @@ __global__ void __launch_bounds__(kVfThreads) verify_kernel(const __grid_constan
       if (i < end) {
         const float4 p = load_probs<VEC>(W.p, i, a.V);
         const float4 q = W.q ? load_probs<VEC>(W.q, i, a.V) : make_float4(0.f, 0.f, 0.f, 0.f);
-        W.of(i, p, q, w);
+        if (exact) W.of<true>(i, p, q, w);
+        else W.of<false>(i, p, q, w);
       }
       const double mine = (w[0] + w[1]) + (w[2] + w[3]);
       double run = mine;

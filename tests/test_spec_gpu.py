@@ -218,6 +218,14 @@ def compare(p, q, x, u, n=None, ver=None, least=0.9):
     return tok, acc
 
 
+def Draw(B, V):
+    """A verifier that draws without drafts, called as one with drafts is."""
+    ver = S().SpecVerifier(B, 0, V)
+    verify = ver.verify
+    ver.verify = lambda p, q, x, u, tok, acc, n_drafted=None: verify(p, None, None, u, tok, acc)
+    return ver
+
+
 def drafts(B, K, V, seed, noise=0.7):
     g = torch.Generator(device="cuda").manual_seed(seed)
     z = 2 * torch.randn(B, K + 1, V, generator=g, device="cuda")
@@ -284,6 +292,21 @@ def test_verify_at_borders_and_with_bad_values():
     assert tok[7].tolist() == [-1, -1, -1] and tok[8].tolist() == [9999, -1, -1]
     assert tok[2, 0] == 4002 and tok[3].tolist() == [4001, 4002, -1] and tok[4, 0] == 4002
     assert tok[5, 0] in (4000, 4002, 4003) and tok[9, 2] == 4001
+
+
+@pytest.mark.parametrize("V", [8, 1001, 40000])
+def test_verify_of_probabilities_below_the_normal_range(V):
+    """Rows whose entries are all tiny, normal and subnormal ones together: weights and their sums as fp64 holds them."""
+    B, K = 64, 1
+    g = torch.Generator(device="cuda").manual_seed(V)
+    p = torch.rand(B, K + 1, V, generator=g, device="cuda") * 2.0 ** -125  # a half of them below 2^-126
+    q = torch.rand(B, K, V, generator=g, device="cuda") * 2.0 ** -125
+    p[::4, :, ::2] = 0.0
+    x = torch.randint(V, (B, K), generator=g, device="cuda").int()
+    u = torch.rand(B, K + 1, generator=g, device="cuda")
+    compare(p, q, x, u)
+    compare(p, None, x, u)
+    compare(p[:, :1].contiguous(), None, x[:, :0], u[:, :1].contiguous(), ver=Draw(B, V))
 
 
 def test_verify_of_rows_apart_on_another_stream_and_in_a_graph():
