@@ -90,9 +90,10 @@ class SpecVerifier:
             _check(rc, "moe_spec_verify")
 
     def _rows(self, t, what, B, rows):
-        """The distance between the rows of t [B, rows, V], one for all of them."""
+        """The distance between the rows of t [B, rows, V], one for all of them (torch allows any between those of one)."""
         s0, s1, s2 = t.stride()
+        ld = s1 if rows > 1 else (s0 if B > 1 else self.V)
         if t.dtype is not _F32 or t.shape != (B, rows, self.V) or t.get_device() != self._dev \
-                or (s2 != 1 and self.V > 1) or s1 < self.V or (B > 1 and s0 != rows * s1):
+                or (s2 != 1 and self.V > 1) or ld < self.V or (B > 1 and s0 != rows * ld):
             raise ValueError(f"{what}: expected float32 [{B}, {rows}, {self.V}] on {self.device}, rows one distance apart")
-        return s1
+        return ld

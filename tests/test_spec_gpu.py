@@ -383,3 +383,27 @@ def test_a_token_is_drawn_without_drafts(B, V):
         assert np.array_equal(tok.cpu().numpy()[safe], want[safe]) and not bool(acc.any())
         if t == 0:
             assert tok[:, 0].tolist() == z.argmax(-1).tolist()
+
+
+@pytest.mark.parametrize("B", [1, 5])
+def test_one_row_a_sequence_may_lie_anywhere(B):
+    """K = 0 over the first row of several, or over rows padded apart; K = 1 over one draft's row of several: torch gives a
+    dimension of one any stride."""
+    V = 1003
+    g = torch.Generator(device="cuda").manual_seed(B)
+    p = torch.softmax(2 * torch.randn(B, 4, V, generator=g, device="cuda"), -1)
+    u = torch.rand(B, 1, generator=g, device="cuda")
+    empty = torch.zeros(B, 0, dtype=torch.int32, device="cuda")
+    want = run_verify(p[:, :1].contiguous(), None, empty, u, ver=Draw(B, V))[0]
+    padded = torch.full((B, V + 13), 9.0, device="cuda")
+    padded[:, :V] = p[:, 0]
+    for t in (p[:, :1], padded[:, None, :V], padded[:, :V].unsqueeze(1), p[:, 0].contiguous().view(B, 1, V)):
+        assert np.array_equal(run_verify(t, None, empty, u, ver=Draw(B, V))[0], want)
+    q = torch.softmax(2 * torch.randn(B, 3, V, generator=g, device="cuda"), -1)
+    x, u2 = torch.randint(V, (B, 1), generator=g, device="cuda").int(), torch.rand(B, 2, generator=g, device="cuda")
+    t = p[:, :2].contiguous()
+    a, b = run_verify(t, q[:, :1].contiguous(), x, u2), run_verify(t, q[:, :1], x, u2)
+    assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
+    if B > 1:  # two rows of four: not one distance for all
+        with pytest.raises(ValueError):
+            run_verify(p[:, :2], None, x, u2)
