@@ -417,12 +417,12 @@ __global__ void __launch_bounds__(Cfg<D, F8, MT>::kThreads, Cfg<D, F8, MT>::kPer
       return a.q + (((int64_t)w.b * a.Tq + t) * a.Hq + h * a.G + (r - t * a.G)) * D;
     };
     // scores in units of log 2 are S times fA or fB, kept above zero (a masked score is -infinity times it): a negative
-    // scale turns the queries' signs, and one of zero is as good as the smallest factor
-    constexpr float kLeast = 1.1754944e-38f;
+    // scale turns the queries' signs, and one of zero is as good as the smallest factor; a NaN stays one
+    auto above_zero = [](float f) { return f < 1.1754944e-38f ? 1.1754944e-38f : f; };
     float fA = a.scale * 1.4426950408889634f, fB;
     if (a.k_scale) fA *= a.k_scale[h];
     const uint32_t flip = fA < 0.f ? 0x80008000u : 0u;
-    fA = fB = fmaxf(fabsf(fA), kLeast);
+    fA = fB = above_zero(fabsf(fA));
     uint32_t qf[C::kWide ? 1 : D / 16][4];
     auto load_queries = [&](uint32_t (&q)[D / 16][4]) {
       const uint16_t* pA = q_row(rA < M ? rA : 0, rA < M ? tA : 0);
@@ -452,8 +452,8 @@ __global__ void __launch_bounds__(Cfg<D, F8, MT>::kThreads, Cfg<D, F8, MT>::kPer
         const uint32_t eA = min(max(__float_as_uint(quad_max(xA)) >> 23, 1u), 252u);
         const uint32_t eB = min(max(__float_as_uint(quad_max(xB)) >> 23, 1u), 252u);
         const float iA = __uint_as_float((254u - eA) << 23), iB = __uint_as_float((254u - eB) << 23);
-        fA = fmaxf(fA * __uint_as_float(eA << 23), kLeast);  // the product may be too small for a number
-        fB = fmaxf(fB * __uint_as_float(eB << 23), kLeast);
+        fA = above_zero(fA * __uint_as_float(eA << 23));  // the product may be too small for a number
+        fB = above_zero(fB * __uint_as_float(eB << 23));
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
           q[c][0] = pack2<true>(lo_bf(q[c][0]) * iA, hi_bf(q[c][0]) * iA);

@@ -500,6 +500,16 @@ def test_attention_scores_of_any_size():
         assert bool(((vals(out) - want).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("kv,D,Hq,Tq", [("bf16", 64, 4, 1), ("bf16", 256, 16, 1), ("bf16", 256, 16, 4), ("e4m3", 128, 8, 2)])
+def test_attention_with_a_scale_that_is_no_number_is_no_number(kv, D, Hq, Tq):
+    c = filled([130, 9, 0], Hq=Hq, Hkv=2, D=D, page=16, kv=kv, Tq=Tq)
+    q = queries(c, 3, Tq)
+    out = torch.zeros_like(q)
+    c.attend(0, i32([0, 1, 2]), q, out, Tq=Tq, scale=math.nan)
+    got = vals(out).view(3, Tq, -1)
+    assert bool(torch.isnan(got[:2]).all()) and not bool(got[2].any())
+
+
 @pytest.mark.parametrize("D,Hq,Tq", [(64, 4, 1), (128, 8, 2), (256, 4, 1), (256, 16, 4)])
 def test_attention_of_values_near_the_largest_of_their_type(D, Hq, Tq):
     """Even scores, and one key late in the sequence a few powers of two above them whose value is 3e38: the mean is finite,
