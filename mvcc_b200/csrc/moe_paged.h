@@ -15,7 +15,9 @@ namespace moe {
 constexpr int kPagedMaxBatch = 4096;   // list entries of one call
 constexpr int kPagedMaxNew = 8;        // new tokens a sequence that the attention takes
 constexpr int kPagedMaxPages = 1 << 20;
-constexpr int kPagedMaxCtas = 320;     // CTAs of the attention grid at most (its partials are sized by it)
+constexpr int kPagedMaxCtas = 320;     // CTAs of the attention grid at most
+// ... for heads of D values: one an SM for 256, two otherwise. The partials are sized by it.
+__host__ __device__ constexpr int paged_max_ctas(int D) { return D == 256 ? kPagedMaxCtas / 2 : kPagedMaxCtas; }
 
 __host__ __device__ inline int kv_size(int kv_type) { return kv_type == MOE_KV_E4M3 ? 1 : 2; }
 
@@ -58,9 +60,10 @@ inline PagedWs paged_ws(const moe_paged_cache* c, int Hq, int max_batch, int max
   const size_t pages_end = o;
   o = base;
   const int rows = paged_block_rows(Hq / c->Hkv, max_new < kPagedMaxNew ? max_new : kPagedMaxNew);
-  L.joins = o;  o = ws_align(o + 32 * (size_t)kPagedMaxCtas);
-  L.ml = o;     o = ws_align(o + sizeof(float) * 2 * kPagedMaxCtas * 2 * (size_t)rows);
-  L.acc = o;    o = ws_align(o + sizeof(float) * kPagedMaxCtas * 2 * (size_t)rows * c->D);
+  const size_t ctas = paged_max_ctas(c->D);
+  L.joins = o;  o = ws_align(o + 32 * ctas);
+  L.ml = o;     o = ws_align(o + sizeof(float) * 2 * ctas * 2 * rows);
+  L.acc = o;    o = ws_align(o + sizeof(float) * ctas * 2 * rows * c->D);
   L.total = o > pages_end ? o : pages_end;
   return L;
 }

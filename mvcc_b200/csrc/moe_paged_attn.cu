@@ -947,7 +947,8 @@ cudaError_t launch_attn(const PAttnArgs& args, const CUtensorMap& mk, const CUte
   const int smem = C::fixed_bytes(a.B) + a.ns * C::kSlot;
   cudaError_t e = grant_smem(fn, smem, C::kPerSm == 1 ? kSmemOne : kSmemTwo, granted);
   if (e != cudaSuccess) return e;
-  a.ctas = std::min(kPagedMaxCtas, paged_sms() * C::kPerSm);
+  static_assert(paged_max_ctas(D) * 2 == kPagedMaxCtas * C::kPerSm, "the partials' room");
+  a.ctas = std::min(paged_max_ctas(D), paged_sms() * C::kPerSm);
   CUtensorMap k = mk, v = mv;
   void* p[] = {&a, &k, &v};
   e = paged_launch(fn, dim3(a.ctas), dim3(C::kThreads), smem, s, p);

@@ -171,9 +171,10 @@ def inv_frequencies(shape, device="cuda"):
 
 
 class PagedAttnBlock:
-    """The attention branch of one layer for a batch over layer `index` of a paged cache."""
+    """The attention branch of one layer for a batch over layer `index` of a paged cache. Blocks whose calls never overlap,
+    as the layers of one step, may share a workspace: `ws`, another block's."""
 
-    def __init__(self, layer, cache: PagedCache, index: int, inv_freq=None):
+    def __init__(self, layer, cache: PagedCache, index: int, inv_freq=None, ws=None):
         s = layer.shape
         _need(s.Hq == cache.Hq and s.Hkv == cache.Hkv and s.D == cache.D, "layer and cache differ in their heads")
         self.layer, self.cache, self.index = layer, cache, index
@@ -184,8 +185,12 @@ class PagedAttnBlock:
         n = _lib.moe_attn_paged_workspace_bytes(ctypes.byref(layer.c), cache._c, cache.max_batch, cache.max_new)
         if n == 0:
             raise ValueError("unsupported attention geometry")
-        self.ws = torch.zeros(n, dtype=torch.uint8, device=cache.device)
-        torch.cuda.current_stream(cache.device).synchronize()
+        if ws is None:
+            ws = torch.zeros(n, dtype=torch.uint8, device=cache.device)
+            torch.cuda.current_stream(cache.device).synchronize()
+        _need(ws.dtype == torch.uint8 and ws.numel() >= n and ws.is_contiguous() and ws.device == cache.device,
+              f"ws: expected at least {n} contiguous bytes on {cache.device}")
+        self.ws = ws
 
     def error_word(self, stream=None):
         rc = _lib.moe_paged_workspace_error(_ptr(self.ws), self.ws.numel(), raw_stream(self.cache._dev, stream))
@@ -220,7 +225,9 @@ class PagedDecodeStack:
         self.cache = PagedCache.empty(stack.L, num_pages, page, a.Hkv, a.D, a.Hq, max_seqs, max_pages, max_batch,
                                       max_new, kv, k_scale, v_scale, dev)
         f = inv_frequencies(a, dev)
-        self.attn = [PagedAttnBlock(b.layer, self.cache, i, f) for i, b in enumerate(stack.attn)]
+        self.attn = []
+        for i, b in enumerate(stack.attn):  # one after another in a step: one workspace for all
+            self.attn.append(PagedAttnBlock(b.layer, self.cache, i, f, self.attn[0].ws if i else None))
         T = max_batch * max_new
         self.moe = [MoeBlock(b.layer, T) for b in stack.moe]
         self.normed = torch.zeros(T, a.H, dtype=torch.int16, device=dev)
@@ -240,8 +247,8 @@ class PagedDecodeStack:
             lm_head_logits(st.head.w, self.normed[:T], logits, stream)
 
     def error_words(self, stream=None):
-        """The attention blocks' error words, joined (read and cleared)."""
+        """The cache's error word and the one that the attention blocks share, joined (read and cleared)."""
         e = self.cache.error_word(stream)
-        for b in self.attn:
+        for b in self.attn[:1]:
             e |= b.error_word(stream)
         return e

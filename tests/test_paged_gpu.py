@@ -764,6 +764,25 @@ def test_paged_stack_step_follows_the_single_sequence_stack():
                 assert int(logits[slot].argmax()) == int(st.next)
 
 
+def test_the_layers_of_a_paged_stack_share_a_workspace_and_its_error_word():
+    st = small_stack(L=3)
+    ps = P().PagedDecodeStack(st, num_pages=12, page=16, max_seqs=4, max_pages=4, max_batch=3, max_new=2)
+    assert len({b.ws.data_ptr() for b in ps.attn}) == 1
+    seqs = i32([0, 1])
+    ps.cache.resize(seqs, i32([20, 3]))
+    ps.step(torch.randn(2, 1024, device="cuda"), seqs)
+    assert ps.error_words() == 0
+    keep = int(ps.cache.tables[0, 0])
+    ps.cache.tables[0, 0] = -7
+    ps.step(torch.randn(2, 1024, device="cuda"), seqs)
+    assert ps.error_words() == P().ERR_PAGE_ID and ps.error_words() == 0
+    ps.cache.tables[0, 0] = keep
+    with pytest.raises(ValueError):
+        P().PagedAttnBlock(st.attn[0].layer, ps.cache, 0, ws=ps.attn[0].ws[:256])
+    with pytest.raises(ValueError):
+        P().PagedAttnBlock(st.attn[0].layer, ps.cache, 0, ws=ps.attn[0].ws.view(torch.int32))
+
+
 def test_drafts_are_verified_and_rolled_back():
     """A speculative step as it is used: grow by the drafts, step, logits, probabilities, verification, shrink to what
     was accepted; the cache then equals one that never saw the rejected tokens."""

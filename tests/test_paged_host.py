@@ -47,6 +47,13 @@ def test_workspace_bytes():
     assert s(0, 10) == 0 and s(65536, 10) == 0 and s(1, 0) == 0 and s(1, 1 << 24) == 0
 
 
+def test_workspace_holds_one_grid_of_partials():
+    """Two parts a CTA, of 16 rows and their maxima and sums; heads of 256 run one CTA an SM, others two."""
+    n = lib().moe_paged_workspace_bytes
+    for D, ctas in ((256, 160), (128, 320), (64, 320)):
+        assert n(ctypes.byref(cache(D=D)), 16, 8, 1) <= ctas * (2 * 16 * (D + 2) * 4 + 32) + 4096
+
+
 def test_page_calls_refuse_before_launch():
     L, ws, big = lib(), ctypes.c_void_p(PTR), 1 << 40
     c = ctypes.byref(cache())
