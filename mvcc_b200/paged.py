@@ -237,8 +237,10 @@ class PagedDecodeStack:
         """One step for Tq new tokens of each listed sequence (-1: an unused slot): hidden fp32 [B Tq, H] is updated in
         place, and logits fp32 [B Tq, V] are written when given. The cache has been grown to the new lengths
         (cache.resize) beforehand."""
-        from .spec import lm_head_logits
+        from .spec import check_logits, lm_head_logits
         st, T = self.stack, seqs.numel() * Tq
+        if logits is not None:  # refused before a layer has run
+            check_logits(st.head.w, T, logits)
         for i in range(st.L):
             self.attn[i].forward_rms(hidden, st.rms1[i], self.attn_out[:T], seqs, Tq, stream)
             self.moe[i].forward(hidden, self.attn_out[:T], self.normed[:T],

@@ -7,6 +7,12 @@ from . import _check, _lib
 from .paged import _F32, _I32, _need, raw_stream
 
 
+def check_logits(weight, T, logits):
+    """Refuses logits that cannot take T rows of the head `weight`."""
+    _need(logits.dtype == torch.float32 and logits.is_contiguous() and logits.numel() == T * weight.shape[0]
+          and logits.device == weight.device, f"logits: expected contiguous float32 [{T}, {weight.shape[0]}]")
+
+
 def lm_head_logits(weight, normed, logits, stream=None):
     """logits fp32 [T, V] = normed bf16 bits [T, H] . weight^T (bf16 bits [V, H]); the weight is read once for every
     four rows."""
@@ -15,8 +21,7 @@ def lm_head_logits(weight, normed, logits, stream=None):
     dev = weight.device
     _need(weight.dtype == normed.dtype == torch.int16 and weight.is_contiguous() and normed.is_contiguous()
           and normed.numel() == T * H and normed.device == dev, "weight [V, H], normed [T, H]: contiguous bf16 bits")
-    _need(logits.dtype == torch.float32 and logits.is_contiguous() and logits.numel() == T * V and logits.device == dev,
-          f"logits: expected contiguous float32 [{T}, {V}]")
+    check_logits(weight, T, logits)
     s = raw_stream(weight.get_device(), stream)
     for t in range(0, T, 4):
         _check(_lib.moe_lm_head_logits(normed.data_ptr() + t * H * 2, weight.data_ptr(), V, H, min(4, T - t),

@@ -783,6 +783,20 @@ def test_the_layers_of_a_paged_stack_share_a_workspace_and_its_error_word():
         P().PagedAttnBlock(st.attn[0].layer, ps.cache, 0, ws=ps.attn[0].ws.view(torch.int32))
 
 
+def test_a_paged_step_with_logits_that_do_not_fit_changes_nothing():
+    st = small_stack()
+    ps = P().PagedDecodeStack(st, num_pages=12, page=16, max_seqs=4, max_pages=4, max_batch=3, max_new=2)
+    seqs = i32([0, 1])
+    ps.cache.resize(seqs, i32([20, 3]))
+    h = torch.randn(2, 1024, device="cuda")
+    before, k = h.clone(), ps.cache.k.clone()
+    for bad in (torch.zeros(3, st.V, device="cuda"), torch.zeros(2, st.V, device="cuda", dtype=torch.bfloat16),
+                torch.zeros(2, st.V), torch.zeros(st.V, 2, device="cuda").T):
+        with pytest.raises(ValueError):
+            ps.step(h, seqs, logits=bad)
+    assert torch.equal(h, before) and torch.equal(ps.cache.k, k)
+
+
 def test_drafts_are_verified_and_rolled_back():
     """A speculative step as it is used: grow by the drafts, step, logits, probabilities, verification, shrink to what
     was accepted; the cache then equals one that never saw the rejected tokens."""
