@@ -8,7 +8,6 @@ new tokens a sequence. Lists, lengths and tables are device tensors, so a step c
 replayed while the sequences grow. torch is used for device memory and streams only.
 """
 import ctypes
-import dataclasses
 
 import torch
 
@@ -232,6 +231,7 @@ class PagedDecodeStack:
         self.moe = [MoeBlock(b.layer, T) for b in stack.moe]
         self.normed = torch.zeros(T, a.H, dtype=torch.int16, device=dev)
         self.attn_out = torch.zeros(T, a.H, dtype=torch.int16, device=dev)
+        torch.cuda.current_stream(dev).synchronize()  # the zeroing: steps may run on any stream
 
     def step(self, hidden, seqs, Tq=1, logits=None, stream=None):
         """One step for Tq new tokens of each listed sequence (-1: an unused slot): hidden fp32 [B Tq, H] is updated in

@@ -797,6 +797,35 @@ def test_a_paged_step_with_logits_that_do_not_fit_changes_nothing():
     assert torch.equal(h, before) and torch.equal(ps.cache.k, k)
 
 
+def test_a_paged_stack_may_step_on_another_stream_at_once(monkeypatch):
+    """Nothing that its making has launched is still on its way, slow as its zeroing may be."""
+    st = small_stack()
+    zeros = torch.zeros
+
+    def slow_zeros(*a, **kw):
+        torch.cuda._sleep(5000000)  # clocks
+        return zeros(*a, **kw)
+    monkeypatch.setattr(torch, "zeros", slow_zeros)
+    ps = P().PagedDecodeStack(st, num_pages=64, page=16, max_seqs=64, max_pages=4, max_batch=64, max_new=8)
+    assert torch.cuda.current_stream().query()
+    monkeypatch.undo()
+    seqs = i32(list(range(64)))
+    ps.cache.resize(seqs, i32([16] * 64))
+    h, torch_stream = torch.randn(64 * 8, 1024, device="cuda"), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    want, got = h.clone(), h.clone()
+    ps.step(want, seqs, Tq=8)
+    first = ps.normed.clone()
+    torch.cuda.synchronize()
+    again = P().PagedDecodeStack(st, num_pages=64, page=16, max_seqs=64, max_pages=4, max_batch=64, max_new=8)
+    for n in ("k", "v", "tables", "refs", "lens"):
+        getattr(again.cache, n).copy_(getattr(ps.cache, n))
+    torch.cuda.synchronize()
+    again.step(got, seqs, Tq=8, stream=torch_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and torch.equal(again.normed, first)
+
+
 def test_drafts_are_verified_and_rolled_back():
     """A speculative step as it is used: grow by the drafts, step, logits, probabilities, verification, shrink to what
     was accepted; the cache then equals one that never saw the rejected tokens."""
