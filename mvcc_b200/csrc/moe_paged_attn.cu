@@ -594,13 +594,19 @@ __global__ void __launch_bounds__(Cfg<D, F8, MT>::kThreads, Cfg<D, F8, MT>::kPer
         // nearly cancel (the error's mean square over 48 ragged sequences 1.35 times that of the output's rounding alone):
         // what it leaves over goes into a second operand and a second product, 16 bits together. Up to 16 rows a kv head
         // that costs nothing (48 sequences: 68.1 against 69.0 us), with four tokens 83.0 against 81.0, with eight, where
-        // the products bound the call, 146 against 126.
+        // the products bound the call, 146 against 126. The first part is cut off below the weight, never at it, so that
+        // a weight above zero has two parts above zero: an infinite value times them is infinite, not no number.
         uint32_t pf[KT / 16][4], pr[F8 ? 1 : KT / 16][4];
         const float yA = kLift - zA, yB = kLift - zB;
         auto weights = [&](int j, int e, float x, float y) {
-          const uint32_t w = pack2<F8>(x, y);
-          pf[j >> 1][(j & 1) * 2 + e] = w;
-          if constexpr (!F8) pr[j >> 1][(j & 1) * 2 + e] = pack2<false>(x - lo_bf(w), y - hi_bf(w));
+          uint32_t& w = pf[j >> 1][(j & 1) * 2 + e];
+          if constexpr (F8) {
+            w = pack2<true>(x, y);
+          } else {
+            constexpr float kBelow = 1.f - 0x1p-22f;
+            w = __byte_perm(__float_as_uint(x * kBelow), __float_as_uint(y * kBelow), 0x7632);
+            pr[j >> 1][(j & 1) * 2 + e] = pack2<false>(x - lo_bf(w), y - hi_bf(w));
+          }
         };
 #pragma unroll
         for (int j = 0; j < KT / 8; ++j) {

@@ -556,6 +556,27 @@ def test_attention_keeps_more_of_a_weight_than_its_output_shows(D, Hq, Tq):
                 assert bool(((got[b, t, h] - o).abs() <= tol).all()), (b, t, h)
 
 
+@pytest.mark.parametrize("D,Hq,Tq", [(64, 4, 1), (64, 16, 3), (128, 8, 2), (256, 16, 1), (256, 16, 4), (256, 16, 8)])
+def test_attention_of_infinite_values_that_a_row_sees(D, Hq, Tq):
+    """A weight above zero times an infinity is that infinity, whatever the weight's bits (one key alone has a weight of a
+    power of two); the columns beside it and the tokens that do not see it keep theirs."""
+    lens = [1, 8, 40, 300]
+    c = filled(lens, Hq=Hq, Hkv=2, D=D, page=16, Tq=Tq)
+    v = c.v.view(torch.bfloat16)
+    for b, n in enumerate(lens):
+        first, last = int(c.tables[b, 0]), int(c.tables[b, (n - 1) // 16])
+        v[0, first, :, 0, 2] = v[0, first, :, 0, 3] = -math.inf
+        v[0, last, :, (n - 1) % 16, 1] = v[0, last, :, (n - 1) % 16, 3] = math.inf
+    for std in (0.25, 0.0):
+        q = queries(c, len(lens), Tq, std=std)
+        out = torch.zeros_like(q)
+        c.attend(0, i32(list(range(len(lens)))), q, out, Tq=Tq)
+        want, tol = attend64(c, 0, list(range(len(lens))), q, Tq, D ** -0.5, "bf16")
+        got, finite = vals(out), torch.isfinite(want)
+        assert bool(((got - want).abs() <= tol)[finite].all())
+        assert torch.equal(torch.nan_to_num(got[~finite], nan=5.0), torch.nan_to_num(want[~finite], nan=5.0))
+
+
 @pytest.mark.parametrize("D,Hq,Tq", [(128, 4, 1), (128, 8, 3), (256, 4, 3), (256, 16, 8)])
 def test_attention_over_8_bits_with_scores_too_small_to_tell(D, Hq, Tq):
     """A scale of zero with tiny queries, and queries of zero with tiny key scales: equal scores, so a row is the mean of
