@@ -323,6 +323,55 @@ def test_append_to_an_e4m3_cache_rounds_and_saturates():
         assert torch.equal(c.k[0, pid, :, p % 16], want_k[t]) and torch.equal(c.v[0, pid, :, p % 16], want_v[t])
 
 
+@pytest.mark.parametrize("D,Hq,Hkv,rope,Tq", [(128, 6, 2, 64, 5), (128, 4, 1, 128, 700), (256, 16, 2, 64, 3), (256, 2, 2, 256, 301),
+                                             (256, 3, 1, 6, 9), (128, 4, 4, 0, 2)])
+def test_append_with_norm_and_rotation_to_an_e4m3_cache(D, Hq, Hkv, rope, Tq):
+    """Normed and rotated keys, and values, in 64 bits against what is stored. Beside the tolerance of the bf16 cache's test:
+    one more fp32 rounding (the division by the scale) and half a step of e4m3, 2^-4 of the value or 2^-10 scales, up to 448
+    scales, where it saturates."""
+    page, far = 32, 100_000 // 32
+    g = torch.Generator(device="cuda").manual_seed(D + rope)
+    ks = 0.002 + 0.01 * torch.rand(2, Hkv, generator=g, device="cuda")  # keys of up to 4.5 saturate in some heads
+    vs = 0.002 + 0.01 * torch.rand(2, Hkv, generator=g, device="cuda")
+    c = make(layers=2, pages=80, page=page, Hkv=Hkv, D=D, max_seqs=3, max_pages=far, kv="e4m3", Hq=Hq, max_batch=4, max_new=Tq,
+             k_scale=ks, v_scale=vs)
+    lens, seqs, nxt = [Tq, far * page - 5, max(0, Tq - 2)], [1, -1, 0, 2], 0
+    for s, n in enumerate(lens):
+        for j in range(max(0, (n - Tq) // page), -(-n // page)):
+            c.tables[s, j], c.refs[nxt] = nxt, 1
+            nxt += 1
+    c.lens.copy_(i32(lens))
+    T = len(seqs) * Tq
+    qkv = bits(1.5 * torch.randn(T, (Hq + 2 * Hkv) * D, generator=g, device="cuda"))
+    qn, kn = (bits(1 + 0.1 * torch.randn(D, generator=g, device="cuda")) for _ in range(2))
+    f = (1e7 ** (-torch.arange(0, rope, 2, dtype=torch.float64) / rope)).cuda() if rope else None
+    q = torch.full((T, Hq * D), 77, dtype=torch.int16, device="cuda")
+    k0, v0 = c.k.clone(), c.v.clone()
+    c.append(1, i32(seqs), qkv, q, Tq=Tq, q_norm=qn, k_norm=kn, inv_freq=f)
+    assert c.error_word() == 0
+    x = vals(qkv).view(T, Hq + 2 * Hkv, D)
+    pos = torch.tensor([lens[s] - Tq + t if s >= 0 else -1 for s in seqs for t in range(Tq)], device="cuda")
+    live = torch.nonzero(pos >= 0)[:, 0]
+    sid = torch.tensor([max(s, 0) for s in seqs for t in range(Tq)], device="cuda")
+    pid, off = c.tables[sid[live], pos[live] // page].long(), pos[live] % page
+    qe, ke = rotate64(x[:, :Hq], vals(qn), pos, f)[live], rotate64(x[:, Hq:Hq + Hkv], vals(kn), pos, f)[live]
+
+    def size(x, w):  # |x_d| + |x_e| of each rotated pair
+        a = rotate64(x, vals(w), pos, None).abs()
+        h = 0 if f is None else f.numel()
+        both = a[..., :h] + a[..., h:2 * h]
+        return torch.cat([both, both, a[..., 2 * h:]], -1)[live]
+    assert bool(((vals(q).view(T, Hq, D)[live] - qe).abs() <= BF * qe.abs() + 24 * F32 * size(x[:, :Hq], qn) + 1e-30).all())
+    for stored, want, slack, sc in ((c.k, ke, 25 * F32 * size(x[:, Hq:Hq + Hkv], kn), ks), (c.v, x[live, Hq + Hkv:], 0.0, vs)):
+        sc = sc[1].double().view(1, Hkv, 1)
+        got = stored[1, pid, :, off].view(torch.float8_e4m3fn).double() * sc
+        want = torch.minimum(torch.maximum(want, -448 * sc), 448 * sc)
+        tol = torch.maximum(2.0 ** -4 * want.abs(), 2.0 ** -10 * sc) + slack + F32 * want.abs()
+        assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() - tol).max())
+    k0[1, pid, :, off], v0[1, pid, :, off] = c.k[1, pid, :, off], c.v[1, pid, :, off]
+    assert torch.equal(c.k, k0) and torch.equal(c.v, v0)  # nothing else is touched
+
+
 def test_append_skips_shared_and_bad_pages_and_bad_sequences():
     c = make(layers=1, pages=8, page=16, Hkv=2, D=64, max_seqs=4, max_pages=3, Hq=2)
     c.resize(i32([0, 1, 2]), i32([5, 6, 7]))
@@ -739,6 +788,98 @@ def small_stack(L=2, vocab=1000, seed=3):
     from mvcc_b200 import stack as st
     return st.DecodeStack(L=L, ctx=64, vocab=vocab, attn=st.AttnShape(H=1024, Hq=8, Hkv=2),
                           moe=m.MoeShape(H=1024, E=32, TOPK=4, I=256, Is=256, G=64), seed=seed)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("B,Tq", [(5, 1), (3, 3), (16, 4), (64, 1)])
+def test_paged_layer_of_more_rows_than_a_projection_takes_at_once(B, Tq, kv):
+    """The layer for 5, 9 and 64 rows against its formula in 64 bits, rounded to bf16 where the layer stores bf16 (the first
+    projection, the rotated queries, the attention's and the gate's output); its keys and values are those that it left in the
+    cache. The bar is the contiguous layer's."""
+    from mvcc_b200 import stack as st
+    from oracle import oracle as O
+    a = st.AttnShape(gate=True)
+    layer = st.synth_attn_layer(a, seed=23)
+    g = torch.Generator(device="cuda").manual_seed(B)
+    kw = {} if kv == "bf16" else {n: 0.02 + 0.01 * torch.rand(2, a.Hkv, generator=g, device="cuda") for n in ("k_scale", "v_scale")}
+    c = make(layers=2, pages=8 * B, page=32, Hkv=a.Hkv, D=a.D, max_seqs=B, max_pages=8, Hq=a.Hq, max_new=Tq, kv=kv, **kw)
+    lens = [1 + (37 * b + 11) % 250 for b in range(B)]
+    seqs = [(b + 1) % B for b in range(B)]
+    c.resize(i32(list(range(B))), i32(lens))
+    seqs[1] = -1
+    hidden = torch.randn(B * Tq, a.H, generator=g, device="cuda")
+    rms = bits(1 + 0.1 * torch.randn(a.H, generator=g, device="cuda"))
+    blk = P().PagedAttnBlock(layer, c, 1)
+    out = torch.full((B * Tq, a.H), 77, dtype=torch.int16, device="cuda")
+    blk.forward_rms(hidden, rms, out, i32(seqs), Tq=Tq)
+    torch.cuda.synchronize()
+    assert blk.error_word() == 0
+    h, w = hidden.double(), {n: vals(t) for n, t in layer.t.items()}
+    x = h / torch.sqrt((h * h).mean(-1, keepdim=True) + a.eps) * vals(rms)
+    qkv, z = vals(bits(x @ w["qkv"].T)), vals(bits(x @ w["gate"].T))
+    pos = torch.tensor([(lens[s] if s >= 0 else 0) - Tq + t for s in seqs for t in range(Tq)], device="cuda")
+    f = P().inv_frequencies(a)
+    q = bits(rotate64(qkv[:, :a.Hq * a.D].view(-1, a.Hq, a.D), w["q_norm"], pos, f)).view(B * Tq, -1)
+    o = vals(bits(attend64(c, 1, seqs, q, Tq, a.D ** -0.5, kv)[0]))
+    want = vals(bits(o * torch.sigmoid(z))) @ w["o"].T
+    assert O.max_rel_err(vals(out).cpu().numpy(), want.cpu().numpy()) < 1e-2
+    for i in range(B * Tq):  # row by row, so that no row hides behind a larger one
+        if pos[i] >= 0:
+            assert O.max_rel_err(vals(out[i]).cpu().numpy(), want[i].cpu().numpy()) < 2e-2, i
+    if kv == "bf16":
+        for b, s in enumerate(seqs):
+            for t in range(Tq):
+                p = int(pos[b * Tq + t])
+                if s >= 0 and p >= 0:
+                    new = vals(c.v[1, int(c.tables[s, p // 32]), :, p % 32])
+                    assert O.max_rel_err(new.cpu().numpy(), qkv[b * Tq + t].view(-1, a.D)[-a.Hkv:].cpu().numpy()) < 1e-2
+
+
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+@pytest.mark.parametrize("B,Tq", [(3, 1), (3, 2), (6, 3)])
+def test_a_captured_step_of_the_stack_is_replayed_as_the_sequences_grow(B, Tq, kv):
+    """Growth and step captured once and replayed, against the same steps called one by one on a second cache."""
+    st = small_stack()
+    ones = {} if kv == "bf16" else {n: torch.full((st.L, 2), 0.03, device="cuda") for n in ("k_scale", "v_scale")}
+    make_one = lambda: P().PagedDecodeStack(st, num_pages=40, page=16, max_seqs=B, max_pages=6, max_batch=B, max_new=Tq, kv=kv,
+                                            **ones)
+    one, two = make_one(), make_one()
+    seqs, start = i32([-1 if b == 1 else b for b in range(B)]), i32([5 + 13 * b % 40 for b in range(B)])
+    who = i32(list(range(B)))
+    for ps in (one, two):
+        ps.cache.resize(who, start)
+    for n in ("k", "v"):
+        t = getattr(one.cache, n)
+        g = torch.Generator(device="cuda").manual_seed(ord(n))
+        r = torch.randn(t.shape, generator=g, device="cuda")
+        t.copy_(bits(r) if kv == "bf16" else (r * 30).to(torch.float8_e4m3fn).view(torch.uint8))
+        getattr(two.cache, n).copy_(t)
+    g = torch.Generator(device="cuda").manual_seed(B)
+    inputs = [torch.randn(B * Tq, 1024, generator=g, device="cuda") for _ in range(4)]
+    hidden, logits, lens = inputs[0].clone(), torch.zeros(B * Tq, st.V, device="cuda"), start + Tq
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        one.step(hidden.clone(), seqs, Tq=Tq, logits=logits.clone())  # the first use of each kernel, at the old lengths
+        one.cache.k.copy_(two.cache.k)
+        one.cache.v.copy_(two.cache.v)
+        s.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            one.cache.resize(who, lens)
+            one.step(hidden, seqs, Tq=Tq, logits=logits)
+        for i, x in enumerate(inputs):
+            hidden.copy_(x)
+            graph.replay()
+            h2, l2 = x.clone(), torch.zeros_like(logits)
+            two.cache.resize(who, lens)
+            two.step(h2, seqs, Tq=Tq, logits=l2)
+            lens += Tq
+            s.synchronize()
+            assert one.error_words(s) == 0 and two.error_words(s) == 0
+            assert torch.equal(hidden, h2) and torch.equal(logits, l2) and bool(torch.isfinite(l2).all())
+            for n in ("k", "v", "tables", "refs", "lens"):
+                assert torch.equal(getattr(one.cache, n), getattr(two.cache, n)), n
 
 
 def test_paged_stack_step_follows_the_single_sequence_stack():
