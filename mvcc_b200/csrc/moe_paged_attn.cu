@@ -569,11 +569,12 @@ __global__ void __launch_bounds__(Cfg<D, F8, MT>::kThreads, Cfg<D, F8, MT>::kPer
         nB = quad_max(nB);
         // The maximum that the weights refer to moves only when a row's grows by more than kSlack (in units of log 2), for
         // moving it rescales the whole accumulator: with the true maximum, every other tile does for some row of a warp.
-        // A common factor 2^kLift of the weights cancels in the division. bf16 weights take 2^-kSlack, so that none passes
-        // one and a sum of products overflows no earlier than with the true maximum; fp32 and bf16 have the exponents to
-        // spare. f16 weights take 2^11: they end below 2^15, and what a long row's many small weights lose below f16's
-        // normal range stays under 2^-35 of the largest each; e4m3 values leave their sums far from fp32's range.
-        constexpr float kSlack = 4.f, kLift = F8 ? 11.f : -kSlack;
+        // A common factor 2^kLift of the weights cancels in the division. bf16 weights take 2^-24, so that none passes 2^-20
+        // and the sums over a million keys of the type's largest value are finite, as their mean is; fp32 and bf16 have the
+        // exponents to spare (a weight below 2^-102 of the largest is lost). f16 weights take 2^11: they end below 2^15, and
+        // what a long row's many small weights lose below f16's normal range stays under 2^-35 of the largest each; e4m3
+        // values leave their sums far from fp32's range.
+        constexpr float kSlack = 4.f, kLift = F8 ? 11.f : -20.f - kSlack;
         if (__any_sync(0xffffffffu, (nA - mA) * fA > kSlack || (nB - mB) * fB > kSlack)) {
           const float cA = mA == nA ? 1.f : ex2((mA - nA) * fA), cB = mB == nB ? 1.f : ex2((mB - nB) * fB);
           lsum[0] *= cA;

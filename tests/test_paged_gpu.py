@@ -581,6 +581,18 @@ def test_attention_of_values_near_the_largest_of_their_type(D, Hq, Tq):
         assert bool(((vals(out).view(B, Tq, -1) - want).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("D,Hq,Tq,n", [(64, 4, 1, 900), (128, 8, 2, 900), (256, 16, 1, 70_000), (256, 16, 4, 900)])
+def test_attention_of_many_values_near_the_largest_of_their_type(D, Hq, Tq, n):
+    """Rows whose keys all have values of 3e38: their sum is far beyond fp32, their mean is not. And values near the smallest,
+    whose mean is off by no more than attend64 allows for any."""
+    c = filled([n, 33], Hq=Hq, Hkv=2, D=D, page=16, Tq=Tq)
+    q = queries(c, 2, Tq, std=0.5)
+    for size in (3e38, -3e38, 1e-37):
+        c.v.view(torch.bfloat16).fill_(size)
+        out = check_attend(c, [0, 1], Tq, q=q)
+        assert bool(torch.isfinite(vals(out)).all())
+
+
 @pytest.mark.parametrize("D,Hq,Tq", [(64, 4, 1), (64, 16, 3), (128, 8, 1), (128, 32, 4), (256, 16, 1), (256, 16, 4), (256, 16, 8)])
 def test_attention_keeps_more_of_a_weight_than_its_output_shows(D, Hq, Tq):
     """Rows of values that nearly cancel, where a weight of 8 bits would show: within the output's rounding (2^-8 of it) and
