@@ -26,10 +26,12 @@
 // the softmax of each tile. At 64 rows that no longer holds: there the register MMAs bound the call.
 //
 // Measured on a B200 (16 query and 2 kv heads of 256, bf16, unless said otherwise; the device copy moves 6.45 TB/s): one
-// sequence of 131071 keys 51 us (5.3 TB/s), 48 ragged sequences of up to 8192 keys 68 us (5.5 TB/s), with 4 and 8 new
-// tokens each 83 and 146 us; 24 sequences of up to 16000 keys, 32 over 8 heads of 128, 4 tokens: 123 us in bf16
-// (5.9 TB/s), 69 us in e4m3 with pages of 16 (5.2 TB/s). The loop over the tiles runs at the read bandwidth for bf16 and
-// one row tile; around it lie 2 us for the units, 1.5 us for the first queries and pages, 2 us for the last merge, 1 to
+// sequence of 131071 keys 51 us (5.3 TB/s), 48 ragged sequences of up to 8192 keys 69 us (5.4 TB/s), with 4 and 8 new
+// tokens each 83 and 147 us, over e4m3 49, 81 and 143 us; 24 sequences of up to 16000 keys, 32 over 8 heads of 128, 4
+// tokens, pages of 16: 124 us in bf16 (5.8 TB/s), 70 us in e4m3 (5.1 TB/s). The batch's tables take room from the ring: 8
+// over 2 heads of 128, 260000 keys in all, 52 us for 256 sequences (12 slots), 71 for 1024 (8 slots, and jobs of
+// 256 keys on average), 184 for 4096 (4 slots, jobs of 64 keys). The loop over the tiles runs at the read bandwidth for
+// bf16 and one row tile; around it lie 2 us for the units, 1.5 us for the first queries and pages, 2 us for the last merge, 1 to
 // 4 us for the slowest CTA and 3 us for the join. With e4m3 the consumers' latency a tile (2000 cycles, two warps a
 // scheduler) bounds it, with four row tiles their products, and the k and v fragments that every row tile loads again.
 #include <algorithm>
@@ -595,7 +597,7 @@ __global__ void __launch_bounds__(Cfg<D, F8, MT>::kThreads, Cfg<D, F8, MT>::kPer
         // nearly cancel (the error's mean square over 48 ragged sequences 1.35 times that of the output's rounding alone):
         // what it leaves over goes into a second operand and a second product, 16 bits together. Up to 16 rows a kv head
         // that costs nothing (48 sequences: 68.1 against 69.0 us), with four tokens 83.0 against 81.0, with eight, where
-        // the products bound the call, 146 against 126. The first part is cut off below the weight, never at it, so that
+        // the products bound the call, 146 against 126. Over e4m3 the 11 bits leave 1.0015 times the rounding's error. The first part is cut off below the weight, never at it, so that
         // a weight above zero has two parts above zero: an infinite value times them is infinite, not no number.
         uint32_t pf[KT / 16][4], pr[F8 ? 1 : KT / 16][4];
         const float yA = kLift - zA, yB = kLift - zB;
