@@ -120,14 +120,15 @@ MOE_API int moe_paged_append(const moe_paged_cache* c, int layer, const int32_t*
 
 /* Causal attention of the new tokens over the cached keys and values of layer `layer`, theirs included: query head h
  * reads kv head h / (Hq / Hkv), softmax(scale q . k) . v, out bf16 [B Tq][Hq D]. Scores, the softmax and all sums are
- * fp32. The weights enter their product with v as two bf16 parts (16 bits of each), over an e4m3 cache as f16 (11 bits);
- * there the queries are f16 too, scaled by the power of two that brings the largest of a head's to [1, 2): exact down to
- * 2^-17, off by 2^-25 at most below. Sums stay finite over 2^20 keys of the type's largest value. Rows of unused slots,
- * of empty sequences and of no token are zero. What lies in a page behind a sequence's end, and what a token may not
- * see, has no influence, NaN and infinities included. G = Hq / Hkv any whole number with Hq <= 128; Tq <= 8; B <= 4096;
- * B Hkv ceil(G Tq / 64) max_pages page at most 2^34 (the work is counted in 32 bits); q, out 16-byte aligned. The
- * batch's work is shared out over the GPU by keys, whatever the lengths, and the parts of a sequence joined in order:
- * the same call gives the same bits. */
+ * fp32. The weights enter their product with v as two bf16 parts (16 bits of each), over an e4m3 cache as f16 (11
+ * bits, or 2^-36 of the row's largest weight where that is more); there the queries are f16 too, scaled by the power
+ * of two that brings the largest of a head's to [1, 2): exact down to 2^-17, off by 2^-25 at most below. Sums stay
+ * finite over 2^20 keys of the type's largest value. Rows of unused slots, of empty sequences and of no token are
+ * zero. What lies in a page behind a sequence's end, and what a token may not see, has no influence, NaN and
+ * infinities included. G = Hq / Hkv any whole number with Hq <= 128; Tq <= 8; B <= 4096; B Hkv ceil(G Tq / 64)
+ * max_pages page at most 2^34 (the work is counted in 32 bits); q, out 16-byte aligned. The batch's work is shared out
+ * over the GPU by keys, whatever the lengths, and the parts of a sequence joined in order: the same call gives the
+ * same bits. */
 MOE_API int moe_paged_attend(const moe_paged_cache* c, int layer, const int32_t* seqs, int B, int Tq,
                              const uint16_t* q, int Hq, float scale, uint16_t* out, void* workspace,
                              size_t workspace_bytes, moe_stream_t stream);

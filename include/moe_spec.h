@@ -26,7 +26,8 @@ MOE_API int moe_lm_head_logits(const uint16_t* normed, const uint16_t* lm_head, 
  * fp32 [R] (NULL = 1): a row with t_r = 0 (or negative or NaN) puts everything on its largest logit, the lowest index
  * of a tie, and an infinite one shares equally. NaN logits and -infinity get probability zero (a NaN never wins, as in
  * moe_lm_head_argmax); +infinity takes all (shared by several); a row with no logit above -infinity is all zeros. probs
- * may be logits itself (with the same ld), but not overlap it otherwise. 1 <= V < 2^24, R >= 0. */
+ * may be logits itself (with the same ld), but not overlap it otherwise. 1 <= V < 2^24, R >= 0. All in fp32: a probability's
+ * relative error stays below 2^-20 + 2^-21 (1 + (m - x_v) / t_r). */
 MOE_API int moe_softmax_rows(const float* logits, int64_t ld_logits, int R, int V, const float* temperature,
                              float* probs, int64_t ld_probs, moe_stream_t stream);
 
